@@ -171,6 +171,71 @@ SMA_API int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const 
                                  void* dv, int64_t B, int64_t H, int64_t N, int64_t D, float scale, void* stream);
 
 /*
+ * Arguments of the entry points for queries and keys of different lengths
+ * (sma_rows_attn_fwd and its companions below).  Zero-initialise it; fields
+ * that an operator does not use stay 0.
+ *
+ *   q [B, H, Nq, D], k and v [B, Hkv, Nk, D], H % Hkv == 0: query head h
+ *   reads key head h / (H / Hkv).  Strides are in elements, for the batch,
+ *   head and row axes; the last axis is contiguous.  Base addresses and the
+ *   strides of axes longer than 1 are multiples of 16 bytes (strides > 0).
+ *
+ *   mask: bool bytes (non-zero = attend) at mask + b*mask_stride[0] +
+ *   h*mask_stride[1] + i*mask_stride[2] + j, a stride of 0 for an axis the
+ *   mask does not depend on; NULL keeps every key.
+ *
+ *   lengths (device int32 [B], or NULL): instead of a mask, the queries are
+ *   the last Nq of the first lengths[b] keys and see keys up to themselves:
+ *   query i keeps key j iff j < lengths[b] - Nq + 1 + i.  Lengths are
+ *   clamped to [0, Nk].
+ *
+ *   k_prefix, v_prefix [Hkv, P, D] (strides for head and row): P more keys in
+ *   front of the others, the same for the whole batch, kept by every query.
+ *
+ *   bias: adds bias_table[bucket, h] (of `dtype`, [bias_buckets, H],
+ *   contiguous) to the scaled score of query i and key j, bucket being that
+ *   of the relative position d = j - i - offset.  One-sided: the last of the
+ *   bias_side entries of bias_starts (host array, ascending from 0) that is
+ *   <= max(-d, 0).  Two-sided: that of |d|, plus bias_side where d > 0.
+ *   offset is bias_offset, or bias_offsets[b] (device int32 [B]) if given.
+ */
+#define SMA_MAX_BIAS_SIDE 128
+typedef struct sma_attn_args {
+  int32_t dtype;
+  float scale;
+  int64_t B, H, Hkv, Nq, Nk, D, P;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const void *k_prefix, *v_prefix;
+  int64_t kp_stride[2], vp_stride[2];
+  const void* mask;
+  int64_t mask_stride[3];
+  const int32_t* lengths;
+  const void* bias_table;
+  const int32_t* bias_starts;
+  const int32_t* bias_offsets;
+  int64_t bias_offset;
+  int32_t bias_side;
+  int32_t bias_two_sided;
+  void* out;   /* [B, H, Nq, D] contiguous */
+  float* lse;  /* [B, H, Nq] natural-log sum of exponentials, or NULL */
+} sma_attn_args;
+
+/*
+ * Attention forward for few query rows per key head (a generated token, a
+ * few drafted ones): each (batch, key head)'s rows are taken 16 at a time
+ * against keys streamed once, split along keys over the SMs when there are
+ * few rows.  Any Nq works; the keys are read again for every 16 rows.
+ * Takes a bool mask (not packed), lengths, a shared prefix and a bias.  Rows
+ * that keep no key get out = 0 and lse = -FLT_MAX.  Keys that none of the 16
+ * rows keeps may hold any values.  D in {64, 128}, scale finite and > 0,
+ * P and Nk up to 2^30, |bias_offset| < 2^30.  Scratch for the split comes
+ * from the library's stream-ordered pool.
+ * No reference counterpart.
+ */
+SMA_API int sma_rows_attn_fwd(const sma_attn_args* args, void* stream);
+
+/*
  * Synchronise `stream`, then report whether any kernel of this library on the
  * current device gave up a bounded device-side wait since the last clear
  * (SMA_ERR_TIMEOUT), or whether the stream holds a CUDA error (SMA_ERR_CUDA).

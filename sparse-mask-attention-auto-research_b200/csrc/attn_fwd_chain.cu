@@ -144,19 +144,6 @@ struct SplitParams {
   unsigned long long epoch;  // distinct per launch, < 2^56, never 0
 };
 
-// Counts one finished piece of an item; a counter left by an earlier launch
-// (another epoch, or whatever the memory held) counts as zero, so counters
-// need no clearing.  True for the piece that completes the item.
-__device__ __forceinline__ bool claim_last_piece(unsigned long long* cnt, unsigned long long epoch, int pieces) {
-  unsigned long long cur = *reinterpret_cast<volatile unsigned long long*>(cnt);
-  for (;;) {
-    const unsigned long long want = ((cur >> 8) == epoch) ? cur + 1ull : ((epoch << 8) | 1ull);
-    const unsigned long long prev = atomicCAS(cnt, cur, want);
-    if (prev == cur) return static_cast<int>(want & 0xFFull) == pieces;
-    cur = prev;
-  }
-}
-
 template <int D>
 constexpr size_t smem_bytes() {
   return 2 * static_cast<size_t>(ChainCfg<D>::kChainBytes) + sizeof(Ctl);

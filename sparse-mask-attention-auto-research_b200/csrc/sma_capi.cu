@@ -102,6 +102,103 @@ int noalloc_scratch(float** out) {
   return sma::kOk;
 }
 
+
+// Checks of the arguments that every entry point on sma_attn_args shares;
+// fills `p`.  Sets `*empty` when there is nothing to write.
+int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool* empty) {
+  *empty = false;
+  if (a == nullptr) return fail(sma::kErrArg, "attention: null arguments");
+  if (a->dtype != SMA_DTYPE_FP16 && a->dtype != SMA_DTYPE_BF16)
+    return fail(sma::kErrDtype, "attention: unsupported dtype, need fp16 or bf16");
+  constexpr int64_t kMax = int64_t{1} << 30;
+  if (a->B < 0 || a->H < 0 || a->Hkv < 0 || a->Nq < 0 || a->Nk < 0 || a->P < 0 || a->D <= 0)
+    return fail(sma::kErrArg, "attention: bad dimension");
+  if (a->D != 64 && a->D != 128) return fail(sma::kErrUnsupportedD, "attention: head dim must be 64 or 128");
+  if (a->Nq > kMax || a->Nk > kMax || a->P > kMax)
+    return fail(sma::kErrUnsupportedN, "attention: sequence length above 2^30");
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(sma::kErrArg, "attention: scale must be finite and > 0");
+  if (a->B == 0 || a->H == 0 || a->Nq == 0) {
+    *empty = true;
+    return sma::kOk;
+  }
+  if (a->B > kMax || a->H > kMax || a->Hkv == 0 || a->H % a->Hkv != 0)
+    return fail(sma::kErrArg, "attention: the key heads must divide the query heads");
+  if (!a->q || !a->out || (a->Nk > 0 && (!a->k || !a->v)) || (a->P > 0 && (!a->k_prefix || !a->v_prefix)))
+    return fail(sma::kErrArg, "attention: null pointer");
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_prefix) || !aligned16(a->v_prefix) ||
+      !aligned16(a->out))
+    return fail(sma::kErrArg, "attention: q/k/v/out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a->lse) & 3u) return fail(sma::kErrArg, "attention: lse must be 4-byte aligned");
+  // Strides of axes that are stepped along: positive multiples of 16 bytes (8 elements).
+  auto strides_ok = [](const int64_t* s, const int64_t* n, int axes) {
+    for (int i = 0; i < axes; ++i)
+      if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 != 0 || s[i] >= (int64_t{1} << 38))) return false;
+    return true;
+  };
+  const int64_t nq[3] = {a->B, a->H, a->Nq}, nk[3] = {a->B, a->Hkv, a->Nk}, npre[2] = {a->Hkv, a->P};
+  if (!strides_ok(a->q_stride, nq, 3) || (a->Nk > 0 && (!strides_ok(a->k_stride, nk, 3) || !strides_ok(a->v_stride, nk, 3))) ||
+      (a->P > 0 && (!strides_ok(a->kp_stride, npre, 2) || !strides_ok(a->vp_stride, npre, 2))))
+    return fail(sma::kErrArg, "attention: strides must be positive multiples of 8 elements");
+  if (a->mask && a->lengths) return fail(sma::kErrArg, "attention: give a mask or lengths, not both");
+  if (reinterpret_cast<uintptr_t>(a->lengths) & 3u) return fail(sma::kErrArg, "attention: lengths must be 4-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (a->mask && a->mask_stride[i] < 0) return fail(sma::kErrArg, "attention: negative mask stride");
+  if (a->bias_table) {
+    if (a->P > 0) return fail(sma::kErrArg, "attention: no bias together with a prefix");
+    if (a->bias_side < 1 || a->bias_side > SMA_MAX_BIAS_SIDE || !a->bias_starts)
+      return fail(sma::kErrArg, "attention: a bias needs 1 to 128 bucket starts for a side");
+    if (a->bias_offset <= -kMax || a->bias_offset >= kMax) return fail(sma::kErrArg, "attention: bias offset out of range");
+    if ((reinterpret_cast<uintptr_t>(a->bias_table) & 1u) || (reinterpret_cast<uintptr_t>(a->bias_offsets) & 3u))
+      return fail(sma::kErrArg, "attention: misaligned bias table or offsets");
+    for (int i = 0; i < a->bias_side; ++i)
+      if (a->bias_starts[i] < 0 || (i == 0 ? a->bias_starts[0] != 0 : a->bias_starts[i] < a->bias_starts[i - 1]))
+        return fail(sma::kErrArg, "attention: bucket starts must ascend from 0");
+  }
+  uint32_t* err = nullptr;
+  const int rc = error_word(&err);
+  if (rc != sma::kOk) return rc;
+  p->dtype = a->dtype;
+  p->q = a->q;
+  p->k = a->k;
+  p->v = a->v;
+  p->k_prefix = a->k_prefix;
+  p->v_prefix = a->v_prefix;
+  for (int i = 0; i < 3; ++i) {
+    p->q_stride[i] = a->q_stride[i];
+    p->k_stride[i] = a->k_stride[i];
+    p->v_stride[i] = a->v_stride[i];
+    p->mask_stride[i] = a->mask_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    p->kp_stride[i] = a->kp_stride[i];
+    p->vp_stride[i] = a->vp_stride[i];
+  }
+  p->mask = static_cast<const uint8_t*>(a->mask);
+  p->lengths = a->lengths;
+  p->bias.table = a->bias_table;
+  p->bias.offsets = a->bias_offsets;
+  p->bias.offset = static_cast<int>(a->bias_offset);
+  p->bias.H = static_cast<int>(a->H);
+  p->bias.side = a->bias_side;
+  p->bias.two_sided = a->bias_two_sided != 0;
+  if (a->bias_table)
+    for (int i = 0; i < a->bias_side; ++i) p->bias.starts[i] = a->bias_starts[i];
+  p->out = a->out;
+  p->lse = a->lse;
+  p->B = a->B;
+  p->H = a->H;
+  p->Hkv = a->Hkv;
+  p->Nq = a->Nq;
+  p->Nk = a->Nk;
+  p->D = a->D;
+  p->P = a->P;
+  p->scale = a->scale;
+  p->err_word = err;
+  p->timeout_ns = g_timeout_ns.load(std::memory_order_relaxed);
+  p->stream = static_cast<cudaStream_t>(stream);
+  return sma::kOk;
+}
+
 }  // namespace
 
 extern "C" {
@@ -279,6 +376,17 @@ int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const void* v,
   if (rc != sma::kOk) return rc;
   return sma_attn_bwd(dtype, q, k, v, out, dout, lse, mask_packed, dq, dk, dv, scratch, scratch + B * H * N * D, B,
                       H, N, D, scale, stream);
+}
+
+int sma_rows_attn_fwd(const sma_attn_args* args, void* stream) {
+  NvtxRange range("sma_rows_attn_fwd");
+  sma::CrossParams p{};
+  bool empty = false;
+  int rc = cross_params(args, stream, &p, &empty);
+  if (rc != sma::kOk || empty) return rc;
+  const char* msg = nullptr;
+  rc = sma::launch_attn_rows(p, &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
 }
 
 int sma_device_status(void* stream, int clear) {

@@ -83,11 +83,59 @@ struct BwdParams {
 // Backward (attn_bwd.cu): head dims 64 and 128.
 int launch_attn_bwd(const BwdParams& p, const char** msg);
 
+// Learned bias by bucketed relative position (rel_bias.cuh has the device side).
+constexpr int kMaxBiasSide = 128;
+// Relative positions are kept within +-2^30 (sequence lengths and offsets are
+// bounded below that), so int arithmetic on them cannot overflow.
+constexpr int kMaxBiasOffset = 1 << 30;
+
+struct BiasSpec {
+  const void* table;       // [buckets, H] of the inputs' type, or nullptr: no bias
+  const int32_t* offsets;  // [B] query offsets, or nullptr: `offset` for all
+  int offset;
+  int H;
+  int side;                // buckets of one side
+  int two_sided;
+  int starts[kMaxBiasSide];  // smallest distance of each of them, ascending from 0
+};
+
+// Attention of queries and keys of different lengths: q [B, H, Nq, D], k and v
+// [B, Hkv, Nk, D] (strides in elements, last axis contiguous), Hkv dividing H.
+struct CrossParams {
+  int dtype;  // 0 = fp16, 1 = bf16
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];  // batch, head, row
+  const void* k_prefix;       // [Hkv, P, D] keys in front, shared by the batch
+  const void* v_prefix;
+  int64_t kp_stride[2], vp_stride[2];  // head, row
+  const uint8_t* mask;        // bool bytes, or nullptr
+  int64_t mask_stride[3];     // batch, head, query (0: broadcast)
+  const int32_t* lengths;     // [B] or nullptr: query i keeps key j < lengths[b] - Nq + 1 + i
+  BiasSpec bias;
+  void* out;                  // [B, H, Nq, D] contiguous
+  float* lse;                 // [B, H, Nq] or nullptr
+  int64_t B, H, Hkv, Nq, Nk, D, P;
+  float scale;
+  uint32_t* err_word;
+  uint64_t timeout_ns;
+  cudaStream_t stream;
+};
+
+// Few query rows per key head (attn_rows.cu): head dims 64 and 128.
+int launch_attn_rows(const CrossParams& p, const char** msg);
+
 // TMA map of the [BH, N, D] view of a contiguous [B, H, N, D] fp16/bf16
 // tensor: boxes of 64 head dims (one 128-byte swizzle span) by `rows` rows,
 // 128-byte swizzle (tma_map.cu).  Returns the driver's status
 // (CUDA_ERROR_NOT_FOUND when the entry point is missing).
 CUresult make_tensor_map_3d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t BH, int64_t N, int rows);
+// TMA map of a [B, H, N, D] fp16/bf16 view with element strides {batch, head,
+// row}: boxes of 64 head dims by `rows` rows, 128-byte swizzle; coordinates
+// (d, row, head, batch).
+CUresult make_tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t N, int64_t H, int64_t B,
+                            const int64_t* stride, int rows);
 // The same view of a contiguous FP32 [BH, N, D] tensor: boxes of 32 elements
 // (128 bytes) by `rows` rows, 128-byte swizzle (tma_map.cu).
 CUresult make_tensor_map_3d_f32(CUtensorMap* m, const void* ptr, int64_t D, int64_t BH, int64_t N, int rows);

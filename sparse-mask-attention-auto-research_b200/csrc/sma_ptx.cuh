@@ -129,6 +129,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
+// 4-D tiled load global -> shared.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
 // 3-D tiled store shared -> global (bulk-group completion).
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src, int c0, int c1,
                                              int c2) {
@@ -201,6 +211,20 @@ __device__ __forceinline__ uint32_t ld_global_u32(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+
+// ---------------------------------------------------------------- split along keys
+// Counts one finished piece of an item; a counter left by an earlier launch
+// (another epoch, or whatever the memory held) counts as zero, so counters
+// need no clearing.  True for the piece that completes the item.
+__device__ __forceinline__ bool claim_last_piece(unsigned long long* cnt, unsigned long long epoch, int pieces) {
+  unsigned long long cur = *reinterpret_cast<volatile unsigned long long*>(cnt);
+  for (;;) {
+    const unsigned long long want = ((cur >> 8) == epoch) ? cur + 1ull : ((epoch << 8) | 1ull);
+    const unsigned long long prev = atomicCAS(cnt, cur, want);
+    if (prev == cur) return static_cast<int>(want & 0xFFull) == pieces;
+    cur = prev;
+  }
 }
 
 // ---------------------------------------------------------------- tcgen05

@@ -70,6 +70,22 @@ CUresult make_tensor_map_3d(CUtensorMap* m, const void* ptr, int dtype, int64_t 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
+CUresult make_tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t N, int64_t H, int64_t B,
+                            const int64_t* stride, int rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return CUDA_ERROR_NOT_FOUND;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(H),
+                        static_cast<cuuint64_t>(B)};
+  // The stride of an axis of length 1 is never used; any valid one will do.
+  auto bytes = [&](int64_t n, int64_t s) { return static_cast<cuuint64_t>((n > 1 ? s : D) * 2); };
+  cuuint64_t strides[3] = {bytes(N, stride[2]), bytes(H, stride[1]), bytes(B, stride[0])};
+  cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(rows), 1u, 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 // FP32 [BH][N][D] tensor, boxes of 32 elements (128 bytes, 128-byte swizzle)
 // by `rows` rows.
 CUresult make_tensor_map_3d_f32(CUtensorMap* m, const void* ptr, int64_t D, int64_t BH, int64_t N, int rows) {

@@ -28,6 +28,8 @@ asynchronously, like the reference.
 """
 
 import contextlib
+import ctypes
+import typing
 
 import torch
 
@@ -201,6 +203,76 @@ def backward(dout, q, k, v, out, lse, mask_packed, dq, dk, dv, scale):
                 dq_accum.data_ptr(), delta.data_ptr(), B, H, N, D, float(scale), _stream_ptr(q.device),
             )
         )
+
+
+def _strided(t):
+    """`t`, or a contiguous copy of it where the kernels cannot step along its
+    strides (last axis contiguous, the others positive multiples of 16 bytes,
+    a 16-byte aligned base)."""
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], st[:-1])
+    ):
+        return t
+    return t.contiguous()
+
+
+def _mask_strides(mask, shape):
+    """`mask` with a contiguous last axis, and its strides (0 where it is
+    broadcast) along the first three axes of `shape` ([B, H, Nq, Nk])."""
+    if mask.shape[3] > 1 and mask.stride(3) != 1:
+        mask = mask.contiguous()
+    return mask, tuple(0 if n == 1 else s for n, s in zip(mask.shape[:3], mask.stride()[:3]))
+
+
+class Bias(typing.NamedTuple):
+    """A relative position bias for the kernels."""
+
+    table: torch.Tensor  # [buckets, H]
+    starts: ctypes.Array  # one side's bucket starts
+    two_sided: bool
+    offset: int
+    offsets: typing.Optional[torch.Tensor]  # int32 [B], or None: offset for all
+
+
+def _attn_args(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None):
+    """sma_attn_args of checked tensors (see include/sma_capi.h), and what it
+    points to that has to outlive the call."""
+    B, H, Nq, D = q.shape
+    Hkv, Nk = k.shape[1:3]
+    mask_ptr, mask_st = None, (0, 0, 0)
+    if mask is not None:
+        mask, mask_st = _mask_strides(mask, (B, H, Nq, Nk))
+        mask_ptr = mask.data_ptr()
+    kp = vp = kp_st = None
+    P = 0
+    if prefix is not None:
+        kp, vp = prefix
+        P = kp.shape[1]
+    table, starts, two_sided, offset, offsets = bias if bias is not None else (None, None, 0, 0, None)
+    raw = _lib.ATTN_ARGS.pack(
+        _DTYPES[q.dtype], scale, B, H, Hkv, Nq, Nk, D, P, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
+        *k.stride()[:3], *v.stride()[:3], *((kp.data_ptr(), vp.data_ptr(), *kp.stride()[:2], *vp.stride()[:2])
+                                           if P else (0, 0, 0, 0, 0, 0)),
+        mask_ptr or 0, *mask_st, 0 if lengths is None else lengths.data_ptr(), 0 if table is None else table.data_ptr(),
+        0 if starts is None else ctypes.addressof(starts), 0 if offsets is None else offsets.data_ptr(), offset,
+        0 if starts is None else len(starts), int(two_sided), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+    )
+    return raw, mask
+
+
+def rows_forward(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None):
+    """Attention of a few query rows per key head (sma_rows_attn_fwd): q
+    [B, H, Nq, D], k and v [B, Hkv, Nk, D], a bool ``mask`` that broadcasts to
+    [B, H, Nq, Nk] or int32 ``lengths`` [B], a shared ``prefix`` (k, v)
+    [Hkv, P, D] and a ``bias``.  Writes ``out`` and, unless None, ``lse``.
+    The callers (cross_attention.py) check the arguments."""
+    args, _keep = _attn_args(q, k, v, out, lse, scale, mask, lengths, prefix, bias)
+    lib = _lib.load()
+    with _device_guard(q.device):
+        _lib.check(lib.sma_rows_attn_fwd(args, _stream_ptr(q.device)))
 
 
 def pack_mask(mask):
