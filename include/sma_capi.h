@@ -200,6 +200,9 @@ SMA_API int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const 
  *   offset is bias_offset, or bias_offsets[b] (device int32 [B]) if given.
  */
 #define SMA_MAX_BIAS_SIDE 128
+#define SMA_MAX_BIAS_DISTANCE 65536 /* largest last start, where bias_distance is used */
+/* Floats per head of bias_distance, `last` being the last bucket's start. */
+#define SMA_BIAS_DISTANCE_LEN(last, two_sided) (((two_sided) ? 2 : 1) * (int64_t)(last) + 1 + 512)
 typedef struct sma_attn_args {
   int32_t dtype;
   float scale;
@@ -219,6 +222,9 @@ typedef struct sma_attn_args {
   int32_t bias_two_sided;
   void* out;   /* [B, H, Nq, D] contiguous */
   float* lse;  /* [B, H, Nq] natural-log sum of exponentials, or NULL */
+  const void* words;      /* mask packed by sma_pack_mask_rows */
+  int64_t word_stride[3];
+  float* bias_distance;   /* room for H * SMA_BIAS_DISTANCE_LEN floats */
 } sma_attn_args;
 
 /*
@@ -234,6 +240,36 @@ typedef struct sma_attn_args {
  * No reference counterpart.
  */
 SMA_API int sma_rows_attn_fwd(const sma_attn_args* args, void* stream);
+
+/*
+ * Packs a bool mask [Bm, Hm, Qm, Nk] with the given batch, head and query
+ * strides (bytes, >= 0; the last axis contiguous) into words [Bm, Hm, Qm, W],
+ * W = 4 * ceil(Nk / 128), contiguous: bit b of word w of a row is the mask at
+ * column 32 w + b, 0 at columns >= Nk.  `words` is 16-byte aligned.
+ * No reference counterpart (the reference's masks are square and dense).
+ */
+SMA_API int sma_pack_mask_rows(const void* mask, const int64_t* stride, void* words, int64_t Bm, int64_t Hm, int64_t Qm,
+                               int64_t Nk, void* stream);
+
+/*
+ * Attention forward for many query rows, on 128-row tiles: `words` (with
+ * word_stride, 0 for an axis the mask does not depend on; NULL keeps every
+ * key) takes the place of `mask`, and a bias also needs bias_distance, which
+ * is filled here (the backward reads it).  Queries of the heads that share a
+ * key head fill a tile together when Nq <= 64.  Nk <= SMA_MAX_SEQ_LEN, no
+ * prefix; otherwise as sma_rows_attn_fwd, except that a key which only some
+ * rows of a tile keep must hold finite values (a key that a mask row shared
+ * by the tile, or the length, leaves out may hold anything).
+ * Rows that keep no key get out = 0 and lse = -FLT_MAX.
+ */
+SMA_API int sma_cross_attn_fwd(const sma_attn_args* args, void* stream);
+
+/*
+ * Attention behind a prefix shared by the batch, the prefix read once for all:
+ * its tiles hold the rows of several sequences.  P > 0, Nk <= SMA_MAX_SEQ_LEN,
+ * `lengths` or nothing for the sequences' own keys, no mask, no bias, no lse.
+ */
+SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
 
 /*
  * Synchronise `stream`, then report whether any kernel of this library on the

@@ -44,7 +44,7 @@
 namespace sma {
 namespace {
 
-constexpr int kRows = 16;    // rows of a tile (one m16n8k16 fragment)
+constexpr int kRows = kRowsTile;  // one m16n8k16 fragment
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 32;   // keys a warp takes at a time
@@ -62,6 +62,8 @@ struct RowsParams {
   const int32_t* lengths;
   uint16_t* out;
   float* lse;
+  float* part_ml;          // every row as a piece for a later merge instead of out / lse (CrossParams)
+  float* part_o;
   float* ws;               // [units][16][4] (max, sum, sum of rounded P, -), then [units][16][D]
   unsigned long long* cnt;  // [items]: launch epoch << 8 | pieces finished
   unsigned long long epoch;
@@ -469,20 +471,25 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
   if (ctl.abort_flag != 0u) return;
   const int rows = min(kRows, p.R - rt * kRows);
   constexpr int kVec = D / 4;  // float4 per row
-  // Writes row r's column group x: final (normalised, the inputs' type) or as
-  // a piece of the item (FP32, not normalised).
+  // Writes row r's column group x: normalised, in the inputs' type, or as a
+  // piece for a later merge (FP32, not normalised).
   auto write_out = [&](int r, int x, const float4& a, float inv) {
     const int rr = rt * kRows + r;
     const int g = rr / p.Nq;
+    if (p.part_o != nullptr) {
+      float* dst = p.part_o + ((static_cast<int64_t>(b) * p.H + hkv * p.G + g) * p.Nq + (rr - g * p.Nq)) * D + 4 * x;
+      *reinterpret_cast<float4*>(dst) = a;
+      return;
+    }
     uint16_t* dst = p.out + ((static_cast<int64_t>(b) * p.H + hkv * p.G + g) * p.Nq + (rr - g * p.Nq)) * D + 4 * x;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(a.x * inv, a.y * inv), pack2<BF16>(a.z * inv, a.w * inv));
   };
-  auto write_lse = [&](int r, float M, float sum) {
-    if (p.lse == nullptr) return;
+  auto write_sums = [&](int r, float M, float sum, float sumr) {
     const int rr = rt * kRows + r;
     const int g = rr / p.Nq;
-    p.lse[(static_cast<int64_t>(b) * p.H + hkv * p.G + g) * p.Nq + (rr - g * p.Nq)] =
-        sum > 0.f ? (M + log2f(sum)) * kLn2 : -FLT_MAX;
+    const int64_t at = (static_cast<int64_t>(b) * p.H + hkv * p.G + g) * p.Nq + (rr - g * p.Nq);
+    if (p.part_ml != nullptr) *reinterpret_cast<float4*>(p.part_ml + at * 4) = make_float4(M, sum, sumr, 0.f);
+    if (p.lse != nullptr) p.lse[at] = sum > 0.f ? (M + log2f(sum)) * kLn2 : -FLT_MAX;
   };
   const int64_t n_units = gridDim.x;
   float* ws_ml = p.ws;
@@ -508,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
     }
     if (p.pieces == 1) {
       write_out(r, x, a, sumr > 0.f ? 1.f / sumr : 0.f);
-      if (x == 0) write_lse(r, M, sum);
+      if (x == 0) write_sums(r, M, sum, sumr);
     } else {
       const int64_t at = static_cast<int64_t>(unit) * kRows + r;
       *reinterpret_cast<float4*>(ws_o + at * D + 4 * x) = a;
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       sumr += f * v.z;
     }
     total[r] = sumr > 0.f ? 1.f / sumr : 0.f;
-    write_lse(r, M, sum);
+    write_sums(r, M, sum, sumr);
   }
   __syncthreads();
   for (int idx = threadIdx.x; idx < rows * kVec; idx += kThreads) {
@@ -599,6 +606,8 @@ int launch(const CrossParams& a, const char** msg) {
   p.lengths = a.lengths;
   p.out = static_cast<uint16_t*>(a.out);
   p.lse = a.lse;
+  p.part_ml = a.part_ml;
+  p.part_o = a.part_o;
   p.err_word = a.err_word;
   p.timeout_ns = a.timeout_ns;
   p.B = static_cast<int>(a.B);

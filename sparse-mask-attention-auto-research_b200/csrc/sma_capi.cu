@@ -6,6 +6,7 @@
 // (CUDA tensors, 4-D shapes, fp16/bf16 dtype) become SMA_* status codes here;
 // the Python shim turns them into RuntimeError like TORCH_CHECK does.
 #include <atomic>
+#include <cfloat>
 #include <cstdio>
 #include <string>
 
@@ -185,6 +186,9 @@ int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool
     for (int i = 0; i < a->bias_side; ++i) p->bias.starts[i] = a->bias_starts[i];
   p->out = a->out;
   p->lse = a->lse;
+  p->words = static_cast<const uint32_t*>(a->words);
+  for (int i = 0; i < 3; ++i) p->word_stride[i] = a->word_stride[i];
+  p->bias_distance = a->bias_distance;
   p->B = a->B;
   p->H = a->H;
   p->Hkv = a->Hkv;
@@ -378,12 +382,101 @@ int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const void* v,
                       H, N, D, scale, stream);
 }
 
+int sma_pack_mask_rows(const void* mask, const int64_t* stride, void* words, int64_t Bm, int64_t Hm, int64_t Qm,
+                       int64_t Nk, void* stream) {
+  NvtxRange range("sma_pack_mask_rows");
+  constexpr int64_t kMax = int64_t{1} << 30;
+  if (Bm < 0 || Hm < 0 || Qm < 0 || Nk < 0 || Bm > kMax || Hm > kMax || Qm > kMax || Nk > kMax)
+    return fail(sma::kErrArg, "pack_mask: bad dimension");
+  if (Bm == 0 || Hm == 0 || Qm == 0 || Nk == 0) return sma::kOk;
+  if (mask == nullptr || words == nullptr || stride == nullptr) return fail(sma::kErrArg, "pack_mask: null pointer");
+  if (!aligned16(words)) return fail(sma::kErrArg, "pack_mask: words must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (stride[i] < 0) return fail(sma::kErrArg, "pack_mask: negative stride");
+  const char* msg = nullptr;
+  const int rc = sma::launch_pack_rows(static_cast<const uint8_t*>(mask), stride, static_cast<uint32_t*>(words), Bm, Hm,
+                                       Qm, Nk, static_cast<cudaStream_t>(stream), &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
+}  // extern "C"
+
+namespace {
+
+// Checks of the 128-row tile kernels on top of cross_params.
+int tile_params(const sma_attn_args* a) {
+  if (a->Nk > SMA_MAX_SEQ_LEN)
+    return fail(sma::kErrUnsupportedN, "attention: more keys than the supported maximum (65536)");
+  if (a->mask) return fail(sma::kErrArg, "attention: this entry takes packed words, not a bool mask");
+  if (a->words) {
+    if (a->lengths) return fail(sma::kErrArg, "attention: give a mask or lengths, not both");
+    if (!aligned16(a->words)) return fail(sma::kErrArg, "attention: words must be 16-byte aligned");
+    for (int i = 0; i < 3; ++i)
+      if (a->word_stride[i] < 0 || a->word_stride[i] % 4 != 0)
+        return fail(sma::kErrArg, "attention: word strides must be multiples of 4 words");
+  }
+  if (a->bias_table) {
+    if (!a->bias_distance || !aligned16(a->bias_distance))
+      return fail(sma::kErrArg, "attention: a bias needs a 16-byte aligned bias_distance");
+    if (a->bias_starts[a->bias_side - 1] > SMA_MAX_BIAS_DISTANCE)
+      return fail(sma::kErrUnsupportedN, "attention: bias distance above the supported maximum (65536)");
+  }
+  return sma::kOk;
+}
+
+// No keys at all: out = 0, lse = -FLT_MAX.
+int write_nothing(const sma::CrossParams& p) {
+  const int64_t rows = p.B * p.H * p.Nq;
+  cudaError_t e = cudaMemsetAsync(p.out, 0, static_cast<size_t>(rows * p.D * 2), p.stream);
+  // -FLT_MAX is the bit pattern 0xFF7FFFFF, which no byte fill makes.
+  if (e == cudaSuccess && p.lse != nullptr) {
+    const int rc = sma::launch_fill(p.lse, rows, -FLT_MAX, p.stream);
+    if (rc != sma::kOk) return fail(rc, "attention: fill launch failed");
+  }
+  return e == cudaSuccess ? sma::kOk : fail_cuda(e, "cudaMemsetAsync");
+}
+
+}  // namespace
+
+extern "C" {
+
+int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
+  NvtxRange range("sma_cross_attn_fwd");
+  sma::CrossParams p{};
+  bool empty = false;
+  int rc = cross_params(args, stream, &p, &empty);
+  if (rc != sma::kOk || empty) return rc;
+  if (p.P > 0) return fail(sma::kErrArg, "attention: no prefix here");
+  rc = tile_params(args);
+  if (rc != sma::kOk) return rc;
+  if (p.Nk == 0) return write_nothing(p);
+  const char* msg = nullptr;
+  rc = sma::launch_attn_cross(p, &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
+int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream) {
+  NvtxRange range("sma_prefix_attn_fwd");
+  sma::CrossParams p{};
+  bool empty = false;
+  int rc = cross_params(args, stream, &p, &empty);
+  if (rc != sma::kOk || empty) return rc;
+  rc = tile_params(args);
+  if (rc != sma::kOk) return rc;
+  if (p.P == 0 || args->words || args->bias_table || args->lse)
+    return fail(sma::kErrArg, "attention: a shared prefix takes P > 0 and no mask, bias or lse");
+  const char* msg = nullptr;
+  rc = sma::launch_shared_prefix(p, &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
 int sma_rows_attn_fwd(const sma_attn_args* args, void* stream) {
   NvtxRange range("sma_rows_attn_fwd");
   sma::CrossParams p{};
   bool empty = false;
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
+  if (p.Nk == 0 && p.P == 0) return write_nothing(p);
   const char* msg = nullptr;
   rc = sma::launch_attn_rows(p, &msg);
   return rc == sma::kOk ? rc : fail(rc, msg);

@@ -116,12 +116,48 @@ struct CrossParams {
   BiasSpec bias;
   void* out;                  // [B, H, Nq, D] contiguous
   float* lse;                 // [B, H, Nq] or nullptr
+  // attn_fwd_cross.cu: the mask packed by launch_pack_rows ([.., W] words with
+  // strides {batch, head, query}, 0: broadcast; nullptr keeps every key), and
+  // room for the bias by relative position, [H][bias_distance_len].
+  const uint32_t* words;
+  int64_t word_stride[3];
+  float* bias_distance;
+  // attn_rows.cu: where given, every row is left as a piece for a later merge
+  // (max, sum, sum of rounded P, - / FP32 O, not normalised; indexed by
+  // (b * H + h) * Nq + i) instead of written to `out`.
+  float* part_ml;
+  float* part_o;
   int64_t B, H, Hkv, Nq, Nk, D, P;
   float scale;
   uint32_t* err_word;
   uint64_t timeout_ns;
   cudaStream_t stream;
 };
+
+// The relative positions d between which buckets change: d <= lo is one
+// bucket, d >= hi is one bucket.
+inline void bias_range(const BiasSpec& s, int* lo, int* hi) {
+  *lo = -s.starts[s.side - 1];
+  *hi = s.two_sided ? s.starts[s.side - 1] : 0;
+}
+// Floats per head of the bias by relative position: lo .. hi and kBiasPad more
+// on either side, so that a tile which overlaps (lo, hi) never leaves it.
+constexpr int kBiasPad = 256;
+
+// Bool bytes -> words [Bm, Hm, Qm, 4 * ceil(Nk / 128)] (attn_fwd_cross.cu).
+int launch_pack_rows(const uint8_t* mask, const int64_t* stride, uint32_t* words, int64_t Bm, int64_t Hm, int64_t Qm,
+                     int64_t Nk, cudaStream_t stream, const char** msg);
+// Fills p.bias_distance from p.bias.
+int launch_bias_expand(const CrossParams& p, const char** msg);
+// Many query rows (attn_fwd_cross.cu), Nk <= kMaxSeqLen.
+int launch_attn_cross(const CrossParams& p, const char** msg);
+// A shared prefix attended once for the batch, P > 0 (attn_fwd_cross.cu).
+int launch_shared_prefix(const CrossParams& p, const char** msg);
+
+constexpr int kRowsTile = 16;  // rows of a tile of attn_rows.cu
+
+// x[0 .. n) = v (attn_fwd_cross.cu).
+int launch_fill(float* x, int64_t n, float v, cudaStream_t stream);
 
 // Few query rows per key head (attn_rows.cu): head dims 64 and 128.
 int launch_attn_rows(const CrossParams& p, const char** msg);
@@ -132,10 +168,10 @@ int launch_attn_rows(const CrossParams& p, const char** msg);
 // (CUDA_ERROR_NOT_FOUND when the entry point is missing).
 CUresult make_tensor_map_3d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t BH, int64_t N, int rows);
 // TMA map of a [B, H, N, D] fp16/bf16 view with element strides {batch, head,
-// row}: boxes of 64 head dims by `rows` rows, 128-byte swizzle; coordinates
-// (d, row, head, batch).
+// row}: boxes of 64 head dims by `rows` rows of `heads` heads of `batches`
+// batches, 128-byte swizzle; coordinates (d, row, head, batch).
 CUresult make_tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t N, int64_t H, int64_t B,
-                            const int64_t* stride, int rows);
+                            const int64_t* stride, int rows, int heads = 1, int batches = 1);
 // The same view of a contiguous FP32 [BH, N, D] tensor: boxes of 32 elements
 // (128 bytes) by `rows` rows, 128-byte swizzle (tma_map.cu).
 CUresult make_tensor_map_3d_f32(CUtensorMap* m, const void* ptr, int64_t D, int64_t BH, int64_t N, int rows);

@@ -71,7 +71,7 @@ CUresult make_tensor_map_3d(CUtensorMap* m, const void* ptr, int dtype, int64_t 
 }
 
 CUresult make_tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int64_t D, int64_t N, int64_t H, int64_t B,
-                            const int64_t* stride, int rows) {
+                            const int64_t* stride, int rows, int heads, int batches) {
   auto fn = encode_fn();
   if (fn == nullptr) return CUDA_ERROR_NOT_FOUND;
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(H),
@@ -79,7 +79,8 @@ CUresult make_tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int64_t 
   // The stride of an axis of length 1 is never used; any valid one will do.
   auto bytes = [&](int64_t n, int64_t s) { return static_cast<cuuint64_t>((n > 1 ? s : D) * 2); };
   cuuint64_t strides[3] = {bytes(N, stride[2]), bytes(H, stride[1]), bytes(B, stride[0])};
-  cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(rows), 1u, 1u};
+  cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(heads),
+                       static_cast<cuuint32_t>(batches)};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   return fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
             const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

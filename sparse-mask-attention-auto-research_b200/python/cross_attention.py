@@ -68,11 +68,25 @@ def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
+# Query rows per key head (queries times the heads that share one) up to which
+# the streaming kernel is taken; above, the 128-row tiles.
+_ROWS = 16
+
+
+def _few_rows(q, k):
+    return q.shape[1] // max(k.shape[1], 1) * q.shape[2] <= _ROWS or k.shape[2] > _lib.SMA_MAX_SEQ_LEN
+
+
 def _attention(q, k, v, mask, scale, bias):
     """out [B, H, Nq, D] of checked fp16 / bf16 inputs."""
     q, k, v = _strided(q), _strided(k), _strided(v)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, mask=mask, bias=bias)
+    if _few_rows(q, k):
+        sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, mask=mask, bias=bias)
+        return out
+    words = None if mask is None else sparse_attn_cuda.pack_mask_rows(mask)
+    distance = None if bias is None else sparse_attn_cuda.bias_distance_buffer(bias, q.shape[1], q.device)
+    sparse_attn_cuda.cross_forward(q, k, v, out, None, scale, words, bias, distance)
     return out
 
 
@@ -116,7 +130,10 @@ def _make_bias(table, q, bidirectional, max_distance, query_offset):
     _require(not bidirectional or buckets % 2 == 0, "a bidirectional bias needs an even number of buckets")
     _require(2 <= side <= _lib.SMA_MAX_BIAS_SIDE, f"2 to {_lib.SMA_MAX_BIAS_SIDE} buckets per side are supported")
     max_distance = int(max_distance)
-    _require(side // 2 < max_distance < 1 << 24, "max_distance must exceed the exact buckets and be below 2**24")
+    _require(
+        side // 2 < max_distance <= _lib.SMA_MAX_BIAS_DISTANCE,
+        f"max_distance must exceed the buckets of one distance each and be at most {_lib.SMA_MAX_BIAS_DISTANCE}",
+    )
     offset, offsets = 0, None
     if isinstance(query_offset, torch.Tensor):
         offsets = query_offset
@@ -188,5 +205,9 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths=None, scale=Non
         q, k_prefix, v_prefix, k, v = (t.bfloat16() for t in (q, k_prefix, v_prefix, k, v))
     q, k_prefix, v_prefix, k, v = (_strided(t) for t in (q, k_prefix, v_prefix, k, v))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, lengths=lengths, prefix=(k_prefix, v_prefix))
+    prefix = (k_prefix, v_prefix)
+    if B == 1 or k_prefix.shape[1] == 0 or S > _lib.SMA_MAX_SEQ_LEN:
+        sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, lengths=lengths, prefix=prefix)
+    else:
+        sparse_attn_cuda.prefix_forward(q, k, v, out, scale, prefix, lengths)
     return out.float() if dtype == torch.float32 else out

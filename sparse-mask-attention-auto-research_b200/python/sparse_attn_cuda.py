@@ -237,7 +237,33 @@ class Bias(typing.NamedTuple):
     offsets: typing.Optional[torch.Tensor]  # int32 [B], or None: offset for all
 
 
-def _attn_args(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None):
+def bias_distance_buffer(bias, H, device):
+    """Room for the bias by relative position (SMA_BIAS_DISTANCE_LEN floats per head)."""
+    last = bias.starts[len(bias.starts) - 1]
+    return torch.empty((H, (2 if bias.two_sided else 1) * last + 513), dtype=torch.float32, device=device)
+
+
+def pack_mask_rows(mask):
+    """bool mask [B or 1, H or 1, Nq or 1, Nk] -> (int32 words [Bm, Hm, Qm, W],
+    their strides): W = 4 * ceil(Nk / 128) words per row, bit b of word w =
+    column 32 w + b, 0 past Nk.  Axes along which the mask does not change
+    (length 1, or expanded) are packed once and have stride 0."""
+    if mask.shape[3] > 1 and mask.stride(3) != 1:
+        mask = mask.contiguous()
+    st = mask.stride()[:3]
+    dims = tuple(1 if s == 0 else n for n, s in zip(mask.shape[:3], st))
+    Nk = mask.shape[3]
+    W = (Nk + 127) // 128 * 4
+    words = torch.empty((*dims, W), dtype=torch.int32, device=mask.device)
+    lib = _lib.load()
+    with _device_guard(mask.device):
+        _lib.check(lib.sma_pack_mask_rows(mask.data_ptr(), (ctypes.c_int64 * 3)(*st), words.data_ptr(), *dims, Nk,
+                                          _stream_ptr(mask.device)))
+    return words, tuple(0 if n == 1 else s for n, s in zip(dims, words.stride()[:3]))
+
+
+def _attn_args(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None, words=None,
+               bias_distance=None):
     """sma_attn_args of checked tensors (see include/sma_capi.h), and what it
     points to that has to outlive the call."""
     B, H, Nq, D = q.shape
@@ -259,6 +285,8 @@ def _attn_args(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, b
         mask_ptr or 0, *mask_st, 0 if lengths is None else lengths.data_ptr(), 0 if table is None else table.data_ptr(),
         0 if starts is None else ctypes.addressof(starts), 0 if offsets is None else offsets.data_ptr(), offset,
         0 if starts is None else len(starts), int(two_sided), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        *((0, 0, 0, 0) if words is None else (words[0].data_ptr(), *words[1])),
+        0 if bias_distance is None else bias_distance.data_ptr(),
     )
     return raw, mask
 
@@ -273,6 +301,25 @@ def rows_forward(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None,
     lib = _lib.load()
     with _device_guard(q.device):
         _lib.check(lib.sma_rows_attn_fwd(args, _stream_ptr(q.device)))
+
+
+def cross_forward(q, k, v, out, lse, scale, words=None, bias=None, bias_distance=None):
+    """Attention of many query rows (sma_cross_attn_fwd): ``words`` from
+    pack_mask_rows or None, a ``bias`` with its bias_distance_buffer.  Writes
+    ``out`` and, unless None, ``lse``."""
+    args, _keep = _attn_args(q, k, v, out, lse, scale, words=words, bias=bias, bias_distance=bias_distance)
+    lib = _lib.load()
+    with _device_guard(q.device):
+        _lib.check(lib.sma_cross_attn_fwd(args, _stream_ptr(q.device)))
+
+
+def prefix_forward(q, k, v, out, scale, prefix, lengths=None):
+    """Attention behind a shared ``prefix`` (k, v) [Hkv, P, D], read once for
+    the batch (sma_prefix_attn_fwd)."""
+    args, _keep = _attn_args(q, k, v, out, None, scale, lengths=lengths, prefix=prefix)
+    lib = _lib.load()
+    with _device_guard(q.device):
+        _lib.check(lib.sma_prefix_attn_fwd(args, _stream_ptr(q.device)))
 
 
 def pack_mask(mask):

@@ -21,7 +21,7 @@ def lib():
 
 STARTS = (ctypes.c_int32 * 4)(0, 1, 2, 8)
 FIELDS = ("dtype scale B H Hkv Nq Nk D P q k v qb qh qn kb kh kn vb vh vn kp vp kph kpn vph vpn mask mb mh mn lengths table "
-          "starts offsets offset side two_sided out lse").split()
+          "starts offsets offset side two_sided out lse words wb wh wq distance").split()
 
 
 def raw(**kw):
@@ -96,7 +96,7 @@ def test_cpu_tensors_are_refused():
         sma.shared_prefix_attention(q, k[0], k[0], k, k)
 
 
-@pytest.mark.parametrize("side,distance", [(16, 128), (32, 128), (8, 64), (64, 256), (2, 3), (3, 9), (128, 1000), (5, 1 << 20)])
+@pytest.mark.parametrize("side,distance", [(16, 128), (32, 128), (8, 64), (64, 256), (2, 3), (3, 9), (128, 1000), (5, 1 << 16)])
 def test_bucket_starts(side, distance):
     """Against the definition in exact fractions; a query's own distance is
     bucket 0, and `distance` and everything beyond it fall in the last one."""
