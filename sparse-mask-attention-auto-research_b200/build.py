@@ -24,7 +24,7 @@ BUILD_DIR = os.path.join(HERE, "_build")
 LIB_PATH = os.path.join(HERE, "libsma.so")
 
 SOURCES = ["sma_capi.cu", "pack_mask.cu", "attn_fwd.cu", "attn_fwd_chain.cu", "tma_map.cu", "attn_bwd.cu",
-           "attn_rows.cu", "attn_fwd_cross.cu"]
+           "attn_rows.cu", "attn_fwd_cross.cu", "attn_bwd_cross.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = [
     "-O3",

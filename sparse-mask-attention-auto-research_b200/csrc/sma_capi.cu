@@ -154,6 +154,8 @@ int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool
     for (int i = 0; i < a->bias_side; ++i)
       if (a->bias_starts[i] < 0 || (i == 0 ? a->bias_starts[0] != 0 : a->bias_starts[i] < a->bias_starts[i - 1]))
         return fail(sma::kErrArg, "attention: bucket starts must ascend from 0");
+    if (a->bias_two_sided && a->bias_starts[a->bias_side - 1] == 0)
+      return fail(sma::kErrArg, "attention: a two-sided bias needs a bucket start above 0");
   }
   uint32_t* err = nullptr;
   const int rc = error_word(&err);
@@ -453,6 +455,37 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
   const char* msg = nullptr;
   rc = sma::launch_attn_cross(p, &msg);
   return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
+int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
+                       float* dq_accum, float* delta, float* bias_part, void* stream) {
+  NvtxRange range("sma_cross_attn_bwd");
+  sma::CrossParams p{};
+  bool empty = false;
+  int rc = cross_params(args, stream, &p, &empty);
+  if (rc != sma::kOk) return rc;
+  if (empty || p.Nk == 0) return fail(sma::kErrArg, "backward: no queries or no keys");
+  if (p.P > 0 || p.lengths) return fail(sma::kErrArg, "backward: no prefix and no lengths");
+  rc = tile_params(args);
+  if (rc != sma::kOk) return rc;
+  if (!p.lse || !dout || !dq || !dk || !dv || !dq_accum || !delta || (p.bias.table && (!dtable || !bias_part)))
+    return fail(sma::kErrArg, "backward: null pointer");
+  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(dq_accum) ||
+      !aligned16(bias_part))
+    return fail(sma::kErrArg, "backward: dout/dq/dk/dv/dq_accum/bias_part must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(delta) & 3u) || (reinterpret_cast<uintptr_t>(dtable) & 1u))
+    return fail(sma::kErrArg, "backward: misaligned delta or dtable");
+  const sma::CrossGrads g{dout, dq, dk, dv, dq_accum, delta, dtable, bias_part};
+  const char* msg = nullptr;
+  rc = sma::launch_attn_cross_bwd(p, g, &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
+int64_t sma_cross_attn_bwd_bias_floats(const sma_attn_args* args) {
+  sma::CrossParams p{};
+  bool empty = false;
+  if (cross_params(args, nullptr, &p, &empty) != sma::kOk || empty || p.Nk == 0 || tile_params(args) != sma::kOk) return -1;
+  return sma::cross_bwd_bias_floats(p);
 }
 
 int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream) {

@@ -154,6 +154,21 @@ int launch_attn_cross(const CrossParams& p, const char** msg);
 // A shared prefix attended once for the batch, P > 0 (attn_fwd_cross.cu).
 int launch_shared_prefix(const CrossParams& p, const char** msg);
 
+// Gradients (attn_bwd_cross.cu), all contiguous; p.out and p.lse are the
+// forward's, p.bias_distance as it left it.
+struct CrossGrads {
+  const void* dout;  // [B, H, Nq, D]
+  void* dq;          // [B, H, Nq, D]
+  void* dk;          // [B, Hkv, Nk, D]
+  void* dv;
+  float* dq_accum;   // [B, H, Nq, D] scratch
+  float* delta;      // [B, H, Nq] scratch
+  void* dtable;      // [buckets, H], with a bias
+  float* bias_part;  // cross_bwd_bias_floats scratch, with a bias
+};
+int64_t cross_bwd_bias_floats(const CrossParams& p);
+int launch_attn_cross_bwd(const CrossParams& p, const CrossGrads& g, const char** msg);
+
 constexpr int kRowsTile = 16;  // rows of a tile of attn_rows.cu
 
 // x[0 .. n) = v (attn_fwd_cross.cu).

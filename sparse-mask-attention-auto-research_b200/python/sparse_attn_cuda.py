@@ -313,6 +313,32 @@ def cross_forward(q, k, v, out, lse, scale, words=None, bias=None, bias_distance
         _lib.check(lib.sma_cross_attn_fwd(args, _stream_ptr(q.device)))
 
 
+def cross_backward(dout, q, k, v, out, lse, scale, words=None, bias=None, bias_distance=None):
+    """Gradients of cross_forward (sma_cross_attn_bwd) from its ``out``,
+    ``lse`` and ``bias_distance``: (dq, dk, dv, dtable or None), contiguous."""
+    args, _keep = _attn_args(q, k, v, out, lse, scale, words=words, bias=bias, bias_distance=bias_distance)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=q.device) for _ in range(2))
+    dq_accum = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    delta = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    dtable = bias_part = None
+    lib = _lib.load()
+    with _device_guard(q.device):
+        if bias is not None:
+            dtable = torch.empty_like(bias.table)
+            floats = lib.sma_cross_attn_bwd_bias_floats(args)
+            _require(floats >= 0, "backward: unsupported arguments")
+            bias_part = torch.empty(floats, dtype=torch.float32, device=q.device)
+        _lib.check(
+            lib.sma_cross_attn_bwd(
+                args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                None if dtable is None else dtable.data_ptr(), dq_accum.data_ptr(), delta.data_ptr(),
+                None if bias_part is None else bias_part.data_ptr(), _stream_ptr(q.device),
+            )
+        )
+    return dq, dk, dv, dtable
+
+
 def prefix_forward(q, k, v, out, scale, prefix, lengths=None):
     """Attention behind a shared ``prefix`` (k, v) [Hkv, P, D], read once for
     the batch (sma_prefix_attn_fwd)."""

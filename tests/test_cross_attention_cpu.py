@@ -67,6 +67,7 @@ BIAS = dict(table=16, starts=ctypes.addressof(STARTS), side=4)
         (dict(BIAS, side=129), L.SMA_ERR_ARG),
         (dict(BIAS, starts=0), L.SMA_ERR_ARG),
         (dict(BIAS, starts=ctypes.addressof(STARTS) + 4, side=2), L.SMA_ERR_ARG),  # does not start at 0
+        (dict(BIAS, side=1, two_sided=1), L.SMA_ERR_ARG),
         (dict(BIAS, offset=1 << 30), L.SMA_ERR_ARG),
         (dict(BIAS, P=8, kp=16, vp=16), L.SMA_ERR_ARG),
         (dict(BIAS, table=17), L.SMA_ERR_ARG),
