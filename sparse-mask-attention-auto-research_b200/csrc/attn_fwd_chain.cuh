@@ -162,9 +162,15 @@ struct SplitParams {
 // each.  One TMA box (64 dims, tn, hb, nb) loads and stores such a tile in
 // row order, clipped at Nq and B.
 //
-// Which keys a row keeps: packed words (strides 0 where the mask broadcasts),
+// A prefix of keys that all batches share may stand in front of the sequences'
+// own: key tiles 0 .. KTp-1 are the prefix's (P keys, every one kept), the
+// rest the sequence's.
+//
+// Which of its own keys a row keeps: packed words (strides 0 where the mask broadcasts),
 // or lengths (key j < lengths[b] - Nq + 1 + query), or every key.
 struct Geo {
+  CUtensorMap tm_kp, tm_vp;
+  int KTp, P;
   int B, H, Hkv, Nq;
   int tn, hb, nb, rows;    // rows = tn * hb * nb
   int gh;                  // tiles of a head group, G / hb
@@ -179,16 +185,6 @@ struct Geo {
   int bias_offset, bias_lo, bias_hi, bias_len;
 };
 struct NoGeo {};
-
-// Split launches of the kX kernels may take in one more piece of every row
-// (its other keys, attended by an earlier launch), and may leave the merged
-// row as such a piece instead of writing O.  Indexed by (b * H + h) * Nq + i.
-struct SplitParamsX : SplitParams {
-  const float* in_ml;  // [rows][4]: max, sum, sum of rounded P, -
-  const float* in_o;   // [rows][D], not normalised
-  float* out_ml;
-  float* out_o;
-};
 
 template <int D>
 constexpr size_t smem_bytes() {
@@ -350,26 +346,14 @@ __device__ __forceinline__ uint32_t group_live(const uint4& v, int g, int k, int
 // p0+pieces-1 for its row r, in piece order: weights 2^(m_p - M) against the
 // row's overall max M, O = sum w_p O_p / sum w_p l_out_p, LSE from
 // sum w_p l_p (M = -inf: an empty row, O = 0 and LSE = -FLT_MAX).
-// kX: `xrow` is the row's index among all rows, for the piece to take in and
-// the one to leave.
-template <int D, bool BF16, bool kX>
-__device__ __noinline__ void merge_pieces(const std::conditional_t<kX, SplitParamsX, SplitParams> sp, int64_t n_units,
-                                          int64_t p0, int r, uint16_t* orow, float* lse_r, bool write_o,
-                                          int64_t xrow) {
+template <int D, bool BF16>
+__device__ __noinline__ void merge_pieces(const SplitParams sp, int64_t n_units, int64_t p0, int r, uint16_t* orow,
+                                          float* lse_r, bool write_o) {
   const float* ml_base = sp.ws;                    // [unit][row][4]
   const float* po_base = sp.ws + n_units * kBM * 4;  // [unit][row][D]
   float M = -INFINITY;
   for (int pc = 0; pc < sp.pieces; ++pc) M = fmaxf(M, __ldcg(ml_base + ((p0 + pc) * kBM + r) * 4));
-  float lr = 0.f, lo = 0.f, w_in = 0.f;
-  if constexpr (kX) {
-    if (sp.in_ml != nullptr) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(sp.in_ml + xrow * 4));
-      M = fmaxf(M, v.x);
-      w_in = (v.x == -INFINITY) ? 0.f : ex2f(v.x - M);
-      lr = w_in * v.y;
-      lo = w_in * v.z;
-    }
-  }
+  float lr = 0.f, lo = 0.f;
   for (int pc = 0; pc < sp.pieces; ++pc) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(ml_base + ((p0 + pc) * kBM + r) * 4));
     const float w = (v.x == -INFINITY) ? 0.f : ex2f(v.x - M);
@@ -382,19 +366,6 @@ __device__ __noinline__ void merge_pieces(const std::conditional_t<kX, SplitPara
     float acc[32];
 #pragma unroll
     for (int q = 0; q < 32; ++q) acc[q] = 0.f;
-    if constexpr (kX) {
-      if (sp.in_ml != nullptr) {
-        const float4* src = reinterpret_cast<const float4*>(sp.in_o + xrow * D + dc * 32);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 o = __ldcg(src + q);
-          acc[4 * q] = w_in * o.x;
-          acc[4 * q + 1] = w_in * o.y;
-          acc[4 * q + 2] = w_in * o.z;
-          acc[4 * q + 3] = w_in * o.w;
-        }
-      }
-    }
     for (int pc = 0; pc < sp.pieces; ++pc) {
       const float mp = __ldcg(ml_base + ((p0 + pc) * kBM + r) * 4);
       const float w = (mp == -INFINITY) ? 0.f : ex2f(mp - M);
@@ -408,14 +379,6 @@ __device__ __noinline__ void merge_pieces(const std::conditional_t<kX, SplitPara
         acc[4 * q + 3] += w * o.w;
       }
     }
-    if constexpr (kX) {
-      if (sp.out_ml != nullptr) {
-        float4* dst = reinterpret_cast<float4*>(sp.out_o + xrow * D + dc * 32);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) dst[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
-        continue;
-      }
-    }
     uint32_t hw[16];
 #pragma unroll
     for (int q = 0; q < 16; ++q) hw[q] = pack2<BF16>(acc[2 * q] * inv, acc[2 * q + 1] * inv);
@@ -424,9 +387,6 @@ __device__ __noinline__ void merge_pieces(const std::conditional_t<kX, SplitPara
 #pragma unroll
       for (int q = 0; q < 4; ++q) dst[q] = make_uint4(hw[4 * q], hw[4 * q + 1], hw[4 * q + 2], hw[4 * q + 3]);
     }
-  }
-  if constexpr (kX) {
-    if (sp.out_ml != nullptr) *reinterpret_cast<float4*>(sp.out_ml + xrow * 4) = make_float4(M, lr, lo, 0.f);
   }
   if (lse_r != nullptr) *lse_r = (lr > 0.f) ? (M + log2f(lr)) * kLn2 : -FLT_MAX;
 }
@@ -465,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           const uint8_t* __restrict__ bmask, uint32_t* pk,
                           const uint32_t* __restrict__ occ, float* __restrict__ lse, int N, int BH, int W,
                           int KT, int total_items, int vec, int o_wide, int head_major, int pf_early,
-                          float scale_log2, const std::conditional_t<kX, SplitParamsX, SplitParams> sp,
+                          float scale_log2, const SplitParams sp,
                           const __grid_constant__ std::conditional_t<kX, Geo, NoGeo> x, uint32_t* err_word,
                           uint64_t timeout_ns) {
   static_assert(!(kX && kBoolIn) && (kX || !kBias), "mode");
@@ -680,8 +640,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int dc = 0; dc < C::kDChunks; ++dc) {
           if constexpr (kX) {
-            tma_load_4d(sK + stage * C::kKVBytes + dc * (kBN * 128), &tm_k, smem_u32(&cc.k_full[stage]), dc * 64,
-                        kt * kBN, it.hkv, x.kv_shared ? 0 : it.b0);
+            const bool pre = kt < x.KTp;
+            tma_load_4d(sK + stage * C::kKVBytes + dc * (kBN * 128), pre ? &x.tm_kp : &tm_k,
+                        smem_u32(&cc.k_full[stage]), dc * 64, (pre ? kt : kt - x.KTp) * kBN, it.hkv,
+                        pre || x.kv_shared ? 0 : it.b0);
           } else {
             tma_load_3d(sK + stage * C::kKVBytes + dc * (kBN * 128), &tm_k, smem_u32(&cc.k_full[stage]), dc * 64,
                         kt * kBN, it.bh);
@@ -701,8 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int dc = 0; dc < C::kDChunks; ++dc) {
           if constexpr (kX) {
-            tma_load_4d(sV + stage * C::kKVBytes + dc * (kBN * 128), &tm_v, smem_u32(&cc.v_full[stage]), dc * 64,
-                        kt * kBN, it.hkv, x.kv_shared ? 0 : it.b0);
+            const bool pre = kt < x.KTp;
+            tma_load_4d(sV + stage * C::kKVBytes + dc * (kBN * 128), pre ? &x.tm_vp : &tm_v,
+                        smem_u32(&cc.v_full[stage]), dc * 64, (pre ? kt : kt - x.KTp) * kBN, it.hkv,
+                        pre || x.kv_shared ? 0 : it.b0);
           } else {
             tma_load_3d(sV + stage * C::kKVBytes + dc * (kBN * 128), &tm_v, smem_u32(&cc.v_full[stage]), dc * 64,
                         kt * kBN, it.bh);
@@ -942,7 +906,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto fetch_words = [&](const Item& it, int kt, uint32_t (&mw)[kWords]) {
       if constexpr (kX) {
         if (x.words == nullptr) {
-          const int limit = x.lengths != nullptr ? row_limit(it, it.q0 + xt) : N;
+          int limit = x.P;  // of the tile's own sequence: the prefix, or the row's keys
+          if (kt >= x.KTp) {
+            kt -= x.KTp;
+            limit = x.lengths != nullptr ? row_limit(it, it.q0 + xt) : N;
+          }
 #pragma unroll
           for (int w = 0; w < kWords; ++w) mw[w] = row_ok(it) ? low_bits(limit - kt * kBN - 32 * w) : 0u;
           return;
@@ -975,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nw = (KT + 31) >> 5;
       if constexpr (kX) {
         if (x.words == nullptr) {  // lengths: the tiles below the row's limit
-          const int tiles = row_ok(it) ? (row_limit(it, it.q0 + xt) + kBN - 1) / kBN : 0;
+          const int tiles = row_ok(it) ? x.KTp + (max(row_limit(it, it.q0 + xt), 0) + kBN - 1) / kBN : 0;
           for (int k = 0; k < nw; ++k) {
             const uint32_t bits = __reduce_or_sync(0xffffffffu, low_bits(tiles - 32 * k));
             if (lane == 0 && bits != 0u) atomicOr(&cc.scan_bits[j % kSlots][k], bits);
@@ -1244,8 +1212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int ch = 1; ch < kWords; ++ch) word = (r >> 5) == ch ? mw[ch] : word;
               dead = r < kBN && ((word >> (r & 31)) & 1u) == 0u;
             }
-          } else if (x.lengths != nullptr) {
-            const int most = row_limit(it, min(it.q0 + x.tn, x.Nq) - 1) - kt_cur * kBN;
+          } else if (x.lengths != nullptr && kt_cur >= x.KTp) {
+            const int most = row_limit(it, min(it.q0 + x.tn, x.Nq) - 1) - (kt_cur - x.KTp) * kBN;
             some = most < kBN;
             dead = r < kBN && r >= most;
           }
@@ -1406,7 +1374,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if constexpr (kSplitK) {
         // A piece of a split item (no O staging, no scan ahead: i+2 is
-        // scanned below like any unit).  Its unnormalised O (FP32) and (max,
+        // scanned below like any unit).  kX leaves the merge to a kernel of
+        // its own (attn_fwd_cross.cu), which spreads it over all SMs.  Its unnormalised O (FP32) and (max,
         // sums) go to the workspace; the piece that completes the item's
         // count merges the item's pieces in piece order, so the result does
         // not depend on which piece finishes last.
@@ -1434,6 +1403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             reinterpret_cast<uint4*>(po + dc * 32)[q] = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
         }
         *reinterpret_cast<float4*>(ml) = make_float4(m_run, l_run, l_out, 0.f);
+        if constexpr (kX) continue;
         __threadfence();
         named_bar_sync(bar_id, 128);
         if (r == 0) {
@@ -1446,9 +1416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_bar_sync(bar_id, 128);
         if (cc.split_last != 0u && row_ok(it)) {
           __threadfence();
-          merge_pieces<D, BF16, kX>(sp, n_units, static_cast<int64_t>(item) * sp.pieces, r, out + row_index(it) * D,
-                                    lse != nullptr ? lse + row_index(it) : nullptr, ctl.abort_flag == 0,
-                                    row_index(it));
+          merge_pieces<D, BF16>(sp, n_units, static_cast<int64_t>(item) * sp.pieces, r, out + row_index(it) * D,
+                                lse != nullptr ? lse + row_index(it) : nullptr, ctl.abort_flag == 0);
         }
       } else if constexpr (C::kStageO) {
         // The work that does not need O goes first, under the last PV's

@@ -71,6 +71,94 @@ __global__ void __launch_bounds__(256)
         kLog2e * (bf16 ? bias_value<true>(bias, bucket, h) : bias_value<false>(bias, bucket, h));
 }
 
+// ---------------------------------------------------------------- merge of a split launch
+// Row (b, h, i) of every piece of its item, and `in` (its other keys, attended
+// by an earlier launch), merged in that order: weights 2^(m_p - M) against
+// the overall maximum M, O = sum w_p O_p / sum w_p l_out_p.  Writes O and the
+// LSE, or (`out_ml`) the merged row as a piece for a later merge.  One warp
+// per row, so every read is a whole row of D floats; bound by reading the
+// pieces, mostly from L2 (they have just been written).
+struct MergeParams {
+  const float* ws;   // [units][128][4] (max, sum, sum of rounded P, -) then [units][128][D]
+  int64_t units;
+  int pieces, groups, QT, head_major;
+  const float* in_ml;
+  const float* in_o;
+  float* out_ml;
+  float* out_o;
+  uint16_t* out;
+  float* lse;
+  int64_t rows;      // B * H * Nq
+};
+
+constexpr int kMergeWarps = 4;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+    merge_rows_kernel(const __grid_constant__ MergeParams m, const __grid_constant__ Geo x) {
+  constexpr int kPer = D / 32;  // floats per lane
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  if (row >= m.rows) return;
+  const int64_t bh = row / x.Nq;
+  const int i = static_cast<int>(row - bh * x.Nq);
+  const int b = static_cast<int>(bh / x.H), h = static_cast<int>(bh - static_cast<int64_t>(b) * x.H);
+  const int qt = i / kBM, per_kv = x.gh * x.hb;
+  const int hkv = h / per_kv, hg = h - hkv * per_kv, bt = b / x.nb;
+  const int r = ((b - bt * x.nb) * x.hb + hg % x.hb) * x.tn + (i - qt * kBM);
+  const int group = (bt * x.Hkv + hkv) * x.gh + hg / x.hb;
+  const int64_t slow = m.QT - 1 - qt;
+  const int64_t item = m.head_major ? static_cast<int64_t>(group) * m.QT + slow : slow * m.groups + group;
+  const float* ml = m.ws + (item * m.pieces * kBM + r) * 4;
+  const float* po = m.ws + m.units * kBM * 4 + (item * m.pieces * kBM + r) * D + lane * kPer;
+
+  float4 in = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  if (m.in_ml != nullptr) in = __ldcg(reinterpret_cast<const float4*>(m.in_ml + row * 4));
+  float M = in.x;
+  for (int p = lane; p < m.pieces; p += 32) M = fmaxf(M, __ldcg(ml + static_cast<int64_t>(p) * kBM * 4));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float w_in = in.x == -INFINITY ? 0.f : ex2f(in.x - M);
+  float l = w_in * in.y, lo = w_in * in.z, acc[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+  if (m.in_o != nullptr) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = w_in * __ldcg(m.in_o + row * D + lane * kPer + e);
+  }
+#pragma unroll 4
+  for (int p = 0; p < m.pieces; ++p) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(ml + static_cast<int64_t>(p) * kBM * 4));
+    const float* src = po + static_cast<int64_t>(p) * kBM * D;
+    float o[kPer];
+    if constexpr (kPer == 4) {
+      const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
+      o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
+    } else {
+      const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
+      o[0] = f.x, o[1] = f.y;
+    }
+    const float w = v.x == -INFINITY ? 0.f : ex2f(v.x - M);
+    l += w * v.y;
+    lo += w * v.z;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] += w * o[e];
+  }
+  if (m.out_ml != nullptr) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) m.out_o[row * D + lane * kPer + e] = acc[e];
+    if (lane == 0) *reinterpret_cast<float4*>(m.out_ml + row * 4) = make_float4(M, l, lo, 0.f);
+    return;
+  }
+  const float inv = lo > 0.f ? 1.f / lo : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(m.out + row * D + lane * kPer);
+#pragma unroll
+  for (int e = 0; e < kPer / 2; ++e) dst[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if (m.lse != nullptr && lane == 0) m.lse[row] = l > 0.f ? (M + log2f(l)) * kLn2 : -FLT_MAX;
+}
+
 __global__ void __launch_bounds__(256) fill_kernel(float* x, int64_t n, float v) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i < n) x[i] = v;
@@ -95,6 +183,10 @@ int choose_pieces(int64_t items, int64_t tiles, int64_t chains, bool merge_anywa
   return best;
 }
 
+// A shared prefix is taken in one pass per sequence when a key head has more
+// rows than this: the rows of one sequence then fill most of a tile.
+constexpr int kOnePassRows = 64;
+
 // The keys of one launch: k and v with their strides {batch, head, row}.
 struct Keys {
   const void* k;
@@ -111,15 +203,16 @@ struct Partial {
 };
 
 template <int D, bool BF16, bool kSplitK, bool kBias>
-int launch(const CrossParams& p, const Keys& keys, const Geo& x, int pieces, Partial in, Partial out, const char** msg) {
+int launch(const CrossParams& p, const Keys& keys, Geo x, int pieces, Partial in, Partial out, const char** msg) {
   using C = ChainCfg<D>;
   constexpr size_t kSmemBytes = smem_bytes<D>();
   const int64_t W = (keys.n + 127) / 128 * 4;
-  const int64_t KT = (keys.n + C::kBN - 1) / C::kBN;
+  const int64_t KT = x.KTp + (keys.n + C::kBN - 1) / C::kBN;
   const int64_t QT = (p.Nq + kBM - 1) / kBM;
   const int64_t groups = (p.B + x.nb - 1) / x.nb * p.Hkv * x.gh;
   const int64_t total = QT * groups * pieces;
-  if (total > 0x3FFFFFFFll) {
+  const int64_t rows = p.B * p.H * p.Nq;
+  if (total > 0x3FFFFFFFll || rows > (int64_t{0x7FFFFFFF} * kMergeWarps)) {
     *msg = "attention: too many query rows";
     return kErrArg;
   }
@@ -127,8 +220,16 @@ int launch(const CrossParams& p, const Keys& keys, const Geo& x, int pieces, Par
   const int64_t so[3] = {p.H * p.Nq * D, p.Nq * D, D};
   const int64_t kb = keys.shared ? 1 : p.B;
   CUresult rc = make_tensor_map_4d(&mq, p.q, p.dtype, D, p.Nq, p.H, p.B, p.q_stride, x.tn, x.hb, x.nb);
-  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mk, keys.k, p.dtype, D, keys.n, p.Hkv, kb, keys.k_stride, C::kBN);
-  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mv, keys.v, p.dtype, D, keys.n, p.Hkv, kb, keys.v_stride, C::kBN);
+  if (rc == CUDA_SUCCESS && keys.n > 0) {
+    rc = make_tensor_map_4d(&mk, keys.k, p.dtype, D, keys.n, p.Hkv, kb, keys.k_stride, C::kBN);
+    if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mv, keys.v, p.dtype, D, keys.n, p.Hkv, kb, keys.v_stride, C::kBN);
+  }
+  if (rc == CUDA_SUCCESS && x.KTp > 0) {
+    const int64_t ks[3] = {0, p.kp_stride[0], p.kp_stride[1]}, vs[3] = {0, p.vp_stride[0], p.vp_stride[1]};
+    rc = make_tensor_map_4d(&x.tm_kp, p.k_prefix, p.dtype, D, p.P, p.Hkv, 1, ks, C::kBN);
+    if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&x.tm_vp, p.v_prefix, p.dtype, D, p.P, p.Hkv, 1, vs, C::kBN);
+    if (keys.n == 0) mk = x.tm_kp, mv = x.tm_vp;  // not used: no tile of its own
+  }
   if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mo, p.out, p.dtype, D, p.Nq, p.H, p.B, so, x.tn, x.hb, x.nb);
   if (rc != CUDA_SUCCESS) {
     *msg = tensor_map_error("attention", rc);
@@ -143,20 +244,13 @@ int launch(const CrossParams& p, const Keys& keys, const Geo& x, int pieces, Par
   // As for the square kernel: head-major once K and V exceed half of L2.
   const int head_major = 2 * kb * p.Hkv * keys.n * D * 2 > dp.l2_bytes / 2 ? 1 : 0;
   const int grid = static_cast<int>(total < dp.sms ? total : dp.sms);
-  SplitParamsX sp{};
+  SplitParams sp{};
   void* ws = nullptr;
   if constexpr (kSplitK) {
-    const size_t cnt_bytes = (static_cast<size_t>(total / pieces) * 8 + 255) / 256 * 256;
-    const size_t rows = static_cast<size_t>(total) * kBM;
-    if (e == cudaSuccess) e = scratch_alloc_async(&ws, cnt_bytes + rows * (4 + D) * sizeof(float), p.stream);
+    if (e == cudaSuccess)
+      e = scratch_alloc_async(&ws, static_cast<size_t>(total) * kBM * (4 + D) * sizeof(float), p.stream);
     sp.pieces = pieces;
-    sp.cnt = static_cast<unsigned long long*>(ws);
-    sp.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + cnt_bytes);
-    sp.epoch = next_launch_epoch();
-    sp.in_ml = in.ml;
-    sp.in_o = in.o;
-    sp.out_ml = out.ml;
-    sp.out_o = out.o;
+    sp.ws = static_cast<float*>(ws);
   }
   if (e == cudaSuccess)
     e = launch_pdl(kern, static_cast<unsigned>(grid), kThreads, kSmemBytes, p.stream, mq, mk, mv, mo,
@@ -164,6 +258,24 @@ int launch(const CrossParams& p, const Keys& keys, const Geo& x, int pieces, Par
                    static_cast<int>(keys.n), static_cast<int>(groups), static_cast<int>(W), static_cast<int>(KT),
                    static_cast<int>(total), 1, o_wide, head_major, 0, p.scale * kLog2e, sp, x, p.err_word,
                    p.timeout_ns);
+  if (kSplitK && e == cudaSuccess) {
+    MergeParams m{};
+    m.ws = sp.ws;
+    m.units = total;
+    m.pieces = pieces;
+    m.groups = static_cast<int>(groups);
+    m.QT = static_cast<int>(QT);
+    m.head_major = head_major;
+    m.in_ml = in.ml;
+    m.in_o = in.o;
+    m.out_ml = out.ml;
+    m.out_o = out.o;
+    m.out = static_cast<uint16_t*>(p.out);
+    m.lse = p.lse;
+    m.rows = rows;
+    e = launch_pdl(merge_rows_kernel<D, BF16>, static_cast<unsigned>((rows + kMergeWarps - 1) / kMergeWarps),
+                   kMergeWarps * 32, 0, p.stream, m, x);
+  }
   if (e == cudaSuccess) e = cudaGetLastError();
   if (ws != nullptr) {
     const cudaError_t ef = cudaFreeAsync(ws, p.stream);
@@ -177,8 +289,10 @@ int launch(const CrossParams& p, const Keys& keys, const Geo& x, int pieces, Par
 }
 
 // One launch over `keys`.  `partial`: takes in / leaves a piece of every row
-// (always the split kernel, which merges).
-int launch_tiles(const CrossParams& p, const Keys& keys, bool partial, Partial in, Partial out, const char** msg) {
+// (always the split kernel, whose merge does that).  `with_prefix`: p's prefix
+// stands in front of the keys.
+int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool partial, Partial in, Partial out,
+                 const char** msg) {
   DeviceProps dp;
   if (!device_props(&dp, msg)) return kErrCuda;
   Geo x{};
@@ -200,6 +314,11 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool partial, Partial i
     x.row_shared = p.words != nullptr && (x.Nq == 1 || p.word_stride[2] == 0) && (x.hb == 1 || p.word_stride[1] == 0);
     x.lengths = p.lengths;
   }
+  const int bn = p.D == 64 ? 128 : 64;
+  if (with_prefix) {
+    x.P = static_cast<int>(p.P);
+    x.KTp = (x.P + bn - 1) / bn;
+  }
   const bool bias = p.bias.table != nullptr;
   if (bias) {
     x.bias = p.bias_distance;
@@ -208,9 +327,8 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool partial, Partial i
     bias_range(p.bias, &x.bias_lo, &x.bias_hi);
     x.bias_len = x.bias_hi - x.bias_lo + 1 + 2 * kBiasPad;
   }
-  const int bn = p.D == 64 ? 128 : 64;
   const int64_t items = (p.B + x.nb - 1) / x.nb * p.Hkv * x.gh * ((p.Nq + kBM - 1) / kBM);
-  const int pieces = choose_pieces(items, (keys.n + bn - 1) / bn, 2 * static_cast<int64_t>(dp.sms), partial);
+  const int pieces = choose_pieces(items, x.KTp + (keys.n + bn - 1) / bn, 2 * static_cast<int64_t>(dp.sms), partial);
   const bool split = partial || pieces > 1;
 #define SMA_LAUNCH(D_, BF_)                                                            \
   (split ? (bias ? launch<D_, BF_, true, true>(p, keys, x, pieces, in, out, msg)       \
@@ -279,18 +397,27 @@ int launch_attn_cross(const CrossParams& p, const char** msg) {
     if (rc != kOk) return rc;
   }
   const Keys keys{p.k, p.v, p.k_stride, p.v_stride, p.Nk, false};
-  return launch_tiles(p, keys, false, {}, {}, msg);
+  return launch_tiles(p, keys, false, false, {}, {}, msg);
 }
 
-// Two launches: the sequences' own keys leave a piece of every row (FP32),
-// then the prefix is attended once for the whole batch, the rows of several
-// sequences in one tile, and its merge takes those pieces in.
+// Either one pass over prefix and own keys per sequence, or the prefix once for
+// the batch: the sequences' own keys leave a piece of every row (FP32), then
+// the prefix is attended with the rows of several sequences in one tile, and
+// its merge takes those pieces in.
 int launch_shared_prefix(const CrossParams& p, const char** msg) {
+  DeviceProps dp;
+  if (!device_props(&dp, msg)) return kErrCuda;
   const int64_t rows = p.B * p.H * p.Nq;
+  const int64_t group_rows = p.H / p.Hkv * p.Nq;
+  const Keys own_keys{p.k, p.v, p.k_stride, p.v_stride, p.Nk, false};
+  const int64_t bn = p.D == 64 ? 128 : 64;
+  const int64_t own_tiles = (p.Nk + bn - 1) / bn, prefix_tiles = (p.P + bn - 1) / bn;
+  if (group_rows > kOnePassRows && own_tiles + prefix_tiles <= kMaxSeqLen / bn)
+    return launch_tiles(p, own_keys, true, false, {}, {}, msg);
   void* ws = nullptr;
   Partial part;
   int rc = kOk;
-  if (p.Nk > 0) {
+  if (p.Nk > 0 || p.P > kMaxSeqLen) {
     const cudaError_t e = scratch_alloc_async(&ws, static_cast<size_t>(rows) * (4 + p.D) * sizeof(float), p.stream);
     if (e != cudaSuccess) {
       *msg = cudaGetErrorString(e);
@@ -298,16 +425,16 @@ int launch_shared_prefix(const CrossParams& p, const char** msg) {
     }
     part.ml = static_cast<float*>(ws);
     part.o = part.ml + rows * 4;
+  }
+  if (p.Nk > 0) {
     CrossParams own = p;
     own.P = 0;
-    own.lse = nullptr;
-    if (p.H / p.Hkv * p.Nq <= kRowsTile) {
+    if (group_rows <= kRowsTile) {
       own.part_ml = part.ml;
       own.part_o = part.o;
       rc = launch_attn_rows(own, msg);
     } else {
-      const Keys keys{p.k, p.v, p.k_stride, p.v_stride, p.Nk, false};
-      rc = launch_tiles(own, keys, true, {}, part, msg);
+      rc = launch_tiles(own, own_keys, false, true, {}, part, msg);
     }
   }
   // A prefix longer than a launch's live-tile lists cover goes in stretches.
@@ -317,12 +444,7 @@ int launch_shared_prefix(const CrossParams& p, const char** msg) {
     const Keys keys{static_cast<const uint16_t*>(p.k_prefix) + at * ks[2],
                     static_cast<const uint16_t*>(p.v_prefix) + at * vs[2], ks, vs, n, true};
     const bool last = at + n == p.P;
-    if (!last && ws == nullptr) {
-      *msg = "attention: prefix too long";
-      rc = kErrUnsupportedN;
-      break;
-    }
-    rc = launch_tiles(p, keys, true, part, last ? Partial{} : part, msg);
+    rc = launch_tiles(p, keys, false, true, at > 0 || p.Nk > 0 ? part : Partial{}, last ? Partial{} : part, msg);
   }
   if (ws != nullptr) {
     const cudaError_t ef = cudaFreeAsync(ws, p.stream);
