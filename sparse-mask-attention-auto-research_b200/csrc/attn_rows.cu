@@ -16,7 +16,7 @@
 // exponentials on padding rows (16384 per 128 keys against the 2048 here).
 //
 // A work unit is (batch, key head, 16-row tile, piece of the keys).  Its four
-// warps work alone: each takes every fourth 32-key chunk of the unit, loads
+// warps work alone: each takes every fourth chunk (8 KiB of keys) of the unit, loads
 // it by TMA into its own ring of kStages stages (128-byte swizzle, one
 // mbarrier per stage), and keeps its own running maximum, sum and O in
 // registers; nothing in the loop waits for another warp.  At the end the
@@ -47,7 +47,6 @@ namespace {
 constexpr int kRows = kRowsTile;  // one m16n8k16 fragment
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kChunk = 32;   // keys a warp takes at a time
 constexpr int kStages = 3;   // chunks in flight per warp
 constexpr int kBatch = 32;   // chunks whose masks a warp packs ahead
 constexpr int kMaxPieces = 255;
@@ -78,6 +77,9 @@ struct RowsParams {
 
 template <int D>
 struct RowsCfg {
+  // Keys a warp takes at a time: 8 KiB of K and V either way, so that two
+  // blocks (eight warps, 192 KiB of loads in flight) fit an SM.
+  static constexpr int kChunk = D == 64 ? 32 : 16;
   static constexpr int kTile = kChunk * D * 2;       // K or V of a chunk
   static constexpr int kStageBytes = 2 * kTile;
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -93,7 +95,7 @@ struct RowsCtl {
   uint32_t abort_flag;
   uint32_t last;
 };
-static_assert(RowsCfg<128>::kSmem + sizeof(RowsCtl) <= 227 * 1024, "shared memory");
+static_assert(2 * (RowsCfg<128>::kSmem + sizeof(RowsCtl) + 1024) <= 228 * 1024, "two blocks per SM");
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;
@@ -154,11 +156,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
 template <int D, bool BF16, bool kBias>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
     attn_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
                      const __grid_constant__ RowsParams p, const __grid_constant__ BiasSpec bias) {
   using C = RowsCfg<D>;
+  constexpr int kChunk = C::kChunk, NT = kChunk / 8;  // keys of a chunk, 8-key tiles of it
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   if ((base & 1023u) != 0u) {
@@ -198,17 +201,6 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
     qi[u] = rr - g * p.Nq;
     head[u] = hkv * p.G + g;
   }
-  uint32_t qa[D / 16][4];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const uint16_t* src = p.q + b * p.q_stride[0] + head[u] * p.q_stride[1] + qi[u] * p.q_stride[2] + 2 * (lane & 3);
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      qa[kk][u] = live_row[u] ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
-      qa[kk][2 + u] = live_row[u] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
-    }
-  }
-
   // Chunks: the prefix's, then the sequence's own up to its length.
   int len = p.Nk;
   if (p.lengths != nullptr) len = max(0, min(p.Nk, __ldg(p.lengths + b)));
@@ -229,6 +221,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
+  uint32_t qa[D / 16][4];
+  bool have_q = false;
   const uint32_t ring = base + warp * C::kWarpBytes;
   uint32_t n_issued = 0, n_used = 0;
   bool ok = true;
@@ -266,17 +260,20 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
         const int g = rr / p.Nq;
         const uint8_t* mrow = p.mask + b * p.mask_stride[0] + (hkv * p.G + g) * p.mask_stride[1] +
                               (rr - g * p.Nq) * p.mask_stride[2];
-        for (int i = 0; i < nb; i += 8) {
+        constexpr int kPer = 32 / kChunk;  // chunks per ballot
+        for (int i = 0; i < nb; i += 8 * kPer) {
           uint8_t x[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int key = (c_lo + warp + kWarps * (i0 + i + u) - np) * kChunk + lane;
-            x[u] = (i + u < nb && key >= 0 && key < len) ? __ldg(mrow + key) : 0;
+            const int ii = i + u * kPer + lane / kChunk;
+            const int key = (c_lo + warp + kWarps * (i0 + ii) - np) * kChunk + lane % kChunk;
+            x[u] = (ii < nb && key >= 0 && key < len) ? __ldg(mrow + key) : 0;
           }
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const uint32_t w = __ballot_sync(0xffffffffu, x[u] != 0);
-            if (i + u < nb && lane == 0) ctl.words[warp][i + u][r] = w;
+            const int ii = i + u * kPer + lane;
+            if (lane < kPer && ii < nb) ctl.words[warp][ii][r] = (w >> (lane * kChunk)) & low_bits(kChunk);
           }
         }
       }
@@ -291,6 +288,18 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
     for (int s = 0; s < kStages && ahead != 0u; ++s) {
       issue(i0 + __ffs(ahead) - 1);
       ahead &= ahead - 1u;
+    }
+    if (!have_q) {  // behind the first requests for keys
+      have_q = true;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint16_t* src = p.q + b * p.q_stride[0] + head[u] * p.q_stride[1] + qi[u] * p.q_stride[2] + 2 * (lane & 3);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qa[kk][u] = live_row[u] ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+          qa[kk][2 + u] = live_row[u] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+        }
+      }
     }
     while (live != 0u) {
       const int i = __ffs(live) - 1;
@@ -313,13 +322,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
         if (pre) w = low_bits(p.P - k0);
         else if (p.mask != nullptr) w = ctl.words[warp][i][p.mask_rows ? 0 : (lane >> 2) + 8 * u];
         else w = low_bits(limit[u] - k0);
-        word[u] = live_row[u] ? w : 0u;
+        word[u] = live_row[u] ? w & low_bits(kChunk) : 0u;
       }
       const uint32_t sK = ring + s * C::kStageBytes, sV = sK + C::kTile;
       // V of keys no row keeps: cleared (see the head comment).
       const uint32_t kept = __reduce_or_sync(0xffffffffu, word[0] | word[1]);
-      if (kept != 0xFFFFFFFFu) {
-        if (((kept >> lane) & 1u) == 0u) {
+      if (kept != low_bits(kChunk)) {
+        if (lane < kChunk && ((kept >> lane) & 1u) == 0u) {
           uint8_t* v = smem + warp * C::kWarpBytes + s * C::kStageBytes + C::kTile + lane * 128;
 #pragma unroll
           for (int x = 0; x < D / 8; ++x)
@@ -329,16 +338,16 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
         __syncwarp();
       }
 
-      float sc[4][4];
+      float sc[NT][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
       const int mat = lane >> 3, mrow = lane & 7;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
-        for (int n = 0; n < 4; n += 2) {
+        for (int n = 0; n < NT; n += 2) {
           const int key = (n + (mat >> 1)) * 8 + mrow;
           const int ch = kk * 2 + (mat & 1);
           uint32_t kb[4];
@@ -349,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       }
       // Scores in units of log2, masked; then the running maximum.
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] *= p.scale_log2;
       if constexpr (kBias) {
@@ -361,13 +370,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           if (b_lo == b_hi) {  // buckets are monotone on each side, so one bucket holds the whole chunk
             const float add = bias_value<BF16>(bias, b_lo, head[u]) * kLog2e;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < NT; ++n) {
               sc[n][2 * u] += add;
               sc[n][2 * u + 1] += add;
             }
           } else {
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int d = d0 + n * 8 + 2 * (lane & 3) + e;
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       for (int u = 0; u < 2; ++u) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t bit = 1u << (n * 8 + 2 * (lane & 3) + e);
@@ -410,9 +419,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       // P, rounded to the inputs' type for the product with V (the type the
       // matrix instruction takes); O is divided by the sum of the rounded
       // values, the LSE uses the unrounded ones.
-      uint32_t pa[2][4];
+      uint32_t pa[kChunk / 16][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float p0 = ex2f(sc[n][2 * u] - mu[u]), p1 = ex2f(sc[n][2 * u + 1] - mu[u]);
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           pa[n >> 1][(n & 1) * 2 + u] = w;
         }
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < kChunk / 16; ++ks) {
 #pragma unroll
         for (int n = 0; n < D / 8; n += 2) {
           const int key = ks * 16 + (mat & 1) * 8 + mrow;
@@ -622,8 +631,9 @@ int launch(const CrossParams& a, const char** msg) {
   p.mask_rows = a.mask != nullptr && (a.Nq == 1 || a.mask_stride[2] == 0) && (p.G == 1 || a.mask_stride[1] == 0) ? 1 : 0;
   p.scale_log2 = a.scale * kLog2e;
   const int64_t items = a.B * a.Hkv * p.RT;
+  constexpr int kChunk = C::kChunk;
   const int64_t chunks = (a.P + kChunk - 1) / kChunk + (a.Nk + kChunk - 1) / kChunk;
-  p.pieces = choose_pieces(items, chunks, static_cast<int64_t>(dp.sms) * (D == 64 ? 2 : 1));
+  p.pieces = choose_pieces(items, chunks, 2 * static_cast<int64_t>(dp.sms));
   const int64_t units = items * p.pieces;
   if (units > 0x7FFFFFFFll) {
     *msg = "attention: too many query rows";
