@@ -212,7 +212,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   int limit[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) limit[u] = p.lengths != nullptr ? len - p.Nq + 1 + qi[u] : len;
-  const int off = kBias ? bias_offset_of(bias, b) : 0;
+  // kBias: range of the tile's queries, of the relative positions between
+  // which buckets change, and each row's bias beyond them.
+  int off = 0, t_lo = 0, t_hi = 0, bias_lo = 0, bias_hi = 0;
+  float far_lo[2] = {0.f, 0.f}, far_hi[2] = {0.f, 0.f};
+  if constexpr (kBias) {
+    off = bias_offset_of(bias, b);
+    t_hi = p.Nq - 1;
+    bias_lo = -ctl.starts[bias.side - 1];
+    bias_hi = bias.two_sided ? -bias_lo : 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!live_row[u]) continue;
+      far_lo[u] = bias_value<BF16>(bias, bias.side - 1, head[u]) * kLog2e;
+      far_hi[u] = bias_value<BF16>(bias, bias.two_sided ? 2 * bias.side - 1 : 0, head[u]) * kLog2e;
+    }
+  }
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lr[2] = {0.f, 0.f};
   float o[D / 8][4];
@@ -362,25 +377,34 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] *= p.scale_log2;
       if constexpr (kBias) {
+        // A chunk beyond the last bucket's start for all rows has one bias per
+        // row, kept in registers.  Otherwise lane x finds the bias of the
+        // chunk's key x, row by row, and the rows' threads fetch it from there.
+        const int d_first = k0 - t_hi - off, d_last = k0 + kChunk - 1 - t_lo - off;
+        if (d_last <= bias_lo || d_first >= bias_hi) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (!live_row[u]) continue;
-          const int d0 = k0 - qi[u] - off;  // relative position of the chunk's first key
-          const int b_lo = bias_bucket(bias, ctl.starts, d0), b_hi = bias_bucket(bias, ctl.starts, d0 + kChunk - 1);
-          if (b_lo == b_hi) {  // buckets are monotone on each side, so one bucket holds the whole chunk
-            const float add = bias_value<BF16>(bias, b_lo, head[u]) * kLog2e;
+          for (int u = 0; u < 2; ++u) {
+            const float add = d_last <= bias_lo ? far_lo[u] : far_hi[u];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               sc[n][2 * u] += add;
               sc[n][2 * u + 1] += add;
             }
-          } else {
+          }
+        } else {
+          const int rows = min(kRows, p.R - rt * kRows);
+#pragma unroll 2
+          for (int r = 0; r < rows; ++r) {
+            const int rr = rt * kRows + r, g = rr / p.Nq;
+            const int bucket = bias_bucket(bias, ctl.starts, k0 + lane - (rr - g * p.Nq) - off);
+            const float x = bias_value<BF16>(bias, bucket, hkv * p.G + g) * kLog2e;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int d = d0 + n * 8 + 2 * (lane & 3) + e;
-                sc[n][2 * u + e] += bias_value<BF16>(bias, bias_bucket(bias, ctl.starts, d), head[u]) * kLog2e;
+                const float y = __shfl_sync(0xffffffffu, x, n * 8 + 2 * (lane & 3) + e);
+                if (r == (lane >> 2)) sc[n][e] += y;
+                if (r == (lane >> 2) + 8) sc[n][2 + e] += y;
               }
           }
         }
