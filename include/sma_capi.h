@@ -222,9 +222,12 @@ typedef struct sma_attn_args {
   int32_t bias_two_sided;
   void* out;   /* [B, H, Nq, D] contiguous */
   float* lse;  /* [B, H, Nq] natural-log sum of exponentials, or NULL */
-  const void* words;      /* mask packed by sma_pack_mask_rows */
-  int64_t word_stride[3];
-  float* bias_distance;   /* room for H * SMA_BIAS_DISTANCE_LEN floats */
+  /* Of the 128-row tile entries: room for the packed mask, int32 words
+   * [B, H, Nq, 4 * ceil(Nk / 128)] with length 1 for an axis whose mask_stride
+   * is 0 (bit b of word w: column 32 w + b, 0 past Nk). */
+  void* words;
+  float* bias_distance; /* room for H * SMA_BIAS_DISTANCE_LEN floats */
+  void* out_lo;         /* O minus its rounded value, like out, or NULL */
 } sma_attn_args;
 
 /*
@@ -242,25 +245,14 @@ typedef struct sma_attn_args {
 SMA_API int sma_rows_attn_fwd(const sma_attn_args* args, void* stream);
 
 /*
- * Packs a bool mask [Bm, Hm, Qm, Nk] with the given batch, head and query
- * strides (bytes, >= 0; the last axis contiguous) into words [Bm, Hm, Qm, W],
- * W = 4 * ceil(Nk / 128), contiguous: bit b of word w of a row is the mask at
- * column 32 w + b, 0 at columns >= Nk.  `words` is 16-byte aligned.
- * No reference counterpart (the reference's masks are square and dense).
- */
-SMA_API int sma_pack_mask_rows(const void* mask, const int64_t* stride, void* words, int64_t Bm, int64_t Hm, int64_t Qm,
-                               int64_t Nk, void* stream);
-
-/*
- * Attention forward for many query rows, on 128-row tiles: `words` (with
- * word_stride, 0 for an axis the mask does not depend on; NULL keeps every
- * key) takes the place of `mask`, and a bias also needs bias_distance, which
- * is filled here (the backward reads it).  Queries of the heads that share a
- * key head fill a tile together when Nq <= 64.  Nk <= SMA_MAX_SEQ_LEN, no
- * prefix; otherwise as sma_rows_attn_fwd, except that a key which only some
- * rows of a tile keep must hold finite values (a key that a mask row shared
- * by the tile, or the length, leaves out may hold anything).
- * Rows that keep no key get out = 0 and lse = -FLT_MAX.
+ * Attention forward for many query rows, on 128-row tiles.  A mask is packed
+ * into `words` first, and a bias laid out in bias_distance (the backward reads
+ * both, with the lse and out_lo, which training needs).  Queries of the heads
+ * that share a key head fill a tile together when Nq <= 64.
+ * Nk <= SMA_MAX_SEQ_LEN, no prefix; otherwise as sma_rows_attn_fwd, except
+ * that a key which only some rows of a tile keep must hold finite values (a
+ * key that a mask row shared by the tile, or the length, leaves out may hold
+ * anything).  Rows that keep no key get out = 0 and lse = -FLT_MAX.
  */
 SMA_API int sma_cross_attn_fwd(const sma_attn_args* args, void* stream);
 
@@ -272,15 +264,15 @@ SMA_API int sma_cross_attn_fwd(const sma_attn_args* args, void* stream);
 SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
 
 /*
- * Backward of sma_cross_attn_fwd: `args` are the forward's, with the out and
- * lse it wrote (lse not NULL) and its bias_distance.  From dout [B, H, Nq, D]
+ * Backward of sma_cross_attn_fwd: `args` are the forward's, with the out, lse,
+ * out_lo, words and bias_distance it wrote (`mask` itself is not read).  From dout [B, H, Nq, D]
  * writes dq [B, H, Nq, D], dk and dv [B, Hkv, Nk, D] (summed over the query
  * heads of a key head) and, with a bias, dtable [bias_buckets, H], all
  * contiguous and of `dtype`; formulas as for sma_attn_bwd, and
  *   dtable[bucket, h] = sum of dS over the pairs in the bucket.
  * Scratch: dq_accum (FP32 [B, H, Nq, D]), delta (FP32 [B, H, Nq]) and, with a
  * bias, bias_part (FP32, sma_cross_attn_bwd_bias_floats(args) elements).
- * At most 1024 tiles of 128 query rows per key head (SMA_ERR_UNSUPPORTED_N).
+ * At most 2048 steps of 64 query rows per key head (SMA_ERR_UNSUPPORTED_N).
  * All values of K, V, Q and dO must be finite.  dq is accumulated by atomic
  * adds in FP32, so its last bits can differ from run to run; dk, dv and
  * dtable do not.

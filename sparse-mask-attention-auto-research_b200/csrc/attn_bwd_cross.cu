@@ -1,12 +1,1044 @@
-// Attention backward of queries and keys of different lengths, with shared key
-// heads and a relative position bias: attn_bwd.cuh (kX) and the sum of the
-// bias gradient over its buckets.
-#include "attn_bwd.cuh"
-
+// Attention backward of queries and keys of different lengths (sm_100a), head
+// dims 64 and 128, with key heads shared by query heads and a relative
+// position bias and its gradient.
+//
+//   P  = exp(scale * q k^T + bias - lse) where the mask keeps the pair, else 0
+//   dV = P^T dO,  dS = P * (dO V^T - Delta),  Delta_i = sum_d dO_id O_id
+//   dQ = scale * dS K,  dK = scale * dS^T Q,  dtable[bucket, h] = sum of dS over the bucket's pairs
+//
+// Kernels, in stream order: cross_delta_kernel (Delta; clears the FP32 dQ
+// accumulator), cross_bwd_kernel, cross_dq_kernel (accumulator -> dq) and,
+// with a bias, bias_reduce_kernel.
+//
+// cross_bwd_kernel is persistent, one CTA per SM, over items (batch, key head,
+// 128-key tile).  K and V of the item stay in shared memory, dK and dV
+// accumulate in TMEM over all query heads that share the key head, and the CTA
+// walks the item's live steps of 64 query rows (those whose mask block keeps
+// a pair).  Two steps are in flight, each with its own S^T / dP^T columns and
+// its own four element-wise warps, so that while one step's exponentials run,
+// the tensor core works on the other's products:
+//
+//   MMA warp, step s: S^T = K Q_s^T, dP^T = V dO_s^T             (M = 128 keys, N = 64 queries)
+//             step s-1: dV += P^T dO (P from TMEM), dK += dS^T Q (dS from shared memory), dQ product
+//   warps 4g..4g+3, steps s = g mod 2: P, dS in registers (thread = key); P
+//             rounded over the S^T columns, dS to shared memory
+//
+// What bounds it: per 64 queries, 16 (D = 64: four S^T, four dP^T, four dV,
+// four dK) tensor instructions at about 64 cycles, the dQ product, and 8192
+// exponentials with some ten instructions each; with the two in turn (one
+// step in flight) each waited for the other.
+//
+// The dQ product: D = 64 takes the dS of two steps as one 128-row operand,
+// dQ = dS K, in TMEM columns of its own (two buffers).  D = 128 has no columns
+// left and computes dQ^T = K^T dS^T of one step over the dP^T columns, which
+// the element-wise warps have read by then.  Four epilogue warps add it into
+// the FP32 accumulator by TMA bulk reduce-adds.
+//
+// Warps: 0-7 element-wise, 8 loader (TMA; mask words, LSE and Delta staged in
+// shared memory), 9 MMA issuer and TMEM owner, 10-13 epilogue, 14 scanner
+// (each item's live steps, kSlots items ahead).  Every wait is bounded and
+// reports through the device error word.
+//
+// P and dS are rounded to the inputs' type, the operand type of the products;
+// Delta uses O with the residual of its rounding that the forward kept, since
+// an error there shifts a whole row of dS.
 #include <algorithm>
+#include <cfloat>
+
+#include "attn_math.cuh"
+#include "rel_bias.cuh"
+#include "sma_internal.h"
+#include "sma_ptx.cuh"
 
 namespace sma {
 namespace {
+
+constexpr int kKeys = 128;  // keys of an item
+constexpr int kQ = 64;      // query rows of a step
+constexpr int kTmemCols = 512;
+constexpr int kEwWarps = 8, kLoaderWarp = 8, kMmaWarp = 9, kEpiWarp = 10, kScanWarp = 14;
+constexpr int kThreads = 15 * 32;
+// Items whose live lists the scanner publishes ahead, and words of a list: one
+// bit per step, up to 2048 steps of the heads that share a key head.
+constexpr int kSlots = 4;
+constexpr int kListWords = 64;
+constexpr int kMaxSteps = 32 * kListWords;
+
+// TMEM columns: S^T of stage g, dP^T of stage g, dV, dK, and for D = 64 two dQ buffers.
+__host__ __device__ constexpr uint32_t col_s(int g) { return 64u * g; }
+__host__ __device__ constexpr uint32_t col_dp(int g) { return 128u + 64u * g; }
+constexpr uint32_t kColDV = 256;
+
+template <int D>
+struct Cfg {
+  static constexpr int kDChunks = D / 64;
+  static constexpr uint32_t kColDK = kColDV + D;
+  static constexpr bool kPairDQ = D == 64;
+  __host__ __device__ static constexpr uint32_t col_dq(int b) { return 384u + 64u * b; }  // D = 64
+  static constexpr int kKVBytes = kKeys * D * 2;
+  static constexpr int kKVBufs = D == 64 ? 2 : 1;
+  static constexpr int kQBytes = kQ * D * 2;
+  static constexpr int kRing = D == 64 ? 4 : 3;      // staged steps
+  static constexpr int kDSBytes = kKeys * kQ * 2;
+  static constexpr int kDSSlots = kPairDQ ? 4 : 2;
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = kKVBufs * kKVBytes;
+  static constexpr int kOffQ = 2 * kKVBufs * kKVBytes;
+  static constexpr int kOffDO = kOffQ + kRing * kQBytes;
+  static constexpr int kOffDS = kOffDO + kRing * kQBytes;
+  static constexpr int kOffDQ = kOffDS + kDSSlots * kDSBytes;  // 4 KiB box per epilogue warp
+  static constexpr int kOffMask = kOffDQ + 4 * 4096;           // [ring][4 words][64 rows]
+  static constexpr int kOffLse = kOffMask + kRing * 4 * kQ * 4;
+  static constexpr int kOffDelta = kOffLse + kRing * kQ * 4;
+  static constexpr int kOffCtl = kOffDelta + kRing * kQ * 4;
+};
+
+struct Ctl {
+  uint64_t kv_full[2], kv_free[2];
+  uint64_t acc_free;               // dV and dK of a live item read out of TMEM
+  uint64_t ld_full[4], tile_free[4];
+  uint64_t st_full[2];             // S^T and dP^T of a stage complete
+  uint64_t p_full[2];              // its P in TMEM and dS in shared memory
+  uint64_t pt_free[2];             // D = 64: its dV and dK products complete
+  uint64_t dq_full[2], dq_free[2];  // D = 64: per dQ buffer (pair of steps); D = 128: per stage
+  uint64_t item_full[kSlots], item_free[kSlots];
+  uint64_t drain;
+  uint32_t live_bits[kSlots][kListWords];
+  uint32_t n_live[kSlots];
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+
+template <int D>
+constexpr size_t smem_bytes() {
+  return Cfg<D>::kOffCtl + sizeof(Ctl);
+}
+static_assert(smem_bytes<64>() <= 227 * 1024 && smem_bytes<128>() <= 227 * 1024, "shared memory budget");
+static_assert(smem_bytes<64>() > 114 * 1024 && smem_bytes<128>() > 114 * 1024, "one CTA per SM: it takes all of TMEM");
+static_assert(Cfg<64>::kOffDQ % 1024 == 0 && Cfg<128>::kOffDQ % 1024 == 0, "swizzle atoms");
+
+// Geometry.  Step ht * QT1 + qt of an item holds tn queries from 64 qt of the
+// hb heads from ht * hb of the key head's group (hb > 1 only when the queries
+// of several heads fit one step); rows past tn * hb are kept zero in shared
+// memory, since the products run over them.
+struct BwdGeo {
+  int B, H, Hkv, Nq, Nk;
+  int tn, hb, gh, rows;    // rows = tn * hb; gh = G / hb
+  int QT1;                 // 64-row steps of Nq
+  const uint32_t* words;   // packed mask rows (16-byte aligned), or nullptr: every key is kept
+  int64_t word_stride[3];  // batch, head, query, in words (0: broadcast)
+  int one_row;             // all query rows of an item have the same mask row
+  // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
+  const float* bias;
+  const int32_t* bias_offsets;
+  int bias_offset, bias_lo, bias_hi, bias_len;
+  // Its gradient by relative position: dS summed along the diagonals of every
+  // 32 x 32 block that overlaps (bias_lo, bias_hi), [B*H][KB][slots][64]
+  // (entry d - 32 (kb - qb) + off, mod 64), and the sums of the blocks beyond
+  // on either side, [B*H][KB][2 (stage)][2 (low, high)].
+  float* near_part;
+  float* far_part;
+  int KB, QB, slots, slot_by_query;
+};
+
+// Block difference j = kb - qb of the 32 x 32 blocks that overlap (lo, hi):
+// their relative positions are 32 j - off + [-31, 31].  The largest such j.
+__host__ __device__ inline int bias_block_max(int hi, int off) {
+  const int x = hi + off + 30;  // 32 j <= x
+  return x >= 0 ? x / 32 : -((-x + 31) / 32);
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u); }
+
+// Next set bit of a live list from cursor (w, x): the step index, or -1.
+__device__ __forceinline__ int next_live(const uint32_t* bits, int& w, uint32_t& x) {
+  while (x == 0u) {
+    if (++w >= kListWords) return -1;
+    x = bits[w];
+  }
+  const int b = __ffs(x) - 1;
+  x &= x - 1u;
+  return w * 32 + b;
+}
+
+// Delta[row] = sum_d dO[row, d] * (O[row, d] + its rounding residual) in FP32,
+// D/8 threads per row; each thread also clears its 8 elements of the FP32 dQ
+// accumulator.  Bound by HBM: three 16-bit reads and a 32-bit write per element.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256)
+    cross_delta_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ out, const uint4* __restrict__ out_lo,
+                       float* __restrict__ delta, float4* __restrict__ dq_acc, int64_t rows) {
+  constexpr int kPerRow = D / 8;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const int64_t gid = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = gid / kPerRow;
+  float acc = 0.f;
+  if (row < rows) {
+    const uint4 a = __ldg(dout + gid), b = __ldg(out + gid), c = __ldg(out_lo + gid);
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    dq_acc[2 * gid] = zero;
+    dq_acc[2 * gid + 1] = zero;
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w}, cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = unpack2<BF16>(aw[e]), y = unpack2<BF16>(bw[e]), z = unpack2<BF16>(cw[e]);
+      acc = fmaf(x.x, y.x + z.x, acc);
+      acc = fmaf(x.y, y.y + z.y, acc);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < kPerRow; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (row < rows && (threadIdx.x % kPerRow) == 0) delta[row] = acc;
+}
+
+// dq[i] = acc[i] in the input dtype, 8 elements per thread.
+template <bool BF16>
+__global__ void __launch_bounds__(256) cross_dq_kernel(const float4* __restrict__ acc, uint4* __restrict__ dq, int64_t n8) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n8) return;
+  const float4 a = __ldcs(acc + 2 * i), b = __ldcs(acc + 2 * i + 1);
+  dq[i] = make_uint4(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w), pack2<BF16>(b.x, b.y), pack2<BF16>(b.z, b.w));
+}
+
+// Sums of a 32 x 32 block along its diagonals.  ds[e] is lane t's element of
+// column e; diagonal k = t - e.  On return lane k holds diagonal k >= 0 in
+// `pos` and lane 32 + k diagonal k < 0 in `neg`.  Neighbouring column blocks
+// of width w are added with the right one shifted by w lanes; what the shift
+// carries round the end belongs to the negative diagonals.
+__device__ __forceinline__ void diagonal_sums(const float (&ds)[32], int lane, float& pos, float& neg) {
+  float m[16], n[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float r = __shfl_sync(0xffffffffu, ds[2 * i + 1], (lane + 1) & 31);
+    m[i] = ds[2 * i] + (lane < 31 ? r : 0.f);
+    n[i] = lane < 31 ? 0.f : r;
+  }
+#pragma unroll
+  for (int w = 2; w < 32; w *= 2) {
+#pragma unroll
+    for (int i = 0; i < 16 / w; ++i) {
+      const float r = __shfl_sync(0xffffffffu, m[2 * i + 1], (lane + w) & 31);
+      const float r2 = __shfl_sync(0xffffffffu, n[2 * i + 1], (lane + w) & 31);
+      m[i] = m[2 * i] + (lane < 32 - w ? r : 0.f);
+      n[i] = n[2 * i] + (lane < 32 - w ? r2 : r);
+    }
+  }
+  pos = m[0];
+  neg = n[0];
+}
+
+template <int D, bool BF16, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ CUtensorMap tm_dq, const float* __restrict__ lse,
+                     const float* __restrict__ delta, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int KT,
+                     int total_items, float scale, const __grid_constant__ BwdGeo x, uint32_t* err_word,
+                     uint64_t timeout_ns) {
+  using C = Cfg<D>;
+  constexpr int kRing = C::kRing;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  if ((base & 1023u) != 0u) {
+    if (threadIdx.x == 0) atomicOr(err_word, kDevErrLayout);
+    return;
+  }
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + C::kOffCtl);
+  // Per ring slot b: word w of query row i at s_mask[(b * 4 + w) * kQ + i];
+  // -LSE * log2(e) and -Delta per query row at s_lse / s_delta [b * kQ + i]
+  // (negated, so that the element-wise pass adds them in packed pairs).
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  float* s_lse = reinterpret_cast<float*>(smem + C::kOffLse);
+  float* s_delta = reinterpret_cast<float*>(smem + C::kOffDelta);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // CTA c takes items c, c + G, ...: the CTAs running at one time share the
+  // Q and dO of a few heads in L2.  Counters over all items of the CTA, the
+  // same in every role: j items (list slot j % kSlots), li items with a live
+  // step (K/V buffer li % kKVBufs), lt live steps (ring slot lt % kRing), the
+  // uses of each stage (step t of an item uses stage t & 1) and lp pairs of
+  // steps of one item (D = 64: dQ buffer lp & 1).
+  const int G = static_cast<int>(gridDim.x);
+  const int n_items = (total_items - static_cast<int>(blockIdx.x) + G - 1) / G;
+  const int VT = x.gh * x.QT1;
+  volatile uint32_t* abort_flag = &ctl.abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&ctl.kv_full[b]), 1);
+      mbar_init(smem_u32(&ctl.kv_free[b]), 1);
+      mbar_init(smem_u32(&ctl.st_full[b]), 1);
+      mbar_init(smem_u32(&ctl.p_full[b]), 4);
+      mbar_init(smem_u32(&ctl.pt_free[b]), 1);
+      mbar_init(smem_u32(&ctl.dq_full[b]), 1);
+      mbar_init(smem_u32(&ctl.dq_free[b]), 4);
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(smem_u32(&ctl.ld_full[b]), 1);
+      mbar_init(smem_u32(&ctl.tile_free[b]), 5);  // a stage's element-wise warps and the MMA issuer
+    }
+    for (int sl = 0; sl < kSlots; ++sl) {
+      mbar_init(smem_u32(&ctl.item_full[sl]), 1);
+      mbar_init(smem_u32(&ctl.item_free[sl]), kEwWarps + 6);  // element-wise, loader, MMA, 4 epilogue warps
+    }
+    mbar_init(smem_u32(&ctl.acc_free), 4);
+    mbar_init(smem_u32(&ctl.drain), 1);
+    ctl.abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (x.rows < kQ) {  // rows the copies never write
+    for (int i = threadIdx.x; i < (C::kOffDS - C::kOffQ) / 16; i += kThreads)
+      *reinterpret_cast<uint4*>(smem + C::kOffQ + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&ctl.tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem_base;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+
+  auto fail = [&]() {
+    ctl.abort_flag = 1;
+    atomicOr(err_word, kDevErrTimeout);
+  };
+  // Batch, key head and key tile of item j, and the first head of the group.
+  struct Item {
+    int b, hkv, kt, h0;
+  };
+  auto item_at = [&](int j) -> Item {
+    const int w = static_cast<int>(blockIdx.x) + j * G;
+    const int bh = w / KT;
+    Item it;
+    it.kt = w - bh * KT;
+    it.b = bh / x.Hkv;
+    it.hkv = bh - it.b * x.Hkv;
+    it.h0 = it.hkv * (x.gh * x.hb);
+    return it;
+  };
+  auto step_head = [&](int v) { return v / x.QT1 * x.hb; };  // relative to h0
+  auto step_q0 = [&](int v) { return v % x.QT1 * kQ; };
+  // Whole-warp wait.
+  auto wait_all = [&](uint64_t& bar, uint32_t parity) -> bool {
+    const bool all = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&bar), parity, abort_flag, timeout_ns));
+    tc_fence_after();
+    return all;
+  };
+  auto arrive_warp = [&](uint64_t& bar) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bar));
+  };
+
+  if (warp == kLoaderWarp) {
+    // ================================================================ loader
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      tma_prefetch_desc(&tm_do);
+      tma_prefetch_desc(&tm_dq);
+    }
+    bool ok = true;
+    int lt = 0, li = 0;
+    int last_copy = -1;
+    // Query and head of this lane's rows (lane, lane + 32) within a step.
+    int rt[2], rh[2];
+    bool rin[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = lane + 32 * u;
+      rin[u] = i < x.rows;
+      rh[u] = rin[u] ? i / x.tn : 0;
+      rt[u] = rin[u] ? i - rh[u] * x.tn : 0;
+    }
+    // Mask words, LSE and Delta of step v of an item, two rows per lane: all
+    // loads issued at once, into registers.
+    auto fetch = [&](const Item& it, int v, uint4 (&w4)[2], float (&l2)[2], float (&de)[2]) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = step_q0(v) + rt[u], h = it.h0 + step_head(v) + rh[u];
+        const bool in = rin[u] && t < x.Nq;
+        const int64_t row = in ? (static_cast<int64_t>(it.b) * x.H + h) * x.Nq + t : 0;
+        w4[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (in) {
+          if (x.words == nullptr) {
+            w4[u] = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
+          } else {
+            w4[u] = __ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] + h * x.word_stride[1] +
+                                                         t * x.word_stride[2] + it.kt * 4));
+          }
+        }
+        l2[u] = in ? __ldg(lse + row) : 0.f;
+        de[u] = in ? __ldg(delta + row) : 0.f;
+      }
+    };
+    auto issue_kv = [&](const Item& it) -> bool {
+      const int b = li % C::kKVBufs;
+      if (li >= C::kKVBufs &&
+          !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&ctl.kv_free[b]), ((li - C::kKVBufs) / C::kKVBufs) & 1,
+                                                     abort_flag, timeout_ns)))
+        return false;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&ctl.kv_full[b]);
+        mbar_arrive_expect_tx(bar, 2 * C::kKVBytes);
+#pragma unroll
+        for (int dc = 0; dc < C::kDChunks; ++dc) {
+          tma_load_4d(base + C::kOffK + b * C::kKVBytes + dc * kKeys * 128, &tm_k, bar, dc * 64, it.kt * kKeys, it.hkv,
+                      it.b);
+          tma_load_4d(base + C::kOffV + b * C::kKVBytes + dc * kKeys * 128, &tm_v, bar, dc * 64, it.kt * kKeys, it.hkv,
+                      it.b);
+        }
+      }
+      ++li;
+      return true;
+    };
+    auto stage = [&](const Item& it, int v, const uint4 (&w4)[2], const float (&l2)[2], const float (&de)[2]) -> bool {
+      const int b = lt % kRing;
+      if (lt >= kRing &&
+          !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&ctl.tile_free[b]), ((lt - kRing) / kRing) & 1,
+                                                     abort_flag, timeout_ns)))
+        return false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = lane + 32 * u;
+        const uint32_t w[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          s_mask[(b * 4 + k) * kQ + i] = w[k] & low_bits(x.Nk - it.kt * kKeys - 32 * k);
+        // -FLT_MAX (a row with no kept key) becomes +inf here; such a row has
+        // no mask bit, so its P is 0 by the select and never uses this value.
+        s_lse[b * kQ + i] = -(l2[u] * kLog2e);
+        s_delta[b * kQ + i] = -de[u];
+      }
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&ctl.ld_full[b]);
+        const int q0 = step_q0(v), h = it.h0 + step_head(v);
+        mbar_arrive_expect_tx(bar, 2 * x.rows * D * 2);
+#pragma unroll
+        for (int dc = 0; dc < C::kDChunks; ++dc) {
+          tma_load_4d(base + C::kOffQ + b * C::kQBytes + dc * kQ * 128, &tm_q, bar, dc * 64, q0, h, it.b);
+          tma_load_4d(base + C::kOffDO + b * C::kQBytes + dc * kQ * 128, &tm_do, bar, dc * 64, q0, h, it.b);
+        }
+        last_copy = lt;
+      }
+      ++lt;
+      return true;
+    };
+    // The loads of the next live step are issued before this one waits for
+    // its slot; at an item's last step, those of the next item's first.
+    uint4 nw[2];
+    float nl[2], nd[2];
+    bool have_next = false;
+    for (int j = 0; ok && j < n_items; ++j) {
+      const int sl = j % kSlots;
+      if (!wait_all(ctl.item_full[sl], (j / kSlots) & 1)) {
+        ok = false;
+        break;
+      }
+      const int n = static_cast<int>(ctl.n_live[sl]);
+      if (n > 0) {
+        const Item it = item_at(j);
+        if (!issue_kv(it)) {
+          ok = false;
+          break;
+        }
+        int cw = 0;
+        uint32_t cx = ctl.live_bits[sl][0];
+        int v_next = next_live(ctl.live_bits[sl], cw, cx);
+        if (!have_next) fetch(it, v_next, nw, nl, nd);
+        have_next = false;
+        for (int t = 0; t < n; ++t) {
+          const int v = v_next;
+          uint4 w4[2];
+          float l2[2], de[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            w4[u] = nw[u];
+            l2[u] = nl[u];
+            de[u] = nd[u];
+          }
+          if (t + 1 < n) {
+            v_next = next_live(ctl.live_bits[sl], cw, cx);
+            fetch(it, v_next, nw, nl, nd);
+          } else if (j + 1 < n_items) {
+            // Published kSlots items ahead of the slowest reader, so never
+            // behind this warp's own release.
+            const int sl1 = (j + 1) % kSlots;
+            if (!wait_all(ctl.item_full[sl1], ((j + 1) / kSlots) & 1)) {
+              ok = false;
+              break;
+            }
+            if (ctl.n_live[sl1] > 0u) {
+              int w1 = 0;
+              uint32_t x1 = ctl.live_bits[sl1][0];
+              const int v1 = next_live(ctl.live_bits[sl1], w1, x1);
+              fetch(item_at(j + 1), v1, nw, nl, nd);
+              have_next = true;
+            }
+          }
+          if (!stage(it, v, w4, l2, de)) {
+            ok = false;
+            break;
+          }
+        }
+        if (!ok) break;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_free[sl]));
+    }
+    if (!ok && lane == 0) {
+      fail();
+      // Let the copies this warp started land before the CTA exits.
+      uint32_t zero = 0;
+      for (int jj = li - C::kKVBufs; jj < li; ++jj)
+        if (jj >= 0) mbar_wait_bounded(smem_u32(&ctl.kv_full[jj % C::kKVBufs]), (jj / C::kKVBufs) & 1, &zero, timeout_ns);
+      for (int g = last_copy - kRing + 1; g <= last_copy; ++g)
+        if (g >= 0) mbar_wait_bounded(smem_u32(&ctl.ld_full[g % kRing]), (g / kRing) & 1, &zero, timeout_ns);
+    }
+  } else if (warp == kMmaWarp) {
+    // ================================================================ MMA issuer
+    bool ok = true;
+    if (lane == 0) {
+      constexpr int kBf = BF16 ? 1 : 0;
+      constexpr uint32_t idesc_s = make_idesc_f16(kKeys, kQ, kBf, 0);                // S^T, dP^T
+      constexpr uint32_t idesc_kv = make_idesc_f16(kKeys, D, kBf, 1);                // dV, dK (B M/N-major)
+      constexpr uint32_t idesc_q = make_idesc_f16(128, 64, kBf, 1, 1);               // dQ, dQ^T (A and B M/N-major)
+      uint32_t lt = 0, lp = 0, use[2] = {0, 0};
+      int li = 0;
+      // The step whose products are still to be issued.
+      struct {
+        bool on = false;
+        int g, slot, li, kv;
+        bool first, pair_end;
+        int kv_free;
+        uint32_t use;
+      } pend;
+      auto wait = [&](uint64_t& bar, uint32_t parity) -> bool {
+        return mbar_wait_bounded(smem_u32(&bar), parity, abort_flag, timeout_ns);
+      };
+      auto flush = [&]() -> bool {
+        if (!pend.on) return true;
+        pend.on = false;
+        const int g = pend.g;
+        // P and dS of the step; before the first products of a live item, the
+        // epilogue warps must have read the previous one's dV / dK.
+        if (!wait(ctl.p_full[g], pend.use & 1)) return false;
+        if (pend.first && pend.li > 0 && !wait(ctl.acc_free, (pend.li - 1) & 1)) return false;
+        tc_fence_after();
+        const uint32_t sQ = base + C::kOffQ + pend.slot * C::kQBytes, sDO = base + C::kOffDO + pend.slot * C::kQBytes;
+        const uint32_t sK = base + C::kOffK + pend.kv * C::kKVBytes;
+        const int ds_slot = C::kPairDQ ? static_cast<int>(lp & 1) * 2 + g : g;
+        const uint32_t sDS = base + C::kOffDS + ds_slot * C::kDSBytes;
+        // 16 query rows per instruction: 8 packed TMEM columns of P^T, 32
+        // bytes of dS's rows, 2048 bytes (16 rows of 128) of dO and Q, whose
+        // 64-dim chunks are kQ * 128 bytes apart.
+#pragma unroll
+        for (int kk = 0; kk < kQ / 16; ++kk)
+          mma_ts(tmem + kColDV, tmem + col_s(g) + kk * 8, smem_desc_sw128(sDO + kk * 2048, kQ * 128, 1024), idesc_kv,
+                 (!pend.first || kk > 0) ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < kQ / 16; ++kk)
+          mma_ss(tmem + C::kColDK, smem_desc_sw128(sDS + kk * 32, 16, 1024),
+                 smem_desc_sw128(sQ + kk * 2048, kQ * 128, 1024), idesc_kv, (!pend.first || kk > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&ctl.tile_free[pend.slot]));
+        if constexpr (C::kPairDQ) {
+          mma_commit(smem_u32(&ctl.pt_free[g]));
+          if (pend.pair_end) {
+            // dQ = dS K of the pair (one step's rows are not used when the
+            // item's last pair has only one): 16 keys per instruction, 2048
+            // bytes into dS's two 64-query tiles and K.
+            const int b = lp & 1;
+            if (lp >= 2 && !wait(ctl.dq_free[b], ((lp >> 1) - 1) & 1)) return false;
+            tc_fence_after();
+            const uint32_t sPair = base + C::kOffDS + b * 2 * C::kDSBytes;
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_ss(tmem + C::col_dq(b), smem_desc_sw128(sPair + kk * 2048, C::kDSBytes, 1024),
+                     smem_desc_sw128(sK + kk * 2048, kKeys * 128, 1024), idesc_q, kk > 0 ? 1u : 0u);
+            mma_commit(smem_u32(&ctl.dq_full[b]));
+            ++lp;
+          }
+        } else {
+          // dQ^T = K^T dS^T of the step, over its dP^T columns.
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_ss(tmem + col_dp(g), smem_desc_sw128(sK + kk * 2048, kKeys * 128, 1024),
+                   smem_desc_sw128(sDS + kk * 2048, kKeys * 128, 1024), idesc_q, kk > 0 ? 1u : 0u);
+          mma_commit(smem_u32(&ctl.dq_full[g]));
+        }
+        if (pend.kv_free >= 0) mma_commit(smem_u32(&ctl.kv_free[pend.kv_free]));
+        return true;
+      };
+      for (int j = 0; ok && j < n_items; ++j) {
+        const int sl = j % kSlots;
+        if (!wait(ctl.item_full[sl], (j / kSlots) & 1)) {
+          ok = false;
+          break;
+        }
+        const int n = static_cast<int>(ctl.n_live[sl]);
+        if (n > 0) {
+          const int kv = li % C::kKVBufs;
+          const uint32_t sK = base + C::kOffK + kv * C::kKVBytes, sV = base + C::kOffV + kv * C::kKVBytes;
+          if (!wait(ctl.kv_full[kv], (li / C::kKVBufs) & 1)) {
+            ok = false;
+            break;
+          }
+          for (int t = 0; t < n; ++t, ++lt) {
+            const int g = t & 1, slot = lt % kRing;
+            // The pending step uses this stage (an item that ended on it).
+            if (pend.on && pend.g == g && !flush()) {
+              ok = false;
+              break;
+            }
+            // The step staged; the stage's columns free: its last P read by
+            // the dV product (D = 64), and its dQ^T read out (D = 128).
+            if (!wait(ctl.ld_full[slot], (lt / kRing) & 1) ||
+                (use[g] > 0 && !wait(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use[g] - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sQ = base + C::kOffQ + slot * C::kQBytes, sDO = base + C::kOffDO + slot * C::kQBytes;
+            // 16 head dims per instruction: swizzle chunk kk / 4 of the rows, 32 bytes into it.
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t ko = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32, qo = (kk >> 2) * (kQ * 128) + (kk & 3) * 32;
+              mma_ss(tmem + col_s(g), smem_desc_sw128(sK + ko, 16, 1024), smem_desc_sw128(sQ + qo, 16, 1024), idesc_s,
+                     kk > 0 ? 1u : 0u);
+            }
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t ko = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32, qo = (kk >> 2) * (kQ * 128) + (kk & 3) * 32;
+              mma_ss(tmem + col_dp(g), smem_desc_sw128(sV + ko, 16, 1024), smem_desc_sw128(sDO + qo, 16, 1024), idesc_s,
+                     kk > 0 ? 1u : 0u);
+            }
+            // st_full covers every earlier product, so the ones that last read
+            // this step's dS slot have done so before it is rewritten.
+            mma_commit(smem_u32(&ctl.st_full[g]));
+            if (!flush()) {
+              ok = false;
+              break;
+            }
+            pend.on = true;
+            pend.g = g;
+            pend.slot = slot;
+            pend.li = li;
+            pend.kv = kv;
+            pend.first = t == 0;
+            pend.pair_end = g == 1 || t + 1 == n;
+            pend.kv_free = t + 1 == n ? kv : -1;
+            pend.use = use[g];
+            ++use[g];
+          }
+          if (!ok) break;
+          ++li;
+          // With two K/V buffers the last step's products may wait for the
+          // next item's first S^T, if that item has a live step; its list
+          // needs nothing of this item.
+          bool keep = false;
+          if (C::kKVBufs == 2 && j + 1 < n_items) {
+            if (!wait(ctl.item_full[(j + 1) % kSlots], ((j + 1) / kSlots) & 1)) {
+              ok = false;
+              break;
+            }
+            keep = ctl.n_live[(j + 1) % kSlots] > 0u;
+          }
+          if (!keep && !flush()) {
+            ok = false;
+            break;
+          }
+        }
+        mbar_arrive(smem_u32(&ctl.item_free[sl]));
+      }
+      if (ok && !flush()) ok = false;
+      if (!ok) fail();
+      // Every MMA this thread issued must complete before TMEM is released.
+      mma_commit(smem_u32(&ctl.drain));
+      uint32_t zero = 0;
+      mbar_wait_bounded(smem_u32(&ctl.drain), 0, &zero, timeout_ns);
+    }
+  } else if (warp == kScanWarp) {
+    // ================================================================ scanner
+    // Item j's live list: bit v set when some query row of step v keeps a key
+    // of the item's tile.  8 steps per batch of loads, 2 rows per lane.
+    bool ok = true;
+    int rt[2], rh[2];
+    bool rin[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = lane + 32 * u;
+      rin[u] = i < x.rows;
+      rh[u] = rin[u] ? i / x.tn : 0;
+      rt[u] = rin[u] ? i - rh[u] * x.tn : 0;
+    }
+    for (int j = 0; j < n_items; ++j) {
+      const int sl = j % kSlots;
+      if (j >= kSlots && !wait_all(ctl.item_free[sl], ((j / kSlots) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      const Item it = item_at(j);
+      uint32_t vmask[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) vmask[w] = low_bits(x.Nk - it.kt * kKeys - 32 * w);
+      auto any_of = [&](const uint4& m) {
+        return (m.x & vmask[0]) | (m.y & vmask[1]) | (m.z & vmask[2]) | (m.w & vmask[3]);
+      };
+      uint32_t mine[2] = {0u, 0u};  // words lane and lane + 32 of the list
+      if (x.words == nullptr || x.one_row) {
+        // No mask, or one mask row for the whole item: all steps or none.
+        bool any = true;
+        if (x.words != nullptr)
+          any = any_of(__ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] +
+                                                            it.h0 * x.word_stride[1] + it.kt * 4))) != 0u;
+        if (any) {
+          mine[0] = low_bits(VT - 32 * lane);
+          mine[1] = low_bits(VT - 32 * (lane + 32));
+        }
+      } else {
+        for (int v0 = 0; v0 < VT; v0 += 8) {
+          uint4 m[8][2];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              const int t = step_q0(v0 + u) + rt[rr], h = it.h0 + step_head(v0 + u) + rh[rr];
+              m[u][rr] = make_uint4(0u, 0u, 0u, 0u);
+              if (v0 + u < VT && rin[rr] && t < x.Nq)
+                m[u][rr] = __ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] +
+                                                                h * x.word_stride[1] + t * x.word_stride[2] +
+                                                                it.kt * 4));
+            }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int v = v0 + u;
+            const bool any = __any_sync(0xffffffffu, (any_of(m[u][0]) | any_of(m[u][1])) != 0u);
+            if (any && lane == ((v >> 5) & 31)) {
+              if (v < 1024) mine[0] |= 1u << (v & 31);
+              else mine[1] |= 1u << (v & 31);
+            }
+          }
+        }
+      }
+      ctl.live_bits[sl][lane] = mine[0];
+      ctl.live_bits[sl][lane + 32] = mine[1];
+      const int n = __reduce_add_sync(0xffffffffu, __popc(mine[0]) + __popc(mine[1]));
+      if (lane == 0) ctl.n_live[sl] = static_cast<uint32_t>(n);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_full[sl]));
+    }
+    if (!ok && lane == 0) fail();
+  } else if (warp < kEwWarps) {
+    // ================================================================ element-wise
+    // Thread t = key t of the tile (TMEM lane); stage g = warp / 4.
+    const int g = warp >> 2;
+    const int t = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float c2 = scale * kLog2e;
+    const uint64_t c2x2 = f2(c2, c2);
+    const int my_word = (t >> 5) * kQ;     // the word holding this key, for each query row
+    const uint32_t kbit = 1u << (t & 31);  // this key's bit in it
+    bool ok = true;
+    uint32_t lt0 = 0, lp0 = 0, use = 0;
+    for (int j = 0; ok && j < n_items; ++j) {
+      const int sl = j % kSlots;
+      ok = wait_all(ctl.item_full[sl], (j / kSlots) & 1);
+      if (!ok) break;
+      const int n = static_cast<int>(ctl.n_live[sl]);
+      if constexpr (!kBias) arrive_warp(ctl.item_free[sl]);  // only the count is needed
+      // kBias: this warp's 32-key block, the walk over the steps, and the bias
+      // gradient of blocks beyond the last bucket's start, per head.
+      int cw = 0, key0 = 0, off = 0, far_head = -1;
+      uint32_t cx = 0u;
+      float far_lo = 0.f, far_hi = 0.f;
+      Item it{};
+      if constexpr (kBias) {
+        it = item_at(j);
+        key0 = it.kt * kKeys + (warp & 3) * 32;
+        off = x.bias_offsets == nullptr
+                  ? x.bias_offset
+                  : max(-kMaxBiasOffset, min(kMaxBiasOffset, __ldg(x.bias_offsets + it.b)));
+        cx = ctl.live_bits[sl][0];
+        if (g == 1) next_live(ctl.live_bits[sl], cw, cx);
+      }
+      auto flush_far = [&]() {
+        if constexpr (kBias) {
+          if (far_head < 0) return;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            far_lo += __shfl_xor_sync(0xffffffffu, far_lo, o);
+            far_hi += __shfl_xor_sync(0xffffffffu, far_hi, o);
+          }
+          if (lane == 0) {
+            float* dst = x.far_part + (((static_cast<int64_t>(it.b) * x.H + far_head) * x.KB + key0 / 32) * 2 + g) * 2;
+            dst[0] = far_lo;
+            dst[1] = far_hi;
+          }
+          far_lo = far_hi = 0.f;
+        }
+      };
+      for (int tt = g; tt < n; tt += 2, ++use) {
+        const uint32_t lt = lt0 + tt;
+        const int b = lt % kRing;
+        int head = 0, q0 = 0;
+        if constexpr (kBias) {
+          const int v = next_live(ctl.live_bits[sl], cw, cx);
+          next_live(ctl.live_bits[sl], cw, cx);  // the other stage's
+          head = it.h0 + step_head(v);           // hb = 1
+          q0 = step_q0(v);
+          if (head != far_head) {
+            flush_far();
+            far_head = head;
+          }
+        }
+        const uint32_t* my_words = s_mask + b * 4 * kQ + my_word;
+        const float* t_lse = s_lse + b * kQ;
+        const float* t_delta = s_delta + b * kQ;
+        uint8_t* ds_row = smem + C::kOffDS +
+                          (C::kPairDQ ? static_cast<int>((lp0 + (tt >> 1)) & 1) * 2 + g : g) * C::kDSBytes + t * 128;
+        ok = wait_all(ctl.ld_full[b], (lt / kRing) & 1) && wait_all(ctl.st_full[g], use & 1);
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          float s[32], dp[32];
+          tmem_ld32f(t_lane + col_s(g) + c * 32, s);
+          tmem_ld32f(t_lane + col_dp(g) + c * 32, dp);
+          // kBias: relative positions of the block are d0 + lane - e; the
+          // bias of a block beyond (bias_lo, bias_hi) is one value.
+          float badd = 0.f;
+          const float* brow = nullptr;
+          int d0 = 0;
+          bool near = false;
+          if constexpr (kBias) {
+            d0 = key0 - (q0 + c * 32) - off;
+            const float* head_row = x.bias + static_cast<int64_t>(head) * x.bias_len;
+            near = d0 + 31 > x.bias_lo && d0 - 31 < x.bias_hi;
+            brow = head_row + (near ? d0 - x.bias_lo + kBiasPad + lane : 0);
+            badd = near ? 0.f : __ldg(head_row + (d0 < x.bias_hi ? 0 : x.bias_len - 1));
+          }
+          tmem_wait_ld();
+          uint32_t pw[16], dw[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const uint4 m4 = *reinterpret_cast<const uint4*>(my_words + c * 32 + e);
+            const float4 l4 = *reinterpret_cast<const float4*>(t_lse + c * 32 + e);
+            const float4 d4 = *reinterpret_cast<const float4*>(t_delta + c * 32 + e);
+            const uint32_t mm[4] = {m4.x, m4.y, m4.z, m4.w};
+            // y = s * scale * log2(e) + bias - lse2 and ds = p * (dp - Delta), two queries per instruction.
+            uint64_t l01 = f2(l4.x, l4.y), l23 = f2(l4.z, l4.w);
+            if constexpr (kBias) {
+              if (near) {
+                l01 = add2(l01, f2(__ldg(brow - e), __ldg(brow - e - 1)));
+                l23 = add2(l23, f2(__ldg(brow - e - 2), __ldg(brow - e - 3)));
+              } else {
+                l01 = add2(l01, f2(badd, badd));
+                l23 = add2(l23, f2(badd, badd));
+              }
+            }
+            float y[4], p[4], ds[4];
+            f2_split(fma2(f2(s[e], s[e + 1]), c2x2, l01), y[0], y[1]);
+            f2_split(fma2(f2(s[e + 2], s[e + 3]), c2x2, l23), y[2], y[3]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = (mm[u] & kbit) ? ex2f(y[u]) : 0.f;
+            f2_split(mul2(f2(p[0], p[1]), add2(f2(dp[e], dp[e + 1]), f2(d4.x, d4.y))), ds[0], ds[1]);
+            f2_split(mul2(f2(p[2], p[3]), add2(f2(dp[e + 2], dp[e + 3]), f2(d4.z, d4.w))), ds[2], ds[3]);
+            pw[e / 2] = pack2<BF16>(p[0], p[1]);
+            pw[e / 2 + 1] = pack2<BF16>(p[2], p[3]);
+            dw[e / 2] = pack2<BF16>(ds[0], ds[1]);
+            dw[e / 2 + 1] = pack2<BF16>(ds[2], ds[3]);
+            if constexpr (kBias) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) s[e + u] = ds[u];  // the scores are used up
+            }
+          }
+          // P over S^T columns this warp has read (chunk c writes 16 c ..,
+          // which chunks <= c have read).
+          tmem_st16(t_lane + col_s(g) + c * 16, pw);
+          // dS: row t of the step's tile, queries 32 c .. +31 = 16-byte chunks
+          // 4 c .. +3 of its 128 bytes, 128-byte swizzle.
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(ds_row + (((c * 4 + q) ^ (t & 7)) * 16)) =
+                make_uint4(dw[4 * q], dw[4 * q + 1], dw[4 * q + 2], dw[4 * q + 3]);
+          if constexpr (kBias) {
+            if (near) {
+              float pos, neg;
+              diagonal_sums(s, lane, pos, neg);
+              const int kb = key0 / 32, qb = q0 / 32 + c;
+              const int slot = x.slot_by_query ? qb : bias_block_max(x.bias_hi, off) - (kb - qb);
+              if (qb < x.QB) {
+                float* dst =
+                    x.near_part + (((static_cast<int64_t>(it.b) * x.H + head) * x.KB + kb) * x.slots + slot) * 64;
+                dst[lane] = pos;
+                dst[32 + lane] = neg;
+              }
+            } else {
+              float sum = 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sum += s[e];
+              if (d0 < x.bias_hi) far_lo += sum;
+              else far_hi += sum;
+            }
+          }
+        }
+        tmem_wait_st();
+        fence_proxy_async_smem();  // dS written by this thread, read by the tensor core
+        arrive_warp(ctl.p_full[g]);
+        arrive_warp(ctl.tile_free[b]);
+      }
+      lt0 += n;
+      lp0 += (n + 1) / 2;
+      if constexpr (kBias) {
+        if (!ok) break;
+        flush_far();
+        arrive_warp(ctl.item_free[sl]);
+      }
+    }
+    if (!ok && lane == 0) fail();
+  } else {
+    // ================================================================ epilogue
+    const int w = (warp - kEpiWarp + 2) & 3;  // a warp reads the TMEM lanes of its index mod 4
+    const int t = w * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    uint8_t* s_dq = smem + C::kOffDQ + w * 4096;
+    const int n_rows = x.hb * x.Nq;  // rows of the accumulator's block that holds a step
+    bool ok = true;
+    uint32_t lp = 0, use[2] = {0, 0}, li = 0;
+    // The staged box (32 rows of 32 columns) is added at (col, row0, block);
+    // rows past the block are clipped by the TMA unit.
+    auto add_box = [&](int col, int row0, int block) {
+      fence_proxy_async_smem();  // staged by every lane, read by the TMA unit
+      __syncwarp();
+      if (lane == 0 && row0 < n_rows) {
+        tma_reduce_add_3d(&tm_dq, smem_u32(s_dq), col, row0, block);
+        bulk_commit_group();
+      }
+    };
+    auto box_free = [&]() {
+      if (lane == 0) bulk_wait_group_read0();
+      __syncwarp();
+    };
+    for (int j = 0; ok && j < n_items; ++j) {
+      const int sl = j % kSlots;
+      ok = wait_all(ctl.item_full[sl], (j / kSlots) & 1);
+      if (!ok) break;
+      const Item it = item_at(j);
+      const int block0 = (it.b * x.Hkv + it.hkv) * x.gh;
+      const int n = static_cast<int>(ctl.n_live[sl]);
+      int cw = 0;
+      uint32_t cx = ctl.live_bits[sl][0];
+      if constexpr (C::kPairDQ) {
+        // Thread t = row t of a pair: the first step's 64 rows, then the second's.
+        for (int tt = 0; tt < n; tt += 2, ++lp) {
+          const int va = next_live(ctl.live_bits[sl], cw, cx);
+          const int vb = tt + 1 < n ? next_live(ctl.live_bits[sl], cw, cx) : -1;
+          const int b = lp & 1;
+          ok = wait_all(ctl.dq_full[b], (lp >> 1) & 1);
+          if (!ok) break;
+          float u[64];
+          tmem_ld32f(t_lane + C::col_dq(b), u);
+          tmem_ld32f(t_lane + C::col_dq(b) + 32, u + 32);
+          tmem_wait_ld();
+          arrive_warp(ctl.dq_free[b]);
+          const int v = w < 2 ? va : vb;
+          if (v < 0) continue;
+          const int row0 = step_q0(v) + (w & 1) * 32;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            box_free();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float* y = u + 32 * h + 4 * c;
+              *reinterpret_cast<float4*>(s_dq + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+                  make_float4(y[0] * scale, y[1] * scale, y[2] * scale, y[3] * scale);
+            }
+            add_box(32 * h, row0, block0 + v / x.QT1);
+          }
+        }
+      } else {
+        // Thread t = head dim t; columns are the step's 64 queries.
+        for (int tt = 0; tt < n; ++tt) {
+          const int v = next_live(ctl.live_bits[sl], cw, cx);
+          const int g = tt & 1;
+          ok = wait_all(ctl.dq_full[g], use[g] & 1);
+          if (!ok) break;
+          ++use[g];
+          float u[64];
+          tmem_ld32f(t_lane + col_dp(g), u);
+          tmem_ld32f(t_lane + col_dp(g) + 32, u + 32);
+          tmem_wait_ld();
+          arrive_warp(ctl.dq_free[g]);
+          const int row0 = step_q0(v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            box_free();
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              *reinterpret_cast<float*>(s_dq + q * 128 + (((lane >> 2) ^ (q & 7)) * 16) + (lane & 3) * 4) =
+                  u[32 * h + q] * scale;
+            add_box(32 * w, row0 + 32 * h, block0 + v / x.QT1);
+          }
+        }
+      }
+      if (!ok) break;
+      // dV and dK of this key tile (lane t = key); zero when no step was live.
+      // The dq_full wait of the item's last step covered all of its products.
+      const int key = it.kt * kKeys + t;
+#pragma unroll 1
+      for (int h = 0; h < D / 32; ++h) {
+        uint32_t vw[16], kw[16];
+        if (n > 0) {
+          float u[32];
+          tmem_ld32f(t_lane + kColDV + h * 32, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) vw[e] = pack2<BF16>(u[2 * e], u[2 * e + 1]);
+          tmem_ld32f(t_lane + C::kColDK + h * 32, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) kw[e] = pack2<BF16>(u[2 * e] * scale, u[2 * e + 1] * scale);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) vw[e] = kw[e] = 0u;
+        }
+        if (key < x.Nk) {
+          const int64_t at = ((static_cast<int64_t>(it.b) * x.Hkv + it.hkv) * x.Nk + key) * D + h * 32;
+          uint4* dvr = reinterpret_cast<uint4*>(dv + at);
+          uint4* dkr = reinterpret_cast<uint4*>(dk + at);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            dvr[q] = make_uint4(vw[4 * q], vw[4 * q + 1], vw[4 * q + 2], vw[4 * q + 3]);
+            dkr[q] = make_uint4(kw[4 * q], kw[4 * q + 1], kw[4 * q + 2], kw[4 * q + 3]);
+          }
+        }
+      }
+      if (n > 0) {
+        arrive_warp(ctl.acc_free);
+        ++li;
+      }
+      arrive_warp(ctl.item_free[sl]);
+    }
+    // The reduce-adds must finish (and stop reading shared memory) before the CTA exits.
+    if (lane == 0) bulk_wait_group0();
+    if (!ok && lane == 0) fail();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
 
 // dtable[bucket][h] = sum of dS over the pairs whose relative position is in
 // the bucket: one block per (head, bucket) adds the diagonal sums of the
@@ -81,22 +1113,23 @@ __global__ void __launch_bounds__(kReduceThreads)
   }
 }
 
-// Fills the geometry; false when the query tiles of a key head exceed the list.
+// Fills the geometry; false when the steps of a key head exceed the list.
 bool geometry(const CrossParams& p, BwdGeo* x) {
   const int G = static_cast<int>(p.H / p.Hkv);
   x->B = static_cast<int>(p.B);
   x->H = static_cast<int>(p.H);
   x->Hkv = static_cast<int>(p.Hkv);
   x->Nq = static_cast<int>(p.Nq);
-  x->tn = std::min<int>(x->Nq, kT);
+  x->Nk = static_cast<int>(p.Nk);
+  x->tn = std::min<int>(x->Nq, kQ);
   x->hb = 1;
   const bool bias = p.bias.table != nullptr;
-  // With a bias a tile holds one head (its blocks belong to one bias row).
+  // With a bias a step holds one head (its blocks belong to one bias row).
   for (int h = 1; !bias && h <= G; ++h)
-    if (G % h == 0 && h * x->tn <= kT) x->hb = h;
+    if (G % h == 0 && h * x->tn <= kQ) x->hb = h;
   x->gh = G / x->hb;
   x->rows = x->tn * x->hb;
-  x->QT1 = (x->Nq + kT - 1) / kT;
+  x->QT1 = (x->Nq + kQ - 1) / kQ;
   x->words = p.words;
   for (int i = 0; i < 3; ++i) x->word_stride[i] = p.word_stride[i];
   x->one_row = p.words != nullptr && (x->Nq == 1 || p.word_stride[2] == 0) && (G == 1 || p.word_stride[1] == 0);
@@ -106,7 +1139,7 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
     x->bias_offset = p.bias.offset;
     bias_range(p.bias, &x->bias_lo, &x->bias_hi);
     x->bias_len = x->bias_hi - x->bias_lo + 1 + 2 * kBiasPad;
-    x->KB = static_cast<int>((p.Nk + kT - 1) / kT * 4);
+    x->KB = static_cast<int>((p.Nk + kKeys - 1) / kKeys * 4);
     x->QB = (x->Nq + 31) / 32;
     // Block differences that overlap (lo, hi): multiples of 32 in an open
     // interval of length hi - lo + 62.
@@ -114,26 +1147,28 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
     x->slot_by_query = slots > x->QB ? 1 : 0;
     x->slots = std::min(slots, x->QB);
   }
-  return static_cast<int64_t>(x->gh) * x->QT1 <= 32 * kListWords<true>;
+  return static_cast<int64_t>(x->gh) * x->QT1 <= kMaxSteps;
 }
 
 template <int D, bool BF16, bool kBias>
 int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg) {
-  using C = BwdCfg<D>;
-  const int64_t KT = (p.Nk + kT - 1) / kT;
+  using C = Cfg<D>;
+  constexpr size_t kSmemBytes = smem_bytes<D>();
+  const int64_t KT = (p.Nk + kKeys - 1) / kKeys;
   const int64_t items = p.B * p.Hkv * KT;
   const int64_t rows = p.B * p.H * p.Nq;
-  if (items > 0x7FFFFFFFll || (rows * (D / 8) + 255) / 256 > 0x7FFFFFFFll) {
+  const int64_t row_blocks = (rows * (D / 8) + 255) / 256;
+  if (items > 0x7FFFFFFFll || row_blocks > 0x7FFFFFFFll) {
     *msg = "backward: batch*heads too large";
     return kErrArg;
   }
   CUtensorMap mq, mk, mv, mdo, mdq;
   const int64_t so[3] = {p.H * p.Nq * D, p.Nq * D, D};
   CUresult rc = make_tensor_map_4d(&mq, p.q, p.dtype, D, p.Nq, p.H, p.B, p.q_stride, x.tn, x.hb);
-  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mk, p.k, p.dtype, D, p.Nk, p.Hkv, p.B, p.k_stride, kT);
-  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mv, p.v, p.dtype, D, p.Nk, p.Hkv, p.B, p.v_stride, kT);
+  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mk, p.k, p.dtype, D, p.Nk, p.Hkv, p.B, p.k_stride, kKeys);
+  if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mv, p.v, p.dtype, D, p.Nk, p.Hkv, p.B, p.v_stride, kKeys);
   if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mdo, g.dout, p.dtype, D, p.Nq, p.H, p.B, so, x.tn, x.hb);
-  // The accumulator in blocks of hb * Nq rows: a tile's rows are consecutive in it.
+  // The accumulator in blocks of hb * Nq rows: a step's rows are consecutive in it.
   if (rc == CUDA_SUCCESS)
     rc = make_tensor_map_3d_f32(&mdq, g.dq_accum, D, p.B * p.Hkv * x.gh, static_cast<int64_t>(x.hb) * p.Nq, 32);
   if (rc != CUDA_SUCCESS) {
@@ -143,40 +1178,31 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
   DeviceProps dp;
   if (!device_props(&dp, msg)) return kErrCuda;
   static std::atomic<bool> smem_set[kMaxDevices] = {};
-  auto kern = attn_bwd_kernel<D, BF16, true, kBias>;
-  cudaError_t e = ensure_smem_limit(kern, C::kSmemBytes, dp.device, smem_set);
+  auto kern = cross_bwd_kernel<D, BF16, kBias>;
+  cudaError_t e = ensure_smem_limit(kern, kSmemBytes, dp.device, smem_set);
   if (e == cudaSuccess && kBias) {
-    // Blocks that no live tile visits count as 0.
+    // Blocks that no live step visits count as 0.
     const int64_t bh_kb = p.B * p.H * x.KB;
     x.near_part = g.bias_part;
     x.far_part = g.bias_part + bh_kb * x.slots * 64;
     e = cudaMemsetAsync(g.bias_part, 0, static_cast<size_t>(bh_kb) * (x.slots * 64 + 4) * sizeof(float), p.stream);
   }
-  if (e == cudaSuccess) {
-    bwd_delta_kernel<D, BF16><<<static_cast<unsigned>((rows * (D / 8) + 255) / 256), 256, 0, p.stream>>>(
-        static_cast<const uint4*>(g.dout), static_cast<const uint4*>(p.out), g.delta,
-        reinterpret_cast<float4*>(g.dq_accum), rows);
-    e = cudaGetLastError();
-  }
-  if (e == cudaSuccess) {
-    const int64_t grid = items < dp.sms ? items : dp.sms;
-    kern<<<static_cast<unsigned>(grid), C::kThreads, C::kSmemBytes, p.stream>>>(
-        mq, mk, mv, mdo, mdq, nullptr, p.lse, g.delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),
-        static_cast<int>(p.Nk), static_cast<int>(KT * 4), static_cast<int>(KT), x.gh * x.QT1, static_cast<int>(items),
-        1, p.scale, x, p.err_word, p.timeout_ns);
-    e = cudaGetLastError();
-  }
-  if (e == cudaSuccess) {
-    const int64_t n8 = rows * D / 8;
-    bwd_dq_convert_kernel<BF16><<<static_cast<unsigned>((n8 + 255) / 256), 256, 0, p.stream>>>(
-        reinterpret_cast<const float4*>(g.dq_accum), static_cast<uint4*>(g.dq), n8);
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess)
+    e = launch_pdl(cross_delta_kernel<D, BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
+                   static_cast<const uint4*>(g.dout), static_cast<const uint4*>(p.out),
+                   static_cast<const uint4*>(p.out_lo), g.delta, reinterpret_cast<float4*>(g.dq_accum), rows);
+  if (e == cudaSuccess)
+    e = launch_pdl(kern, static_cast<unsigned>(std::min<int64_t>(items, dp.sms)), kThreads, kSmemBytes, p.stream, mq, mk,
+                   mv, mdo, mdq, p.lse, g.delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),
+                   static_cast<int>(KT), static_cast<int>(items), p.scale, x, p.err_word, p.timeout_ns);
+  if (e == cudaSuccess)
+    e = launch_pdl(cross_dq_kernel<BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
+                   reinterpret_cast<const float4*>(g.dq_accum), static_cast<uint4*>(g.dq), rows * D / 8);
   if (e == cudaSuccess && kBias) {
     const dim3 grid(static_cast<unsigned>(p.H), static_cast<unsigned>(p.bias.side * (p.bias.two_sided ? 2 : 1)));
     bias_reduce_kernel<BF16><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, g.dtable);
-    e = cudaGetLastError();
   }
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     *msg = cudaGetErrorString(e);
     return kErrLaunch;
@@ -200,7 +1226,7 @@ int64_t cross_bwd_bias_floats(const CrossParams& p) {
 int launch_attn_cross_bwd(const CrossParams& p, const CrossGrads& g, const char** msg) {
   BwdGeo x{};
   if (!geometry(p, &x)) {
-    *msg = "backward: more than 1024 query tiles (128 rows) share a key head";
+    *msg = "backward: more than 2048 steps of 64 query rows share a key head";
     return kErrUnsupportedN;
   }
   if (p.D == 128) return p.dtype == 1 ? launch_b<128, true>(p, g, x, msg) : launch_b<128, false>(p, g, x, msg);

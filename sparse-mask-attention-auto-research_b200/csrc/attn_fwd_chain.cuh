@@ -54,6 +54,7 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include "attn_math.cuh"
 #include "mask_bits.cuh"
 #include "rel_bias.cuh"
 #include "sma_internal.h"
@@ -107,8 +108,6 @@ struct ChainCfg {
   static constexpr int kMaxN = kMaxSeq;
 };
 constexpr float kRescaleThreshold = 8.0f;
-constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 struct ChainCtl {
   uint64_t sched_full[kSlots];
@@ -179,6 +178,7 @@ struct Geo {
   int row_shared;          // every row of a tile has the same mask row
   const int32_t* lengths;
   int kv_shared;           // all batches read the keys of batch 0
+  uint16_t* out_lo;        // O minus its rounded value, in the inputs' type, or nullptr
   // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
   const float* bias;
   const int32_t* bias_offsets;
@@ -192,47 +192,10 @@ constexpr size_t smem_bytes() {
 }
 static_assert(smem_bytes<64>() <= 227 * 1024 && smem_bytes<128>() <= 227 * 1024, "shared memory budget");
 
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Packed FP32 pairs (sm_100a f32x2 instructions): one issue slot for two lanes' worth of FMA / add.
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_split(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 __device__ __forceinline__ float max3f(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
 }
 
 __device__ __forceinline__ void named_bar_sync(int id, int count) {
@@ -1453,6 +1416,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
         }
         if (lse != nullptr && row_ok(it)) lse[row_index(it)] = lse_row;
+        if constexpr (kX) {
+          if (x.out_lo != nullptr && row_ok(it)) {
+            uint4* dst = reinterpret_cast<uint4*>(x.out_lo + row_index(it) * D);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              uint32_t lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int w = 4 * q + e;
+                const float2 hi = unpack2<BF16>(h[w]);
+                const uint32_t a = w < 16 ? u0[2 * w] : u1[2 * w - 32], b = w < 16 ? u0[2 * w + 1] : u1[2 * w - 31];
+                lo[e] = pack2<BF16>(fmaf(__uint_as_float(a), inv, -hi.x), fmaf(__uint_as_float(b), inv, -hi.y));
+              }
+              dst[q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+        }
         fence_proxy_async_smem();
         named_bar_sync(bar_id, 128);
         if (r == 0 && ctl.abort_flag == 0) {
@@ -1498,6 +1478,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint4* dst = reinterpret_cast<uint4*>(orow + dc * 32);
 #pragma unroll
               for (int q = 0; q < 4; ++q) dst[q] = make_uint4(hw[4 * q], hw[4 * q + 1], hw[4 * q + 2], hw[4 * q + 3]);
+            }
+          }
+          if constexpr (kX) {
+            if (store && x.out_lo != nullptr) {
+              uint32_t lo[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float2 hi = unpack2<BF16>(hw[e]);
+                lo[e] = pack2<BF16>(fmaf(__uint_as_float(u[2 * e]), inv, -hi.x),
+                                    fmaf(__uint_as_float(u[2 * e + 1]), inv, -hi.y));
+              }
+              uint4* dst = reinterpret_cast<uint4*>(x.out_lo + row_index(it) * D + dc * 32);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) dst[q] = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
             }
           }
         }

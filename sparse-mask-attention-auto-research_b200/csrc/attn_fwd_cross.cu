@@ -155,7 +155,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   const float inv = lo > 0.f ? 1.f / lo : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(m.out + row * D + lane * kPer);
 #pragma unroll
-  for (int e = 0; e < kPer / 2; ++e) dst[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  for (int e = 0; e < kPer / 2; ++e) {
+    const uint32_t w = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    dst[e] = w;
+    if (x.out_lo != nullptr) {
+      const float2 hi = unpack2<BF16>(w);
+      reinterpret_cast<uint32_t*>(x.out_lo + row * D + lane * kPer)[e] =
+          pack2<BF16>(fmaf(acc[2 * e], inv, -hi.x), fmaf(acc[2 * e + 1], inv, -hi.y));
+    }
+  }
   if (m.lse != nullptr && lane == 0) m.lse[row] = l > 0.f ? (M + log2f(l)) * kLn2 : -FLT_MAX;
 }
 
@@ -308,6 +316,7 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool 
   x.nb = keys.shared ? std::max(1, std::min<int>(x.B, kBM / (x.tn * x.hb))) : 1;
   x.rows = x.tn * x.hb * x.nb;
   x.kv_shared = keys.shared ? 1 : 0;
+  x.out_lo = static_cast<uint16_t*>(p.out_lo);
   if (!keys.shared) {
     x.words = p.words;
     for (int i = 0; i < 3; ++i) x.word_stride[i] = p.word_stride[i];
@@ -392,6 +401,11 @@ int launch_bias_expand(const CrossParams& p, const char** msg) {
 }
 
 int launch_attn_cross(const CrossParams& p, const char** msg) {
+  if (p.mask != nullptr) {
+    const int rc = launch_pack_rows(p.mask, p.mask_stride, p.words, p.word_stride[0] ? p.B : 1,
+                                    p.word_stride[1] ? p.H : 1, p.word_stride[2] ? p.Nq : 1, p.Nk, p.stream, msg);
+    if (rc != kOk) return rc;
+  }
   if (p.bias.table != nullptr) {
     const int rc = launch_bias_expand(p, msg);
     if (rc != kOk) return rc;

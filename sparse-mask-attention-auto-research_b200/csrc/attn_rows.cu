@@ -37,6 +37,7 @@
 #include <cfloat>
 #include <cmath>
 
+#include "attn_math.cuh"
 #include "rel_bias.cuh"
 #include "sma_internal.h"
 #include "sma_ptx.cuh"
@@ -50,8 +51,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 3;   // chunks in flight per warp
 constexpr int kBatch = 32;   // chunks whose masks a warp packs ahead
 constexpr int kMaxPieces = 255;
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 struct RowsParams {
   const uint16_t* q;
@@ -96,31 +95,6 @@ struct RowsCtl {
   uint32_t last;
 };
 static_assert(2 * (RowsCfg<128>::kSmem + sizeof(RowsCtl) + 1024) <= 228 * 1024, "two blocks per SM");
-
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-}
-
-// The sum of the two values as `pack2` rounded them.
-template <bool BF16>
-__device__ __forceinline__ float sum2(uint32_t x) {
-  if constexpr (BF16) return __uint_as_float(x << 16) + __uint_as_float(x & 0xFFFF0000u);
-  const float2 f = __half22float2(*reinterpret_cast<__half2*>(&x));
-  return f.x + f.y;
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -451,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float p0 = ex2f(sc[n][2 * u] - mu[u]), p1 = ex2f(sc[n][2 * u + 1] - mu[u]);
           l[u] += p0 + p1;
           const uint32_t w = pack2<BF16>(p0, p1);
-          lr[u] += sum2<BF16>(w);
+          const float2 rounded = unpack2<BF16>(w);
+          lr[u] += rounded.x + rounded.y;
           pa[n >> 1][(n & 1) * 2 + u] = w;
         }
 #pragma unroll

@@ -188,9 +188,6 @@ int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool
     for (int i = 0; i < a->bias_side; ++i) p->bias.starts[i] = a->bias_starts[i];
   p->out = a->out;
   p->lse = a->lse;
-  p->words = static_cast<const uint32_t*>(a->words);
-  for (int i = 0; i < 3; ++i) p->word_stride[i] = a->word_stride[i];
-  p->bias_distance = a->bias_distance;
   p->B = a->B;
   p->H = a->H;
   p->Hkv = a->Hkv;
@@ -384,45 +381,37 @@ int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const void* v,
                       H, N, D, scale, stream);
 }
 
-int sma_pack_mask_rows(const void* mask, const int64_t* stride, void* words, int64_t Bm, int64_t Hm, int64_t Qm,
-                       int64_t Nk, void* stream) {
-  NvtxRange range("sma_pack_mask_rows");
-  constexpr int64_t kMax = int64_t{1} << 30;
-  if (Bm < 0 || Hm < 0 || Qm < 0 || Nk < 0 || Bm > kMax || Hm > kMax || Qm > kMax || Nk > kMax)
-    return fail(sma::kErrArg, "pack_mask: bad dimension");
-  if (Bm == 0 || Hm == 0 || Qm == 0 || Nk == 0) return sma::kOk;
-  if (mask == nullptr || words == nullptr || stride == nullptr) return fail(sma::kErrArg, "pack_mask: null pointer");
-  if (!aligned16(words)) return fail(sma::kErrArg, "pack_mask: words must be 16-byte aligned");
-  for (int i = 0; i < 3; ++i)
-    if (stride[i] < 0) return fail(sma::kErrArg, "pack_mask: negative stride");
-  const char* msg = nullptr;
-  const int rc = sma::launch_pack_rows(static_cast<const uint8_t*>(mask), stride, static_cast<uint32_t*>(words), Bm, Hm,
-                                       Qm, Nk, static_cast<cudaStream_t>(stream), &msg);
-  return rc == sma::kOk ? rc : fail(rc, msg);
-}
-
 }  // extern "C"
 
 namespace {
 
-// Checks of the 128-row tile kernels on top of cross_params.
-int tile_params(const sma_attn_args* a) {
+// Checks of the 128-row tile kernels on top of cross_params; fills the fields
+// that only they use.
+int tile_params(const sma_attn_args* a, sma::CrossParams* p) {
   if (a->Nk > SMA_MAX_SEQ_LEN)
     return fail(sma::kErrUnsupportedN, "attention: more keys than the supported maximum (65536)");
-  if (a->mask) return fail(sma::kErrArg, "attention: this entry takes packed words, not a bool mask");
   if (a->words) {
     if (a->lengths) return fail(sma::kErrArg, "attention: give a mask or lengths, not both");
     if (!aligned16(a->words)) return fail(sma::kErrArg, "attention: words must be 16-byte aligned");
-    for (int i = 0; i < 3; ++i)
-      if (a->word_stride[i] < 0 || a->word_stride[i] % 4 != 0)
-        return fail(sma::kErrArg, "attention: word strides must be multiples of 4 words");
+  } else if (a->mask) {
+    return fail(sma::kErrArg, "attention: a mask needs room for its words");
   }
+  if (!aligned16(a->out_lo)) return fail(sma::kErrArg, "attention: out_lo must be 16-byte aligned");
   if (a->bias_table) {
     if (!a->bias_distance || !aligned16(a->bias_distance))
       return fail(sma::kErrArg, "attention: a bias needs a 16-byte aligned bias_distance");
     if (a->bias_starts[a->bias_side - 1] > SMA_MAX_BIAS_DISTANCE)
       return fail(sma::kErrUnsupportedN, "attention: bias distance above the supported maximum (65536)");
   }
+  p->words = static_cast<uint32_t*>(a->words);
+  const int64_t W = (a->Nk + 127) / 128 * 4, n[3] = {a->B, a->H, a->Nq};
+  int64_t step = W;
+  for (int i = 2; i >= 0; --i) {
+    p->word_stride[i] = a->mask_stride[i] != 0 ? step : 0;
+    if (a->mask_stride[i] != 0) step *= n[i];
+  }
+  p->bias_distance = a->bias_distance;
+  p->out_lo = a->out_lo;
   return sma::kOk;
 }
 
@@ -430,6 +419,8 @@ int tile_params(const sma_attn_args* a) {
 int write_nothing(const sma::CrossParams& p) {
   const int64_t rows = p.B * p.H * p.Nq;
   cudaError_t e = cudaMemsetAsync(p.out, 0, static_cast<size_t>(rows * p.D * 2), p.stream);
+  if (e == cudaSuccess && p.out_lo != nullptr)
+    e = cudaMemsetAsync(p.out_lo, 0, static_cast<size_t>(rows * p.D * 2), p.stream);
   // -FLT_MAX is the bit pattern 0xFF7FFFFF, which no byte fill makes.
   if (e == cudaSuccess && p.lse != nullptr) {
     const int rc = sma::launch_fill(p.lse, rows, -FLT_MAX, p.stream);
@@ -449,7 +440,7 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
   if (p.P > 0) return fail(sma::kErrArg, "attention: no prefix here");
-  rc = tile_params(args);
+  rc = tile_params(args, &p);
   if (rc != sma::kOk) return rc;
   if (p.Nk == 0) return write_nothing(p);
   const char* msg = nullptr;
@@ -466,9 +457,9 @@ int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, vo
   if (rc != sma::kOk) return rc;
   if (empty || p.Nk == 0) return fail(sma::kErrArg, "backward: no queries or no keys");
   if (p.P > 0 || p.lengths) return fail(sma::kErrArg, "backward: no prefix and no lengths");
-  rc = tile_params(args);
+  rc = tile_params(args, &p);
   if (rc != sma::kOk) return rc;
-  if (!p.lse || !dout || !dq || !dk || !dv || !dq_accum || !delta || (p.bias.table && (!dtable || !bias_part)))
+  if (!p.lse || !p.out_lo || !dout || !dq || !dk || !dv || !dq_accum || !delta || (p.bias.table && (!dtable || !bias_part)))
     return fail(sma::kErrArg, "backward: null pointer");
   if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(dq_accum) ||
       !aligned16(bias_part))
@@ -484,7 +475,7 @@ int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, vo
 int64_t sma_cross_attn_bwd_bias_floats(const sma_attn_args* args) {
   sma::CrossParams p{};
   bool empty = false;
-  if (cross_params(args, nullptr, &p, &empty) != sma::kOk || empty || p.Nk == 0 || tile_params(args) != sma::kOk) return -1;
+  if (cross_params(args, nullptr, &p, &empty) != sma::kOk || empty || p.Nk == 0 || tile_params(args, &p) != sma::kOk) return -1;
   return sma::cross_bwd_bias_floats(p);
 }
 
@@ -494,10 +485,10 @@ int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream) {
   bool empty = false;
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
-  rc = tile_params(args);
+  rc = tile_params(args, &p);
   if (rc != sma::kOk) return rc;
-  if (p.P == 0 || args->words || args->bias_table || args->lse)
-    return fail(sma::kErrArg, "attention: a shared prefix takes P > 0 and no mask, bias or lse");
+  if (p.P == 0 || args->mask || args->words || args->bias_table || args->lse || args->out_lo)
+    return fail(sma::kErrArg, "attention: a shared prefix takes P > 0 and no mask, bias, lse or out_lo");
   const char* msg = nullptr;
   rc = sma::launch_shared_prefix(p, &msg);
   return rc == sma::kOk ? rc : fail(rc, msg);

@@ -116,12 +116,14 @@ struct CrossParams {
   BiasSpec bias;
   void* out;                  // [B, H, Nq, D] contiguous
   float* lse;                 // [B, H, Nq] or nullptr
-  // attn_fwd_cross.cu: the mask packed by launch_pack_rows ([.., W] words with
-  // strides {batch, head, query}, 0: broadcast; nullptr keeps every key), and
-  // room for the bias by relative position, [H][bias_distance_len].
-  const uint32_t* words;
+  // attn_fwd_cross.cu and attn_bwd_cross.cu: the packed mask ([.., W] words with
+  // strides {batch, head, query}, 0: broadcast; nullptr keeps every key), the
+  // bias by relative position, [H][bias_hi - bias_lo + 1 + 2 kBiasPad], and
+  // O minus its rounded value, in the inputs' type (nullptr: not wanted).
+  uint32_t* words;
   int64_t word_stride[3];
   float* bias_distance;
+  void* out_lo;
   // attn_rows.cu: where given, every row is left as a piece for a later merge
   // (max, sum, sum of rounded P, - / FP32 O, not normalised; indexed by
   // (b * H + h) * Nq + i) instead of written to `out`.

@@ -33,10 +33,10 @@ SMA_MAX_BIAS_DISTANCE = 65536
 # sma_attn_args, field by field (every 8-byte field falls on its alignment):
 # dtype, scale; B H Hkv Nq Nk D P; q k v; their strides; k_prefix v_prefix;
 # their strides; mask; its strides; lengths, bias_table, bias_starts,
-# bias_offsets; bias_offset; bias_side, bias_two_sided; out, lse, words; its
-# strides; bias_distance.
+# bias_offsets; bias_offset; bias_side, bias_two_sided; out, lse, words,
+# bias_distance, out_lo.
 # Packing it as bytes costs about 1 us where a ctypes.Structure takes 5.
-ATTN_ARGS = struct.Struct("@if7q3P9q2P4qP3q4Pq2i3P3qP")
+ATTN_ARGS = struct.Struct("@if7q3P9q2P4qP3q4Pq2i5P")
 
 # Every symbol include/sma_capi.h declares, with (restype, argtypes).
 _i64 = ctypes.c_int64
@@ -65,7 +65,6 @@ SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _vp],
     ),
-    "sma_pack_mask_rows": (ctypes.c_int, [_vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _i64, _vp]),
     "sma_rows_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_cross_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_cross_attn_bwd": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

@@ -79,15 +79,6 @@ def _few_rows(q, k):
     return q.shape[1] // max(k.shape[1], 1) * q.shape[2] <= _ROWS or k.shape[2] > _lib.SMA_MAX_SEQ_LEN
 
 
-def _tiles_forward(q, k, v, mask, scale, bias, lse):
-    """The 128-row tiles: (out, packed mask, bias by relative position)."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    words = None if mask is None else sparse_attn_cuda.pack_mask_rows(mask)
-    distance = None if bias is None else sparse_attn_cuda.bias_distance_buffer(bias, q.shape[1], q.device)
-    sparse_attn_cuda.cross_forward(q, k, v, out, lse, scale, words, bias, distance)
-    return out, words, distance
-
-
 class CrossAttentionFunction(Function):
     """Autograd node of cross_attention (table and bias None) and
     relative_bias_attention: ``table`` is the differentiable input, the rest
@@ -96,48 +87,53 @@ class CrossAttentionFunction(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, mask, scale, bias):
         q, k, v = _strided(q), _strided(k), _strided(v)
+        offsets = None
         if bias is not None:
             bias = bias._replace(table=table)
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        out, words, distance = _tiles_forward(q, k, v, mask, scale, bias, lse)
+            offsets = bias.offsets
+            ctx.bias = bias._replace(table=None, offsets=None)
+        else:
+            ctx.bias = None
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        saved, ctx.mask_strides = sparse_attn_cuda.cross_forward(q, k, v, out, scale, mask, bias, training=True)
         ctx.scale = scale
-        ctx.word_strides = None if words is None else words[1]
-        ctx.bias = None if bias is None else bias._replace(table=None, offsets=None)
-        ctx.save_for_backward(q, k, v, out, lse, None if words is None else words[0], table, distance,
-                              None if bias is None else bias.offsets)
+        ctx.save_for_backward(q, k, v, out, saved, table, offsets)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, words, table, distance, offsets = ctx.saved_tensors
+        q, k, v, out, saved, table, offsets = ctx.saved_tensors
         if q.numel() == 0 or k.numel() == 0:
             dtable = None if table is None else torch.zeros_like(table)
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), dtable, None, None, None
         dout = dout.contiguous()
         if dout.data_ptr() % 16 != 0:
             dout = dout.clone()
-        if words is not None:
-            words = (words, ctx.word_strides)
         bias = None if ctx.bias is None else ctx.bias._replace(table=table, offsets=offsets)
-        dq, dk, dv, dtable = sparse_attn_cuda.cross_backward(dout, q, k, v, out, lse, ctx.scale, words, bias, distance)
+        dq, dk, dv, dtable = sparse_attn_cuda.cross_backward(dout, q, k, v, out, ctx.scale, saved, ctx.mask_strides, bias)
         return dq, dk, dv, dtable, None, None, None
+
+
+# With gradients: 64-row steps of the queries of all heads that share a key head.
+_MAX_STEPS = 2048
 
 
 def _attention(q, k, v, mask, scale, bias):
     """out [B, H, Nq, D] of checked fp16 / bf16 inputs."""
     table = None if bias is None else bias.table
     if _needs_grad(q, k, v) or (table is not None and _needs_grad(table)):
-        Nk, tiles = k.shape[2], q.shape[1] // max(k.shape[1], 1) * ((q.shape[2] + 127) // 128)
+        Nk, steps = k.shape[2], q.shape[1] // max(k.shape[1], 1) * ((q.shape[2] + 63) // 64)
         _require(Nk <= _lib.SMA_MAX_SEQ_LEN, f"with gradients at most {_lib.SMA_MAX_SEQ_LEN} keys are supported")
-        _require(tiles <= 1024, "with gradients at most 1024 tiles of 128 queries may share a key head")
+        _require(steps <= _MAX_STEPS, f"with gradients at most {_MAX_STEPS} steps of 64 queries may share a key head")
         return CrossAttentionFunction.apply(q, k, v, table, mask, scale, bias)
     q, k, v = _strided(q), _strided(k), _strided(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if _few_rows(q, k):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, mask=mask, bias=bias)
-        return out
-    return _tiles_forward(q, k, v, mask, scale, bias, None)[0]
+        sparse_attn_cuda.rows_forward(q, k, v, out, scale, mask=mask, bias=bias)
+    else:
+        sparse_attn_cuda.cross_forward(q, k, v, out, scale, mask, bias)
+    return out
 
 
 def cross_attention(q, k, v, mask=None, scale=None):
@@ -257,7 +253,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths=None, scale=Non
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     prefix = (k_prefix, v_prefix)
     if B == 1 or k_prefix.shape[1] == 0 or S > _lib.SMA_MAX_SEQ_LEN:
-        sparse_attn_cuda.rows_forward(q, k, v, out, None, scale, lengths=lengths, prefix=prefix)
+        sparse_attn_cuda.rows_forward(q, k, v, out, scale, lengths=lengths, prefix=prefix)
     else:
         sparse_attn_cuda.prefix_forward(q, k, v, out, scale, prefix, lengths)
     return out.float() if dtype == torch.float32 else out

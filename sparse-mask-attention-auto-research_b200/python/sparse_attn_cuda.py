@@ -219,9 +219,9 @@ def _strided(t):
     return t.contiguous()
 
 
-def _mask_strides(mask, shape):
-    """`mask` with a contiguous last axis, and its strides (0 where it is
-    broadcast) along the first three axes of `shape` ([B, H, Nq, Nk])."""
+def _mask_strides(mask):
+    """`mask` with a contiguous last axis, and its strides along the others (0
+    where it is broadcast)."""
     if mask.shape[3] > 1 and mask.stride(3) != 1:
         mask = mask.contiguous()
     return mask, tuple(0 if n == 1 else s for n, s in zip(mask.shape[:3], mask.stride()[:3]))
@@ -237,115 +237,132 @@ class Bias(typing.NamedTuple):
     offsets: typing.Optional[torch.Tensor]  # int32 [B], or None: offset for all
 
 
-def bias_distance_buffer(bias, H, device):
-    """Room for the bias by relative position (SMA_BIAS_DISTANCE_LEN floats per head)."""
-    last = bias.starts[len(bias.starts) - 1]
-    return torch.empty((H, (2 if bias.two_sided else 1) * last + 513), dtype=torch.float32, device=device)
-
-
-def pack_mask_rows(mask):
-    """bool mask [B or 1, H or 1, Nq or 1, Nk] -> (int32 words [Bm, Hm, Qm, W],
-    their strides): W = 4 * ceil(Nk / 128) words per row, bit b of word w =
-    column 32 w + b, 0 past Nk.  Axes along which the mask does not change
-    (length 1, or expanded) are packed once and have stride 0."""
-    if mask.shape[3] > 1 and mask.stride(3) != 1:
-        mask = mask.contiguous()
-    st = mask.stride()[:3]
-    dims = tuple(1 if s == 0 else n for n, s in zip(mask.shape[:3], st))
-    Nk = mask.shape[3]
-    W = (Nk + 127) // 128 * 4
-    words = torch.empty((*dims, W), dtype=torch.int32, device=mask.device)
-    lib = _lib.load()
-    with _device_guard(mask.device):
-        _lib.check(lib.sma_pack_mask_rows(mask.data_ptr(), (ctypes.c_int64 * 3)(*st), words.data_ptr(), *dims, Nk,
-                                          _stream_ptr(mask.device)))
-    return words, tuple(0 if n == 1 else s for n, s in zip(dims, words.stride()[:3]))
-
-
-def _attn_args(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None, words=None,
-               bias_distance=None):
-    """sma_attn_args of checked tensors (see include/sma_capi.h), and what it
-    points to that has to outlive the call."""
+def _attn_args(q, k, v, out, scale, mask_ptr=0, mask_strides=(0, 0, 0), lengths=None, prefix=None, bias=None, lse=0,
+               words=0, bias_distance=0, out_lo=0):
+    """sma_attn_args (include/sma_capi.h) of checked tensors and addresses."""
     B, H, Nq, D = q.shape
     Hkv, Nk = k.shape[1:3]
-    mask_ptr, mask_st = None, (0, 0, 0)
-    if mask is not None:
-        mask, mask_st = _mask_strides(mask, (B, H, Nq, Nk))
-        mask_ptr = mask.data_ptr()
-    kp = vp = kp_st = None
-    P = 0
-    if prefix is not None:
+    if prefix is not None and prefix[0].shape[1]:
         kp, vp = prefix
-        P = kp.shape[1]
-    table, starts, two_sided, offset, offsets = bias if bias is not None else (None, None, 0, 0, None)
-    raw = _lib.ATTN_ARGS.pack(
+        P, pre = kp.shape[1], (kp.data_ptr(), vp.data_ptr(), *kp.stride()[:2], *vp.stride()[:2])
+    else:
+        P, pre = 0, (0, 0, 0, 0, 0, 0)
+    if bias is not None:
+        starts = bias.starts
+        add = (bias.table.data_ptr(), ctypes.addressof(starts), 0 if bias.offsets is None else bias.offsets.data_ptr(),
+               bias.offset, len(starts), int(bias.two_sided))
+    else:
+        add = (0, 0, 0, 0, 0, 0)
+    return _lib.ATTN_ARGS.pack(
         _DTYPES[q.dtype], scale, B, H, Hkv, Nq, Nk, D, P, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
-        *k.stride()[:3], *v.stride()[:3], *((kp.data_ptr(), vp.data_ptr(), *kp.stride()[:2], *vp.stride()[:2])
-                                           if P else (0, 0, 0, 0, 0, 0)),
-        mask_ptr or 0, *mask_st, 0 if lengths is None else lengths.data_ptr(), 0 if table is None else table.data_ptr(),
-        0 if starts is None else ctypes.addressof(starts), 0 if offsets is None else offsets.data_ptr(), offset,
-        0 if starts is None else len(starts), int(two_sided), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        *((0, 0, 0, 0) if words is None else (words[0].data_ptr(), *words[1])),
-        0 if bias_distance is None else bias_distance.data_ptr(),
+        *k.stride()[:3], *v.stride()[:3], *pre, mask_ptr, *mask_strides, 0 if lengths is None else lengths.data_ptr(),
+        *add, out.data_ptr(), lse, words, bias_distance, out_lo,
     )
-    return raw, mask
 
 
-def rows_forward(q, k, v, out, lse, scale, mask=None, lengths=None, prefix=None, bias=None):
+def rows_forward(q, k, v, out, scale, mask=None, lengths=None, prefix=None, bias=None):
     """Attention of a few query rows per key head (sma_rows_attn_fwd): q
     [B, H, Nq, D], k and v [B, Hkv, Nk, D], a bool ``mask`` that broadcasts to
     [B, H, Nq, Nk] or int32 ``lengths`` [B], a shared ``prefix`` (k, v)
-    [Hkv, P, D] and a ``bias``.  Writes ``out`` and, unless None, ``lse``.
-    The callers (cross_attention.py) check the arguments."""
-    args, _keep = _attn_args(q, k, v, out, lse, scale, mask, lengths, prefix, bias)
+    [Hkv, P, D] and a ``bias``.  Writes ``out``.  The callers
+    (cross_attention.py) check the arguments."""
+    mask_ptr, mask_st = 0, (0, 0, 0)
+    if mask is not None:
+        mask, mask_st = _mask_strides(mask)
+        mask_ptr = mask.data_ptr()
+    args = _attn_args(q, k, v, out, scale, mask_ptr, mask_st, lengths, prefix, bias)
     lib = _lib.load()
     with _device_guard(q.device):
         _lib.check(lib.sma_rows_attn_fwd(args, _stream_ptr(q.device)))
 
 
-def cross_forward(q, k, v, out, lse, scale, words=None, bias=None, bias_distance=None):
-    """Attention of many query rows (sma_cross_attn_fwd): ``words`` from
-    pack_mask_rows or None, a ``bias`` with its bias_distance_buffer.  Writes
-    ``out`` and, unless None, ``lse``."""
-    args, _keep = _attn_args(q, k, v, out, lse, scale, words=words, bias=bias, bias_distance=bias_distance)
-    lib = _lib.load()
-    with _device_guard(q.device):
-        _lib.check(lib.sma_cross_attn_fwd(args, _stream_ptr(q.device)))
-
-
-def cross_backward(dout, q, k, v, out, lse, scale, words=None, bias=None, bias_distance=None):
-    """Gradients of cross_forward (sma_cross_attn_bwd) from its ``out``,
-    ``lse`` and ``bias_distance``: (dq, dk, dv, dtable or None), contiguous."""
-    args, _keep = _attn_args(q, k, v, out, lse, scale, words=words, bias=bias, bias_distance=bias_distance)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=q.device) for _ in range(2))
-    dq_accum = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    delta = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    dtable = bias_part = None
-    lib = _lib.load()
-    with _device_guard(q.device):
-        if bias is not None:
-            dtable = torch.empty_like(bias.table)
-            floats = lib.sma_cross_attn_bwd_bias_floats(args)
-            _require(floats >= 0, "backward: unsupported arguments")
-            bias_part = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _lib.check(
-            lib.sma_cross_attn_bwd(
-                args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                None if dtable is None else dtable.data_ptr(), dq_accum.data_ptr(), delta.data_ptr(),
-                None if bias_part is None else bias_part.data_ptr(), _stream_ptr(q.device),
-            )
-        )
-    return dq, dk, dv, dtable
-
-
 def prefix_forward(q, k, v, out, scale, prefix, lengths=None):
     """Attention behind a shared ``prefix`` (k, v) [Hkv, P, D], read once for
     the batch (sma_prefix_attn_fwd)."""
-    args, _keep = _attn_args(q, k, v, out, None, scale, lengths=lengths, prefix=prefix)
+    args = _attn_args(q, k, v, out, scale, lengths=lengths, prefix=prefix)
     lib = _lib.load()
     with _device_guard(q.device):
         _lib.check(lib.sma_prefix_attn_fwd(args, _stream_ptr(q.device)))
+
+
+def _saved_layout(q, k, mask_strides, bias, training):
+    """Byte offsets (words, bias_distance, lse, out_lo; 0 where there is none,
+    each a multiple of 16) within the buffer a forward fills for itself and
+    its backward, and the buffer's size.  The first 16 bytes are not used, so
+    that no offset is 0."""
+    B, H, Nq, D = q.shape
+    end = 16
+    words = distance = lse = out_lo = 0
+    if mask_strides is not None:
+        words = end
+        rows = 1
+        for n, s in zip((B, H, Nq), mask_strides):
+            if s:
+                rows *= n
+        end += rows * ((k.shape[2] + 127) // 128 * 16)
+    if bias is not None:
+        distance = end
+        n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 513
+        end += (H * n * 4 + 15) // 16 * 16
+    if training:
+        lse = end
+        end += (B * H * Nq * 4 + 15) // 16 * 16
+        out_lo = end
+        end += B * H * Nq * D * 2
+    return words, distance, lse, out_lo, end
+
+
+def cross_forward(q, k, v, out, scale, mask=None, bias=None, training=False):
+    """Attention of many query rows (sma_cross_attn_fwd).  Writes ``out``;
+    returns what cross_backward needs of this call besides the tensors:
+    (buffer, strides of the mask or None)."""
+    mask_ptr, mask_st = 0, None
+    if mask is not None:
+        mask, mask_st = _mask_strides(mask)
+        mask_ptr = mask.data_ptr()
+    words, distance, lse, out_lo, size = _saved_layout(q, k, mask_st, bias, training)
+    saved, base = None, 0
+    if size > 16:
+        saved = torch.empty(size, dtype=torch.uint8, device=q.device)
+        base = saved.data_ptr()
+    args = _attn_args(q, k, v, out, scale, mask_ptr, mask_st or (0, 0, 0), bias=bias, lse=lse and base + lse,
+                      words=words and base + words, bias_distance=distance and base + distance,
+                      out_lo=out_lo and base + out_lo)
+    lib = _lib.load()
+    with _device_guard(q.device):
+        _lib.check(lib.sma_cross_attn_fwd(args, _stream_ptr(q.device)))
+    return saved, mask_st
+
+
+def cross_backward(dout, q, k, v, out, scale, saved, mask_strides=None, bias=None):
+    """Gradients of cross_forward(training=True) (sma_cross_attn_bwd) from its
+    ``out`` and what it returned: (dq, dk, dv, dtable or None), contiguous."""
+    words, distance, lse, out_lo, _ = _saved_layout(q, k, mask_strides, bias, True)
+    base = saved.data_ptr()
+    args = _attn_args(q, k, v, out, scale, 0, mask_strides or (0, 0, 0), bias=bias, lse=base + lse,
+                      words=words and base + words, bias_distance=distance and base + distance, out_lo=base + out_lo)
+    lib = _lib.load()
+    dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+    dv = torch.empty_like(dk)
+    with _device_guard(q.device):
+        # Scratch: the FP32 accumulator of dq, Delta, and partial sums of the bias gradient.
+        n_q = q.numel()
+        n_delta = (n_q // q.shape[3] + 3) // 4 * 4
+        n_bias, dtable = 0, None
+        if bias is not None:
+            dtable = torch.empty_like(bias.table)
+            n_bias = lib.sma_cross_attn_bwd_bias_floats(args)
+            _require(n_bias >= 0, "backward: unsupported arguments")
+        scratch = torch.empty(n_q + n_delta + n_bias, dtype=torch.float32, device=q.device)
+        acc = scratch.data_ptr()
+        _lib.check(
+            lib.sma_cross_attn_bwd(
+                args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                None if dtable is None else dtable.data_ptr(), acc, acc + 4 * n_q,
+                None if dtable is None else acc + 4 * (n_q + n_delta), _stream_ptr(q.device),
+            )
+        )
+    return dq, dk, dv, dtable
 
 
 def pack_mask(mask):

@@ -21,7 +21,7 @@ def lib():
 
 STARTS = (ctypes.c_int32 * 4)(0, 1, 2, 8)
 FIELDS = ("dtype scale B H Hkv Nq Nk D P q k v qb qh qn kb kh kn vb vh vn kp vp kph kpn vph vpn mask mb mh mn lengths table "
-          "starts offsets offset side two_sided out lse words wb wh wq distance").split()
+          "starts offsets offset side two_sided out lse words distance out_lo").split()
 
 
 def raw(**kw):

@@ -239,5 +239,5 @@ def test_empty_inputs_have_zero_gradients():
 def test_too_many_query_tiles_are_refused():
     q = torch.empty(1, 2049, 1, 64, device=DEV).half().requires_grad_(True)
     k = torch.empty(1, 1, 8, 64, device=DEV).half()
-    with pytest.raises(RuntimeError, match="1024"):
+    with pytest.raises(RuntimeError, match="2048"):
         cross_attention(q, k, k)
