@@ -270,18 +270,17 @@ SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
  * heads of a key head) and, with a bias, dtable [bias_buckets, H], all
  * contiguous and of `dtype`; formulas as for sma_attn_bwd, and
  *   dtable[bucket, h] = sum of dS over the pairs in the bucket.
- * Scratch: dq_accum (FP32 [B, H, Nq, D]), delta (FP32 [B, H, Nq]) and, with a
- * bias, bias_part (FP32, sma_cross_attn_bwd_bias_floats(args) elements).
+ * scratch: sma_cross_attn_bwd_scratch(args) floats.
  * At most 2048 steps of 64 query rows per key head (SMA_ERR_UNSUPPORTED_N).
  * All values of K, V, Q and dO must be finite.  dq is accumulated by atomic
  * adds in FP32, so its last bits can differ from run to run; dk, dv and
  * dtable do not.
  */
 SMA_API int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
-                               float* dq_accum, float* delta, float* bias_part, void* stream);
+                               float* scratch, void* stream);
 
-/* Elements of bias_part; 0 without a bias, -1 for arguments that the backward refuses. */
-SMA_API int64_t sma_cross_attn_bwd_bias_floats(const sma_attn_args* args);
+/* Floats of scratch sma_cross_attn_bwd needs; -1 for arguments that it refuses. */
+SMA_API int64_t sma_cross_attn_bwd_scratch(const sma_attn_args* args);
 
 /*
  * Synchronise `stream`, then report whether any kernel of this library on the

@@ -6,9 +6,10 @@
 //   dV = P^T dO,  dS = P * (dO V^T - Delta),  Delta_i = sum_d dO_id O_id
 //   dQ = scale * dS K,  dK = scale * dS^T Q,  dtable[bucket, h] = sum of dS over the bucket's pairs
 //
-// Kernels, in stream order: cross_delta_kernel (Delta; clears the FP32 dQ
-// accumulator), cross_bwd_kernel, cross_dq_kernel (accumulator -> dq) and,
-// with a bias, bias_reduce_kernel.
+// Kernels, in stream order: transpose_words_kernel (the packed mask by key,
+// where query rows have masks of their own), cross_delta_kernel (Delta, and
+// clears the FP32 dQ accumulator), cross_bwd_kernel, cross_dq_kernel
+// (accumulator -> dq) and, with a bias, bias_reduce_kernel.
 //
 // cross_bwd_kernel is persistent, one CTA per SM, over items (batch, key head,
 // 128-key tile).  K and V of the item stay in shared memory, dK and dV
@@ -34,8 +35,11 @@
 // the element-wise warps have read by then.  Four epilogue warps add it into
 // the FP32 accumulator by TMA bulk reduce-adds.
 //
-// Warps: 0-7 element-wise, 8 loader (TMA; mask words, LSE and Delta staged in
-// shared memory), 9 MMA issuer and TMEM owner, 10-13 epilogue, 14 scanner
+// Warps: 0-7 element-wise (each thread reads the 64 mask bits of its key for a
+// step as one 8-byte word, a step ahead), 8 loader (Q, dO, K, V by TMA, LSE and
+// Delta by cp.async, kRing steps ahead with nothing held in registers: a
+// loader that carried them through registers ran at one step per load
+// latency), 9 MMA issuer and TMEM owner, 10-13 epilogue, 14 scanner
 // (each item's live steps, kSlots items ahead).  Every wait is bounded and
 // reports through the device error word.
 //
@@ -87,8 +91,7 @@ struct Cfg {
   static constexpr int kOffDO = kOffQ + kRing * kQBytes;
   static constexpr int kOffDS = kOffDO + kRing * kQBytes;
   static constexpr int kOffDQ = kOffDS + kDSSlots * kDSBytes;  // 4 KiB box per epilogue warp
-  static constexpr int kOffMask = kOffDQ + 4 * 4096;           // [ring][4 words][64 rows]
-  static constexpr int kOffLse = kOffMask + kRing * 4 * kQ * 4;
+  static constexpr int kOffLse = kOffDQ + 4 * 4096;
   static constexpr int kOffDelta = kOffLse + kRing * kQ * 4;
   static constexpr int kOffCtl = kOffDelta + kRing * kQ * 4;
 };
@@ -128,6 +131,10 @@ struct BwdGeo {
   const uint32_t* words;   // packed mask rows (16-byte aligned), or nullptr: every key is kept
   int64_t word_stride[3];  // batch, head, query, in words (0: broadcast)
   int one_row;             // all query rows of an item have the same mask row
+  // Otherwise the mask by key, [..][key of KT * 128] 64-bit words of a step's
+  // rows, strides in such words for batch, head block (ht) and 64-query step.
+  const uint2* words_t;
+  int64_t t_stride[3];
   // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
   const float* bias;
   const int32_t* bias_offsets;
@@ -161,13 +168,60 @@ __device__ __forceinline__ int next_live(const uint32_t* bits, int& w, uint32_t&
   return w * 32 + b;
 }
 
-// Delta[row] = sum_d dO[row, d] * (O[row, d] + its rounding residual) in FP32,
-// D/8 threads per row; each thread also clears its 8 elements of the FP32 dQ
-// accumulator.  Bound by HBM: three 16-bit reads and a 32-bit write per element.
+// 32 x 32 bit transpose over a warp: bit k of lane r goes to bit r of lane k.
+// Five exchanges of halves of ever smaller blocks.
+__device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    const uint32_t low = w == 16 ? 0x0000FFFFu : w == 8 ? 0x00FF00FFu : w == 4 ? 0x0F0F0F0Fu : w == 2 ? 0x33333333u : 0x55555555u;
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, w);
+    x = (lane & w) ? (((y >> w) & low) | (x & ~low)) : ((x & low) | ((y & low) << w));
+  }
+  return x;
+}
+
+// words (rows of queries) -> words_t (BwdGeo): one warp per (batch, head block,
+// step, 32 keys), its 64 rows' words transposed.  Bound by reading and writing
+// the packed mask once, mostly in L2.
+constexpr int kTransposeWarps = 8;
+__global__ void __launch_bounds__(kTransposeWarps * 32)
+    transpose_words_kernel(const __grid_constant__ BwdGeo x, uint2* __restrict__ out, int Bm, int Hm, int key_words,
+                           int64_t total) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kTransposeWarps + (threadIdx.x >> 5);
+  if (w >= total) return;
+  // [Bm][Hm head blocks][QT1][key_words]
+  const int kw = static_cast<int>(w % key_words);
+  int64_t rest = w / key_words;
+  const int qt = static_cast<int>(rest % x.QT1);
+  rest /= x.QT1;
+  const int hm = static_cast<int>(rest % Hm);
+  const int64_t b = rest / Hm;
+  uint32_t v[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u, hr = i / x.tn, t = qt * kQ + i - hr * x.tn;
+    const int64_t h = static_cast<int64_t>(hm) * x.hb + hr;
+    v[u] = i < x.rows && t < x.Nq
+               ? __ldg(x.words + b * x.word_stride[0] + h * x.word_stride[1] + t * x.word_stride[2] + kw)
+               : 0u;
+    v[u] = transpose_bits(v[u], lane);
+  }
+  out[w * 32 + lane] = make_uint2(v[0], v[1]);
+}
+
+// Per row: -Delta, Delta = sum_d dO[row, d] * (O[row, d] + its rounding
+// residual) in FP32, and -lse * log2(e) (negated, so that the element-wise
+// pass adds them in packed pairs); D/8 threads per row, each of which also
+// clears its 8 elements of the FP32 dQ accumulator.  Bound by HBM: three
+// 16-bit reads and a 32-bit write per element.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256)
     cross_delta_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ out, const uint4* __restrict__ out_lo,
-                       float* __restrict__ delta, float4* __restrict__ dq_acc, int64_t rows) {
+                       const float* __restrict__ lse, float* __restrict__ neg_delta, float* __restrict__ neg_lse2,
+                       float4* __restrict__ dq_acc, int64_t rows) {
   constexpr int kPerRow = D / 8;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
@@ -189,7 +243,12 @@ __global__ void __launch_bounds__(256)
   }
 #pragma unroll
   for (int o = 1; o < kPerRow; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (row < rows && (threadIdx.x % kPerRow) == 0) delta[row] = acc;
+  if (row < rows && (threadIdx.x % kPerRow) == 0) {
+    neg_delta[row] = -acc;
+    // -FLT_MAX (a row with no kept key) becomes +inf; such a row has no mask
+    // bit, so its P is 0 by the select and never uses this value.
+    neg_lse2[row] = -(lse[row] * kLog2e);
+  }
 }
 
 // dq[i] = acc[i] in the input dtype, 8 elements per thread.
@@ -234,8 +293,8 @@ template <int D, bool BF16, bool kBias>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                     const __grid_constant__ CUtensorMap tm_dq, const float* __restrict__ lse,
-                     const float* __restrict__ delta, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int KT,
+                     const __grid_constant__ CUtensorMap tm_dq, const float* __restrict__ neg_lse2,
+                     const float* __restrict__ neg_delta, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int KT,
                      int total_items, float scale, const __grid_constant__ BwdGeo x, uint32_t* err_word,
                      uint64_t timeout_ns) {
   using C = Cfg<D>;
@@ -247,10 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   Ctl& ctl = *reinterpret_cast<Ctl*>(smem + C::kOffCtl);
-  // Per ring slot b: word w of query row i at s_mask[(b * 4 + w) * kQ + i];
-  // -LSE * log2(e) and -Delta per query row at s_lse / s_delta [b * kQ + i]
-  // (negated, so that the element-wise pass adds them in packed pairs).
-  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  // Per ring slot b, row i: -LSE * log2(e) and -Delta at s_lse / s_delta
+  // [b * kQ + i], 0 for rows past the problem's (whose Q and dO are 0 too, so
+  // that their P and dS reach nothing).
   float* s_lse = reinterpret_cast<float*>(smem + C::kOffLse);
   float* s_delta = reinterpret_cast<float*>(smem + C::kOffDelta);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -276,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ctl.dq_free[b]), 4);
     }
     for (int b = 0; b < 4; ++b) {
-      mbar_init(smem_u32(&ctl.ld_full[b]), 1);
+      mbar_init(smem_u32(&ctl.ld_full[b]), 1 + 32);  // TMA bytes, and every lane's cp.async
       mbar_init(smem_u32(&ctl.tile_free[b]), 5);  // a stage's element-wise warps and the MMA issuer
     }
     for (int sl = 0; sl < kSlots; ++sl) {
@@ -325,6 +383,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto step_head = [&](int v) { return v / x.QT1 * x.hb; };  // relative to h0
   auto step_q0 = [&](int v) { return v % x.QT1 * kQ; };
+  // The 128 words (by key) of step v of an item, where the mask is by key.
+  auto step_words = [&](const Item& it, int v) {
+    const int ht = v / x.QT1;
+    return x.words_t + it.b * x.t_stride[0] + (it.hkv * x.gh + ht) * x.t_stride[1] + (v - ht * x.QT1) * x.t_stride[2] +
+           it.kt * kKeys;
+  };
   // Whole-warp wait.
   auto wait_all = [&](uint64_t& bar, uint32_t parity) -> bool {
     const bool all = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&bar), parity, abort_flag, timeout_ns));
@@ -348,7 +412,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     bool ok = true;
     int lt = 0, li = 0;
-    int last_copy = -1;
     // Query and head of this lane's rows (lane, lane + 32) within a step.
     int rt[2], rh[2];
     bool rin[2];
@@ -359,27 +422,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       rh[u] = rin[u] ? i / x.tn : 0;
       rt[u] = rin[u] ? i - rh[u] * x.tn : 0;
     }
-    // Mask words, LSE and Delta of step v of an item, two rows per lane: all
-    // loads issued at once, into registers.
-    auto fetch = [&](const Item& it, int v, uint4 (&w4)[2], float (&l2)[2], float (&de)[2]) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = step_q0(v) + rt[u], h = it.h0 + step_head(v) + rh[u];
-        const bool in = rin[u] && t < x.Nq;
-        const int64_t row = in ? (static_cast<int64_t>(it.b) * x.H + h) * x.Nq + t : 0;
-        w4[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (in) {
-          if (x.words == nullptr) {
-            w4[u] = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
-          } else {
-            w4[u] = __ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] + h * x.word_stride[1] +
-                                                         t * x.word_stride[2] + it.kt * 4));
-          }
-        }
-        l2[u] = in ? __ldg(lse + row) : 0.f;
-        de[u] = in ? __ldg(delta + row) : 0.f;
-      }
-    };
     auto issue_kv = [&](const Item& it) -> bool {
       const int b = li % C::kKVBufs;
       if (li >= C::kKVBufs &&
@@ -400,44 +442,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++li;
       return true;
     };
-    auto stage = [&](const Item& it, int v, const uint4 (&w4)[2], const float (&l2)[2], const float (&de)[2]) -> bool {
+    // Step v of an item into ring slot lt % kRing, once the element-wise warps
+    // and the products are done with the step before in it.
+    auto stage = [&](const Item& it, int v) -> bool {
       const int b = lt % kRing;
       if (lt >= kRing &&
           !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&ctl.tile_free[b]), ((lt - kRing) / kRing) & 1,
                                                      abort_flag, timeout_ns)))
         return false;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int i = lane + 32 * u;
-        const uint32_t w[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          s_mask[(b * 4 + k) * kQ + i] = w[k] & low_bits(x.Nk - it.kt * kKeys - 32 * k);
-        // -FLT_MAX (a row with no kept key) becomes +inf here; such a row has
-        // no mask bit, so its P is 0 by the select and never uses this value.
-        s_lse[b * kQ + i] = -(l2[u] * kLog2e);
-        s_delta[b * kQ + i] = -de[u];
-      }
-      __syncwarp();
+      const uint32_t bar = smem_u32(&ctl.ld_full[b]);
+      const int q0 = step_q0(v), h0 = it.h0 + step_head(v);
       if (lane == 0) {
-        const uint32_t bar = smem_u32(&ctl.ld_full[b]);
-        const int q0 = step_q0(v), h = it.h0 + step_head(v);
         mbar_arrive_expect_tx(bar, 2 * x.rows * D * 2);
 #pragma unroll
         for (int dc = 0; dc < C::kDChunks; ++dc) {
-          tma_load_4d(base + C::kOffQ + b * C::kQBytes + dc * kQ * 128, &tm_q, bar, dc * 64, q0, h, it.b);
-          tma_load_4d(base + C::kOffDO + b * C::kQBytes + dc * kQ * 128, &tm_do, bar, dc * 64, q0, h, it.b);
+          tma_load_4d(base + C::kOffQ + b * C::kQBytes + dc * kQ * 128, &tm_q, bar, dc * 64, q0, h0, it.b);
+          tma_load_4d(base + C::kOffDO + b * C::kQBytes + dc * kQ * 128, &tm_do, bar, dc * 64, q0, h0, it.b);
         }
-        last_copy = lt;
       }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = q0 + rt[u];
+        const bool in = rin[u] && t < x.Nq;
+        const int64_t row = in ? (static_cast<int64_t>(it.b) * x.H + h0 + rh[u]) * x.Nq + t : 0;
+        cp_async4_zfill(smem_u32(s_lse + b * kQ + lane + 32 * u), neg_lse2 + row, in);
+        cp_async4_zfill(smem_u32(s_delta + b * kQ + lane + 32 * u), neg_delta + row, in);
+      }
+      cp_async_arrive(bar);
       ++lt;
       return true;
     };
-    // The loads of the next live step are issued before this one waits for
-    // its slot; at an item's last step, those of the next item's first.
-    uint4 nw[2];
-    float nl[2], nd[2];
-    bool have_next = false;
     for (int j = 0; ok && j < n_items; ++j) {
       const int sl = j % kSlots;
       if (!wait_all(ctl.item_full[sl], (j / kSlots) & 1)) {
@@ -447,61 +481,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n = static_cast<int>(ctl.n_live[sl]);
       if (n > 0) {
         const Item it = item_at(j);
-        if (!issue_kv(it)) {
-          ok = false;
-          break;
-        }
+        ok = issue_kv(it);
         int cw = 0;
         uint32_t cx = ctl.live_bits[sl][0];
-        int v_next = next_live(ctl.live_bits[sl], cw, cx);
-        if (!have_next) fetch(it, v_next, nw, nl, nd);
-        have_next = false;
-        for (int t = 0; t < n; ++t) {
-          const int v = v_next;
-          uint4 w4[2];
-          float l2[2], de[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            w4[u] = nw[u];
-            l2[u] = nl[u];
-            de[u] = nd[u];
-          }
-          if (t + 1 < n) {
-            v_next = next_live(ctl.live_bits[sl], cw, cx);
-            fetch(it, v_next, nw, nl, nd);
-          } else if (j + 1 < n_items) {
-            // Published kSlots items ahead of the slowest reader, so never
-            // behind this warp's own release.
-            const int sl1 = (j + 1) % kSlots;
-            if (!wait_all(ctl.item_full[sl1], ((j + 1) / kSlots) & 1)) {
-              ok = false;
-              break;
-            }
-            if (ctl.n_live[sl1] > 0u) {
-              int w1 = 0;
-              uint32_t x1 = ctl.live_bits[sl1][0];
-              const int v1 = next_live(ctl.live_bits[sl1], w1, x1);
-              fetch(item_at(j + 1), v1, nw, nl, nd);
-              have_next = true;
-            }
-          }
-          if (!stage(it, v, w4, l2, de)) {
-            ok = false;
-            break;
-          }
-        }
+        for (int t = 0; ok && t < n; ++t) ok = stage(it, next_live(ctl.live_bits[sl], cw, cx));
         if (!ok) break;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_free[sl]));
     }
+    cp_async_wait_all();
     if (!ok && lane == 0) {
       fail();
       // Let the copies this warp started land before the CTA exits.
       uint32_t zero = 0;
       for (int jj = li - C::kKVBufs; jj < li; ++jj)
         if (jj >= 0) mbar_wait_bounded(smem_u32(&ctl.kv_full[jj % C::kKVBufs]), (jj / C::kKVBufs) & 1, &zero, timeout_ns);
-      for (int g = last_copy - kRing + 1; g <= last_copy; ++g)
+      for (int g = lt - kRing; g < lt; ++g)
         if (g >= 0) mbar_wait_bounded(smem_u32(&ctl.ld_full[g % kRing]), (g / kRing) & 1, &zero, timeout_ns);
     }
   } else if (warp == kMmaWarp) {
@@ -669,17 +665,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kScanWarp) {
     // ================================================================ scanner
     // Item j's live list: bit v set when some query row of step v keeps a key
-    // of the item's tile.  8 steps per batch of loads, 2 rows per lane.
+    // of the item's tile.  A step's words of the tile are 1 KiB in a row, 32
+    // bytes per lane; 8 steps per batch of loads.
     bool ok = true;
-    int rt[2], rh[2];
-    bool rin[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i = lane + 32 * u;
-      rin[u] = i < x.rows;
-      rh[u] = rin[u] ? i / x.tn : 0;
-      rt[u] = rin[u] ? i - rh[u] * x.tn : 0;
-    }
     for (int j = 0; j < n_items; ++j) {
       const int sl = j % kSlots;
       if (j >= kSlots && !wait_all(ctl.item_free[sl], ((j / kSlots) - 1) & 1)) {
@@ -687,19 +675,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const Item it = item_at(j);
-      uint32_t vmask[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) vmask[w] = low_bits(x.Nk - it.kt * kKeys - 32 * w);
-      auto any_of = [&](const uint4& m) {
-        return (m.x & vmask[0]) | (m.y & vmask[1]) | (m.z & vmask[2]) | (m.w & vmask[3]);
-      };
       uint32_t mine[2] = {0u, 0u};  // words lane and lane + 32 of the list
-      if (x.words == nullptr || x.one_row) {
+      if (x.words_t == nullptr) {
         // No mask, or one mask row for the whole item: all steps or none.
         bool any = true;
-        if (x.words != nullptr)
-          any = any_of(__ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] +
-                                                            it.h0 * x.word_stride[1] + it.kt * 4))) != 0u;
+        if (x.words != nullptr) {
+          const uint4 m = __ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] +
+                                                               it.h0 * x.word_stride[1] + it.kt * 4));
+          any = (m.x | m.y | m.z | m.w) != 0u;
+        }
         if (any) {
           mine[0] = low_bits(VT - 32 * lane);
           mine[1] = low_bits(VT - 32 * (lane + 32));
@@ -708,20 +692,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int v0 = 0; v0 < VT; v0 += 8) {
           uint4 m[8][2];
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-#pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-              const int t = step_q0(v0 + u) + rt[rr], h = it.h0 + step_head(v0 + u) + rh[rr];
-              m[u][rr] = make_uint4(0u, 0u, 0u, 0u);
-              if (v0 + u < VT && rin[rr] && t < x.Nq)
-                m[u][rr] = __ldg(reinterpret_cast<const uint4*>(x.words + it.b * x.word_stride[0] +
-                                                                h * x.word_stride[1] + t * x.word_stride[2] +
-                                                                it.kt * 4));
-            }
+          for (int u = 0; u < 8; ++u) {
+            const uint4* src = reinterpret_cast<const uint4*>(step_words(it, min(v0 + u, VT - 1))) + lane * 2;
+            m[u][0] = __ldg(src);
+            m[u][1] = __ldg(src + 1);
+          }
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const int v = v0 + u;
-            const bool any = __any_sync(0xffffffffu, (any_of(m[u][0]) | any_of(m[u][1])) != 0u);
+            const uint32_t o = m[u][0].x | m[u][0].y | m[u][0].z | m[u][0].w | m[u][1].x | m[u][1].y | m[u][1].z | m[u][1].w;
+            const bool any = __any_sync(0xffffffffu, o != 0u) && v < VT;
             if (any && lane == ((v >> 5) & 31)) {
               if (v < 1024) mine[0] |= 1u << (v & 31);
               else mine[1] |= 1u << (v & 31);
@@ -745,30 +725,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float c2 = scale * kLog2e;
     const uint64_t c2x2 = f2(c2, c2);
-    const int my_word = (t >> 5) * kQ;     // the word holding this key, for each query row
-    const uint32_t kbit = 1u << (t & 31);  // this key's bit in it
     bool ok = true;
     uint32_t lt0 = 0, lp0 = 0, use = 0;
+    // Mask bits of this key for the 64 queries of the next step of this stage.
+    uint2 next_words = make_uint2(0u, 0u);
+    bool have_words = false;
+    auto item_bit = [&](const Item& it) -> uint2 {  // one mask row for the item
+      const int key = it.kt * kKeys + t;
+      uint32_t bit = key < x.Nk ? 1u : 0u;
+      if (x.words != nullptr)
+        bit &= __ldg(x.words + it.b * x.word_stride[0] + it.h0 * x.word_stride[1] + (key >> 5)) >> (key & 31);
+      return bit ? make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu) : make_uint2(0u, 0u);
+    };
+    auto fetch_words = [&](const Item& it, int v) {
+      return x.words_t != nullptr ? __ldg(step_words(it, v) + t) : item_bit(it);
+    };
     for (int j = 0; ok && j < n_items; ++j) {
       const int sl = j % kSlots;
       ok = wait_all(ctl.item_full[sl], (j / kSlots) & 1);
       if (!ok) break;
       const int n = static_cast<int>(ctl.n_live[sl]);
-      if constexpr (!kBias) arrive_warp(ctl.item_free[sl]);  // only the count is needed
-      // kBias: this warp's 32-key block, the walk over the steps, and the bias
-      // gradient of blocks beyond the last bucket's start, per head.
-      int cw = 0, key0 = 0, off = 0, far_head = -1;
-      uint32_t cx = 0u;
+      const Item it = item_at(j);
+      int cw = 0;
+      uint32_t cx = ctl.live_bits[sl][0];
+      if (g == 1) next_live(ctl.live_bits[sl], cw, cx);
+      int v_next = n > g ? next_live(ctl.live_bits[sl], cw, cx) : -1;
+      if (n > g && !have_words) next_words = fetch_words(it, v_next);
+      have_words = false;
+      // kBias: this warp's 32-key block, and the bias gradient of blocks
+      // beyond the last bucket's start, per head.
+      int key0 = 0, off = 0, far_head = -1;
       float far_lo = 0.f, far_hi = 0.f;
-      Item it{};
       if constexpr (kBias) {
-        it = item_at(j);
         key0 = it.kt * kKeys + (warp & 3) * 32;
         off = x.bias_offsets == nullptr
                   ? x.bias_offset
                   : max(-kMaxBiasOffset, min(kMaxBiasOffset, __ldg(x.bias_offsets + it.b)));
-        cx = ctl.live_bits[sl][0];
-        if (g == 1) next_live(ctl.live_bits[sl], cw, cx);
       }
       auto flush_far = [&]() {
         if constexpr (kBias) {
@@ -789,18 +781,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tt = g; tt < n; tt += 2, ++use) {
         const uint32_t lt = lt0 + tt;
         const int b = lt % kRing;
+        const int v = v_next;
+        const uint2 words = next_words;
         int head = 0, q0 = 0;
         if constexpr (kBias) {
-          const int v = next_live(ctl.live_bits[sl], cw, cx);
-          next_live(ctl.live_bits[sl], cw, cx);  // the other stage's
-          head = it.h0 + step_head(v);           // hb = 1
+          head = it.h0 + step_head(v);  // hb = 1
           q0 = step_q0(v);
           if (head != far_head) {
             flush_far();
             far_head = head;
           }
         }
-        const uint32_t* my_words = s_mask + b * 4 * kQ + my_word;
+        // The next step's words, a step ahead; at the last one those of the
+        // next item's first (its list needs nothing of this item).
+        if (tt + 2 < n) {
+          next_live(ctl.live_bits[sl], cw, cx);  // the other stage's
+          v_next = next_live(ctl.live_bits[sl], cw, cx);
+          if (x.words_t != nullptr) next_words = fetch_words(it, v_next);
+        } else if (j + 1 < n_items) {
+          const int sl1 = (j + 1) % kSlots;
+          ok = wait_all(ctl.item_full[sl1], ((j + 1) / kSlots) & 1);
+          if (!ok) break;
+          if (static_cast<int>(ctl.n_live[sl1]) > g) {
+            int w1 = 0;
+            uint32_t x1 = ctl.live_bits[sl1][0];
+            if (g == 1) next_live(ctl.live_bits[sl1], w1, x1);
+            const int v1 = next_live(ctl.live_bits[sl1], w1, x1);
+            next_words = fetch_words(item_at(j + 1), v1);
+            have_words = true;
+          }
+        }
         const float* t_lse = s_lse + b * kQ;
         const float* t_delta = s_delta + b * kQ;
         uint8_t* ds_row = smem + C::kOffDS +
@@ -809,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
+          const uint32_t word = c == 0 ? words.x : words.y;
           float s[32], dp[32];
           tmem_ld32f(t_lane + col_s(g) + c * 32, s);
           tmem_ld32f(t_lane + col_dp(g) + c * 32, dp);
@@ -829,10 +840,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pw[16], dw[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const uint4 m4 = *reinterpret_cast<const uint4*>(my_words + c * 32 + e);
             const float4 l4 = *reinterpret_cast<const float4*>(t_lse + c * 32 + e);
             const float4 d4 = *reinterpret_cast<const float4*>(t_delta + c * 32 + e);
-            const uint32_t mm[4] = {m4.x, m4.y, m4.z, m4.w};
             // y = s * scale * log2(e) + bias - lse2 and ds = p * (dp - Delta), two queries per instruction.
             uint64_t l01 = f2(l4.x, l4.y), l23 = f2(l4.z, l4.w);
             if constexpr (kBias) {
@@ -848,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             f2_split(fma2(f2(s[e], s[e + 1]), c2x2, l01), y[0], y[1]);
             f2_split(fma2(f2(s[e + 2], s[e + 3]), c2x2, l23), y[2], y[3]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = (mm[u] & kbit) ? ex2f(y[u]) : 0.f;
+            for (int u = 0; u < 4; ++u) p[u] = (word & (1u << (e + u))) ? ex2f(y[u]) : 0.f;
             f2_split(mul2(f2(p[0], p[1]), add2(f2(dp[e], dp[e + 1]), f2(d4.x, d4.y))), ds[0], ds[1]);
             f2_split(mul2(f2(p[2], p[3]), add2(f2(dp[e + 2], dp[e + 3]), f2(d4.z, d4.w))), ds[2], ds[3]);
             pw[e / 2] = pack2<BF16>(p[0], p[1]);
@@ -897,11 +906,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       lt0 += n;
       lp0 += (n + 1) / 2;
-      if constexpr (kBias) {
-        if (!ok) break;
-        flush_far();
-        arrive_warp(ctl.item_free[sl]);
-      }
+      if (!ok) break;
+      flush_far();
+      arrive_warp(ctl.item_free[sl]);
     }
     if (!ok && lane == 0) fail();
   } else {
@@ -1133,6 +1140,11 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
   x->words = p.words;
   for (int i = 0; i < 3; ++i) x->word_stride[i] = p.word_stride[i];
   x->one_row = p.words != nullptr && (x->Nq == 1 || p.word_stride[2] == 0) && (G == 1 || p.word_stride[1] == 0);
+  if (p.words != nullptr && !x->one_row) {
+    x->t_stride[2] = (p.Nk + kKeys - 1) / kKeys * kKeys;
+    x->t_stride[1] = p.word_stride[1] != 0 ? x->t_stride[2] * x->QT1 : 0;
+    x->t_stride[0] = p.word_stride[0] != 0 ? x->t_stride[2] * x->QT1 * (p.word_stride[1] != 0 ? p.H / x->hb : 1) : 0;
+  }
   if (bias) {
     x->bias = p.bias_distance;
     x->bias_offsets = p.bias.offsets;
@@ -1148,6 +1160,23 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
     x->slots = std::min(slots, x->QB);
   }
   return static_cast<int64_t>(x->gh) * x->QT1 <= kMaxSteps;
+}
+
+// Offsets, in floats, within the scratch of a backward: the FP32 accumulator of
+// dq at 0, -Delta and -lse2, the mask by key, partial sums of the bias gradient.
+struct Scratch {
+  int64_t delta, words, bias, end;
+};
+Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
+  auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
+  const int64_t rows = p.B * p.H * p.Nq;
+  Scratch s{};
+  s.delta = rows * p.D;
+  s.words = s.delta + up(2 * rows);
+  const int64_t Bm = p.word_stride[0] != 0 ? p.B : 1, Hm = p.word_stride[1] != 0 ? p.H / x.hb : 1;
+  s.bias = s.words + 2 * Bm * Hm * x.QT1 * x.t_stride[2];
+  s.end = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0);
+  return s;
 }
 
 template <int D, bool BF16, bool kBias>
@@ -1170,7 +1199,7 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
   if (rc == CUDA_SUCCESS) rc = make_tensor_map_4d(&mdo, g.dout, p.dtype, D, p.Nq, p.H, p.B, so, x.tn, x.hb);
   // The accumulator in blocks of hb * Nq rows: a step's rows are consecutive in it.
   if (rc == CUDA_SUCCESS)
-    rc = make_tensor_map_3d_f32(&mdq, g.dq_accum, D, p.B * p.Hkv * x.gh, static_cast<int64_t>(x.hb) * p.Nq, 32);
+    rc = make_tensor_map_3d_f32(&mdq, g.scratch, D, p.B * p.Hkv * x.gh, static_cast<int64_t>(x.hb) * p.Nq, 32);
   if (rc != CUDA_SUCCESS) {
     *msg = tensor_map_error("backward", rc);
     return kErrCuda;
@@ -1182,22 +1211,34 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
   cudaError_t e = ensure_smem_limit(kern, kSmemBytes, dp.device, smem_set);
   if (e == cudaSuccess && kBias) {
     // Blocks that no live step visits count as 0.
-    const int64_t bh_kb = p.B * p.H * x.KB;
-    x.near_part = g.bias_part;
-    x.far_part = g.bias_part + bh_kb * x.slots * 64;
-    e = cudaMemsetAsync(g.bias_part, 0, static_cast<size_t>(bh_kb) * (x.slots * 64 + 4) * sizeof(float), p.stream);
+    const Scratch s = scratch_layout(p, x);
+    x.near_part = g.scratch + s.bias;
+    x.far_part = x.near_part + p.B * p.H * x.KB * x.slots * 64;
+    e = cudaMemsetAsync(x.near_part, 0, static_cast<size_t>(s.end - s.bias) * sizeof(float), p.stream);
+  }
+  const Scratch at = scratch_layout(p, x);
+  float* neg_delta = g.scratch + at.delta;
+  float4* dq_accum = reinterpret_cast<float4*>(g.scratch);
+  if (e == cudaSuccess && x.t_stride[2] != 0) {
+    const int Bm = p.word_stride[0] != 0 ? x.B : 1, Hm = p.word_stride[1] != 0 ? x.H / x.hb : 1;
+    const int key_words = static_cast<int>(KT * 4);
+    const int64_t total = static_cast<int64_t>(Bm) * Hm * x.QT1 * key_words;
+    uint2* words_t = reinterpret_cast<uint2*>(g.scratch + at.words);
+    e = launch_pdl(transpose_words_kernel, static_cast<unsigned>((total + kTransposeWarps - 1) / kTransposeWarps),
+                   kTransposeWarps * 32, 0, p.stream, x, words_t, Bm, Hm, key_words, total);
+    x.words_t = words_t;
   }
   if (e == cudaSuccess)
     e = launch_pdl(cross_delta_kernel<D, BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
                    static_cast<const uint4*>(g.dout), static_cast<const uint4*>(p.out),
-                   static_cast<const uint4*>(p.out_lo), g.delta, reinterpret_cast<float4*>(g.dq_accum), rows);
+                   static_cast<const uint4*>(p.out_lo), p.lse, neg_delta, neg_delta + rows, dq_accum, rows);
   if (e == cudaSuccess)
     e = launch_pdl(kern, static_cast<unsigned>(std::min<int64_t>(items, dp.sms)), kThreads, kSmemBytes, p.stream, mq, mk,
-                   mv, mdo, mdq, p.lse, g.delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),
+                   mv, mdo, mdq, neg_delta + rows, neg_delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),
                    static_cast<int>(KT), static_cast<int>(items), p.scale, x, p.err_word, p.timeout_ns);
   if (e == cudaSuccess)
     e = launch_pdl(cross_dq_kernel<BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
-                   reinterpret_cast<const float4*>(g.dq_accum), static_cast<uint4*>(g.dq), rows * D / 8);
+                   dq_accum, static_cast<uint4*>(g.dq), rows * D / 8);
   if (e == cudaSuccess && kBias) {
     const dim3 grid(static_cast<unsigned>(p.H), static_cast<unsigned>(p.bias.side * (p.bias.two_sided ? 2 : 1)));
     bias_reduce_kernel<BF16><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, g.dtable);
@@ -1217,10 +1258,10 @@ int launch_b(const CrossParams& p, const CrossGrads& g, const BwdGeo& x, const c
 
 }  // namespace
 
-int64_t cross_bwd_bias_floats(const CrossParams& p) {
+int64_t cross_bwd_scratch_floats(const CrossParams& p) {
   BwdGeo x{};
   geometry(p, &x);
-  return p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0;
+  return scratch_layout(p, x).end;
 }
 
 int launch_attn_cross_bwd(const CrossParams& p, const CrossGrads& g, const char** msg) {

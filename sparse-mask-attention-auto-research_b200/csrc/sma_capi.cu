@@ -449,7 +449,7 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
 }
 
 int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
-                       float* dq_accum, float* delta, float* bias_part, void* stream) {
+                       float* scratch, void* stream) {
   NvtxRange range("sma_cross_attn_bwd");
   sma::CrossParams p{};
   bool empty = false;
@@ -459,24 +459,23 @@ int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, vo
   if (p.P > 0 || p.lengths) return fail(sma::kErrArg, "backward: no prefix and no lengths");
   rc = tile_params(args, &p);
   if (rc != sma::kOk) return rc;
-  if (!p.lse || !p.out_lo || !dout || !dq || !dk || !dv || !dq_accum || !delta || (p.bias.table && (!dtable || !bias_part)))
+  if (!p.lse || !p.out_lo || !dout || !dq || !dk || !dv || !scratch || (p.bias.table && !dtable))
     return fail(sma::kErrArg, "backward: null pointer");
-  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(dq_accum) ||
-      !aligned16(bias_part))
-    return fail(sma::kErrArg, "backward: dout/dq/dk/dv/dq_accum/bias_part must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(delta) & 3u) || (reinterpret_cast<uintptr_t>(dtable) & 1u))
-    return fail(sma::kErrArg, "backward: misaligned delta or dtable");
-  const sma::CrossGrads g{dout, dq, dk, dv, dq_accum, delta, dtable, bias_part};
+  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(scratch))
+    return fail(sma::kErrArg, "backward: dout/dq/dk/dv/scratch must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(dtable) & 1u) return fail(sma::kErrArg, "backward: misaligned dtable");
+  const sma::CrossGrads g{dout, dq, dk, dv, dtable, scratch};
   const char* msg = nullptr;
   rc = sma::launch_attn_cross_bwd(p, g, &msg);
   return rc == sma::kOk ? rc : fail(rc, msg);
 }
 
-int64_t sma_cross_attn_bwd_bias_floats(const sma_attn_args* args) {
+int64_t sma_cross_attn_bwd_scratch(const sma_attn_args* args) {
   sma::CrossParams p{};
   bool empty = false;
-  if (cross_params(args, nullptr, &p, &empty) != sma::kOk || empty || p.Nk == 0 || tile_params(args, &p) != sma::kOk) return -1;
-  return sma::cross_bwd_bias_floats(p);
+  if (cross_params(args, nullptr, &p, &empty) != sma::kOk || empty || p.Nk == 0 || tile_params(args, &p) != sma::kOk)
+    return -1;
+  return sma::cross_bwd_scratch_floats(p);
 }
 
 int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream) {

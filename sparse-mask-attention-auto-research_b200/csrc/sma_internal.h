@@ -163,12 +163,10 @@ struct CrossGrads {
   void* dq;          // [B, H, Nq, D]
   void* dk;          // [B, Hkv, Nk, D]
   void* dv;
-  float* dq_accum;   // [B, H, Nq, D] scratch
-  float* delta;      // [B, H, Nq] scratch
   void* dtable;      // [buckets, H], with a bias
-  float* bias_part;  // cross_bwd_bias_floats scratch, with a bias
+  float* scratch;    // cross_bwd_scratch_floats elements
 };
-int64_t cross_bwd_bias_floats(const CrossParams& p);
+int64_t cross_bwd_scratch_floats(const CrossParams& p);
 int launch_attn_cross_bwd(const CrossParams& p, const CrossGrads& g, const char** msg);
 
 constexpr int kRowsTile = 16;  // rows of a tile of attn_rows.cu

@@ -193,6 +193,20 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// 4-byte asynchronous copy global -> shared by this thread; without `in` the
+// destination is zeroed and the source not read.
+__device__ __forceinline__ void cp_async4_zfill(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
+               "r"(in ? 4 : 0)
+               : "memory");
+}
+// Arrives on `bar` (counted in its initial count) when this thread's earlier
+// cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Hint: bring `bytes` of global memory at `src` into L2 (no completion to
 // wait for, no registers held).  Address and size multiples of 16 bytes.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {

@@ -67,8 +67,8 @@ SIGNATURES = {
     ),
     "sma_rows_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_cross_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
-    "sma_cross_attn_bwd": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "sma_cross_attn_bwd_bias_floats": (_i64, [ctypes.c_char_p]),
+    "sma_cross_attn_bwd": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sma_cross_attn_bwd_scratch": (_i64, [ctypes.c_char_p]),
     "sma_prefix_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_device_status": (ctypes.c_int, [_vp, ctypes.c_int]),
     "sma_set_wait_timeout_ns": (ctypes.c_int, [ctypes.c_uint64]),

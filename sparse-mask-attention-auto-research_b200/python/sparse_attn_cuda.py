@@ -345,22 +345,14 @@ def cross_backward(dout, q, k, v, out, scale, saved, mask_strides=None, bias=Non
     dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
     dv = torch.empty_like(dk)
     with _device_guard(q.device):
-        # Scratch: the FP32 accumulator of dq, Delta, and partial sums of the bias gradient.
-        n_q = q.numel()
-        n_delta = (n_q // q.shape[3] + 3) // 4 * 4
-        n_bias, dtable = 0, None
-        if bias is not None:
-            dtable = torch.empty_like(bias.table)
-            n_bias = lib.sma_cross_attn_bwd_bias_floats(args)
-            _require(n_bias >= 0, "backward: unsupported arguments")
-        scratch = torch.empty(n_q + n_delta + n_bias, dtype=torch.float32, device=q.device)
-        acc = scratch.data_ptr()
+        dtable = None if bias is None else torch.empty_like(bias.table)
+        floats = lib.sma_cross_attn_bwd_scratch(args)
+        _require(floats >= 0, "backward: unsupported arguments")
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         _lib.check(
-            lib.sma_cross_attn_bwd(
-                args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                None if dtable is None else dtable.data_ptr(), acc, acc + 4 * n_q,
-                None if dtable is None else acc + 4 * (n_q + n_delta), _stream_ptr(q.device),
-            )
+            lib.sma_cross_attn_bwd(args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   None if dtable is None else dtable.data_ptr(), scratch.data_ptr(),
+                                   _stream_ptr(q.device))
         )
     return dq, dk, dv, dtable
 
