@@ -25,7 +25,7 @@
 //             rounded over the S^T columns, dS to shared memory
 //
 // What bounds it: per 64 queries, 16 (D = 64: four S^T, four dP^T, four dV,
-// four dK) tensor instructions at about 64 cycles, the dQ product, and 8192
+// four dK) tensor instructions at 31 to 47 cycles, the dQ product, and 8192
 // exponentials with some ten instructions each; with the two in turn (one
 // step in flight) each waited for the other.
 //
@@ -502,8 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ================================================================ MMA issuer
+    // The whole warp walks along, converged; one elected lane issues.
     bool ok = true;
-    if (lane == 0) {
+    {
       constexpr int kBf = BF16 ? 1 : 0;
       constexpr uint32_t idesc_s = make_idesc_f16(kKeys, kQ, kBf, 0);                // S^T, dP^T
       constexpr uint32_t idesc_kv = make_idesc_f16(kKeys, D, kBf, 1);                // dV, dK (B M/N-major)
@@ -518,65 +519,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         int kv_free;
         uint32_t use;
       } pend;
-      auto wait = [&](uint64_t& bar, uint32_t parity) -> bool {
-        return mbar_wait_bounded(smem_u32(&bar), parity, abort_flag, timeout_ns);
-      };
+      // The descriptor `bytes` further on (addresses fit its field, in units of 16 bytes).
+      auto step = [](uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); };
       auto flush = [&]() -> bool {
         if (!pend.on) return true;
         pend.on = false;
         const int g = pend.g;
         // P and dS of the step; before the first products of a live item, the
         // epilogue warps must have read the previous one's dV / dK.
-        if (!wait(ctl.p_full[g], pend.use & 1)) return false;
-        if (pend.first && pend.li > 0 && !wait(ctl.acc_free, (pend.li - 1) & 1)) return false;
-        tc_fence_after();
+        if (!wait_all(ctl.p_full[g], pend.use & 1)) return false;
+        if (pend.first && pend.li > 0 && !wait_all(ctl.acc_free, (pend.li - 1) & 1)) return false;
         const uint32_t sQ = base + C::kOffQ + pend.slot * C::kQBytes, sDO = base + C::kOffDO + pend.slot * C::kQBytes;
         const uint32_t sK = base + C::kOffK + pend.kv * C::kKVBytes;
         const int ds_slot = C::kPairDQ ? static_cast<int>(lp & 1) * 2 + g : g;
         const uint32_t sDS = base + C::kOffDS + ds_slot * C::kDSBytes;
+        const uint64_t dDO = smem_desc_sw128(sDO, kQ * 128, 1024), dQ = smem_desc_sw128(sQ, kQ * 128, 1024);
+        const uint64_t dDS = smem_desc_sw128(sDS, 16, 1024), dK = smem_desc_sw128(sK, kKeys * 128, 1024);
         // 16 query rows per instruction: 8 packed TMEM columns of P^T, 32
         // bytes of dS's rows, 2048 bytes (16 rows of 128) of dO and Q, whose
         // 64-dim chunks are kQ * 128 bytes apart.
 #pragma unroll
         for (int kk = 0; kk < kQ / 16; ++kk)
-          mma_ts(tmem + kColDV, tmem + col_s(g) + kk * 8, smem_desc_sw128(sDO + kk * 2048, kQ * 128, 1024), idesc_kv,
+          mma_ts_warp(tmem + kColDV, tmem + col_s(g) + kk * 8, step(dDO, kk * 2048), idesc_kv,
                  (!pend.first || kk > 0) ? 1u : 0u);
 #pragma unroll
         for (int kk = 0; kk < kQ / 16; ++kk)
-          mma_ss(tmem + C::kColDK, smem_desc_sw128(sDS + kk * 32, 16, 1024),
-                 smem_desc_sw128(sQ + kk * 2048, kQ * 128, 1024), idesc_kv, (!pend.first || kk > 0) ? 1u : 0u);
-        mma_commit(smem_u32(&ctl.tile_free[pend.slot]));
+          mma_ss_warp(tmem + C::kColDK, step(dDS, kk * 32), step(dQ, kk * 2048), idesc_kv,
+                      (!pend.first || kk > 0) ? 1u : 0u);
+        mma_commit_warp(smem_u32(&ctl.tile_free[pend.slot]));
         if constexpr (C::kPairDQ) {
-          mma_commit(smem_u32(&ctl.pt_free[g]));
+          mma_commit_warp(smem_u32(&ctl.pt_free[g]));
           if (pend.pair_end) {
             // dQ = dS K of the pair (one step's rows are not used when the
             // item's last pair has only one): 16 keys per instruction, 2048
             // bytes into dS's two 64-query tiles and K.
             const int b = lp & 1;
-            if (lp >= 2 && !wait(ctl.dq_free[b], ((lp >> 1) - 1) & 1)) return false;
-            tc_fence_after();
-            const uint32_t sPair = base + C::kOffDS + b * 2 * C::kDSBytes;
+            if (lp >= 2 && !wait_all(ctl.dq_free[b], ((lp >> 1) - 1) & 1)) return false;
+                const uint64_t dPair = smem_desc_sw128(base + C::kOffDS + b * 2 * C::kDSBytes, C::kDSBytes, 1024);
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_ss(tmem + C::col_dq(b), smem_desc_sw128(sPair + kk * 2048, C::kDSBytes, 1024),
-                     smem_desc_sw128(sK + kk * 2048, kKeys * 128, 1024), idesc_q, kk > 0 ? 1u : 0u);
-            mma_commit(smem_u32(&ctl.dq_full[b]));
+              mma_ss_warp(tmem + C::col_dq(b), step(dPair, kk * 2048), step(dK, kk * 2048), idesc_q, kk > 0 ? 1u : 0u);
+            mma_commit_warp(smem_u32(&ctl.dq_full[b]));
             ++lp;
           }
         } else {
           // dQ^T = K^T dS^T of the step, over its dP^T columns.
+          const uint64_t dDSn = smem_desc_sw128(sDS, kKeys * 128, 1024);
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ss(tmem + col_dp(g), smem_desc_sw128(sK + kk * 2048, kKeys * 128, 1024),
-                   smem_desc_sw128(sDS + kk * 2048, kKeys * 128, 1024), idesc_q, kk > 0 ? 1u : 0u);
-          mma_commit(smem_u32(&ctl.dq_full[g]));
+            mma_ss_warp(tmem + col_dp(g), step(dK, kk * 2048), step(dDSn, kk * 2048), idesc_q, kk > 0 ? 1u : 0u);
+          mma_commit_warp(smem_u32(&ctl.dq_full[g]));
         }
-        if (pend.kv_free >= 0) mma_commit(smem_u32(&ctl.kv_free[pend.kv_free]));
+        if (pend.kv_free >= 0) mma_commit_warp(smem_u32(&ctl.kv_free[pend.kv_free]));
         return true;
       };
       for (int j = 0; ok && j < n_items; ++j) {
         const int sl = j % kSlots;
-        if (!wait(ctl.item_full[sl], (j / kSlots) & 1)) {
+        if (!wait_all(ctl.item_full[sl], (j / kSlots) & 1)) {
           ok = false;
           break;
         }
@@ -584,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n > 0) {
           const int kv = li % C::kKVBufs;
           const uint32_t sK = base + C::kOffK + kv * C::kKVBytes, sV = base + C::kOffV + kv * C::kKVBytes;
-          if (!wait(ctl.kv_full[kv], (li / C::kKVBufs) & 1)) {
+          if (!wait_all(ctl.kv_full[kv], (li / C::kKVBufs) & 1)) {
             ok = false;
             break;
           }
@@ -597,29 +596,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // The step staged; the stage's columns free: its last P read by
             // the dV product (D = 64), and its dQ^T read out (D = 128).
-            if (!wait(ctl.ld_full[slot], (lt / kRing) & 1) ||
-                (use[g] > 0 && !wait(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use[g] - 1) & 1))) {
+            if (!wait_all(ctl.ld_full[slot], (lt / kRing) & 1) ||
+                (use[g] > 0 && !wait_all(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use[g] - 1) & 1))) {
               ok = false;
               break;
             }
-            tc_fence_after();
-            const uint32_t sQ = base + C::kOffQ + slot * C::kQBytes, sDO = base + C::kOffDO + slot * C::kQBytes;
+                const uint32_t sQ = base + C::kOffQ + slot * C::kQBytes, sDO = base + C::kOffDO + slot * C::kQBytes;
+            const uint64_t dK = smem_desc_sw128(sK, 16, 1024), dV = smem_desc_sw128(sV, 16, 1024);
+            const uint64_t dQ = smem_desc_sw128(sQ, 16, 1024), dDO = smem_desc_sw128(sDO, 16, 1024);
             // 16 head dims per instruction: swizzle chunk kk / 4 of the rows, 32 bytes into it.
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t ko = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32, qo = (kk >> 2) * (kQ * 128) + (kk & 3) * 32;
-              mma_ss(tmem + col_s(g), smem_desc_sw128(sK + ko, 16, 1024), smem_desc_sw128(sQ + qo, 16, 1024), idesc_s,
-                     kk > 0 ? 1u : 0u);
+              mma_ss_warp(tmem + col_s(g), step(dK, ko), step(dQ, qo), idesc_s, kk > 0 ? 1u : 0u);
             }
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t ko = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32, qo = (kk >> 2) * (kQ * 128) + (kk & 3) * 32;
-              mma_ss(tmem + col_dp(g), smem_desc_sw128(sV + ko, 16, 1024), smem_desc_sw128(sDO + qo, 16, 1024), idesc_s,
-                     kk > 0 ? 1u : 0u);
+              mma_ss_warp(tmem + col_dp(g), step(dV, ko), step(dDO, qo), idesc_s, kk > 0 ? 1u : 0u);
             }
             // st_full covers every earlier product, so the ones that last read
             // this step's dS slot have done so before it is rewritten.
-            mma_commit(smem_u32(&ctl.st_full[g]));
+            mma_commit_warp(smem_u32(&ctl.st_full[g]));
             if (!flush()) {
               ok = false;
               break;
@@ -642,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // needs nothing of this item.
           bool keep = false;
           if (C::kKVBufs == 2 && j + 1 < n_items) {
-            if (!wait(ctl.item_full[(j + 1) % kSlots], ((j + 1) / kSlots) & 1)) {
+            if (!wait_all(ctl.item_full[(j + 1) % kSlots], ((j + 1) / kSlots) & 1)) {
               ok = false;
               break;
             }
@@ -653,12 +651,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
         }
-        mbar_arrive(smem_u32(&ctl.item_free[sl]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.item_free[sl]));
       }
       if (ok && !flush()) ok = false;
-      if (!ok) fail();
+      if (!ok && lane == 0) fail();
       // Every MMA this thread issued must complete before TMEM is released.
-      mma_commit(smem_u32(&ctl.drain));
+      mma_commit_warp(smem_u32(&ctl.drain));
       uint32_t zero = 0;
       mbar_wait_bounded(smem_u32(&ctl.drain), 0, &zero, timeout_ns);
     }
