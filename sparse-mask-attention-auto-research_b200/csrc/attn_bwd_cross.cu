@@ -61,7 +61,13 @@ constexpr int kKeys = 128;  // keys of an item
 constexpr int kQ = 64;      // query rows of a step
 constexpr int kTmemCols = 512;
 constexpr int kEwWarps = 8, kLoaderWarp = 8, kMmaWarp = 9, kEpiWarp = 10, kScanWarp = 14;
-constexpr int kThreads = 15 * 32;
+constexpr int kThreads = 16 * 32;  // warp 15 only fills its warpgroup
+// Register split after start-up: the launch gives every thread 128; the two
+// warpgroups of loader, MMA, epilogue and scanner drop to 104 and the
+// element-wise ones rise to 152: 256 x (104 + 152) = 512 x 128.
+constexpr int kRegsOther = 104;
+constexpr int kRegsEw = 152;
+static_assert(256 * (kRegsOther + kRegsEw) <= kThreads * 128, "register split");
 // Items whose live lists the scanner publishes ahead, and words of a list: one
 // bit per step, up to 2048 steps of the heads that share a key head.
 constexpr int kSlots = 4;
@@ -93,7 +99,8 @@ struct Cfg {
   static constexpr int kOffDQ = kOffDS + kDSSlots * kDSBytes;  // 4 KiB box per epilogue warp
   static constexpr int kOffLse = kOffDQ + 4 * 4096;
   static constexpr int kOffDelta = kOffLse + kRing * kQ * 4;
-  static constexpr int kOffCtl = kOffDelta + kRing * kQ * 4;
+  static constexpr int kOffBias = kOffDelta + kRing * kQ * 4;  // [8 element-wise warps][96]
+  static constexpr int kOffCtl = kOffBias + kEwWarps * 96 * 4;
 };
 
 struct Ctl {
@@ -403,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kLoaderWarp) {
     // ================================================================ loader
+    regs_dec<kRegsOther>();
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
@@ -503,13 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ================================================================ MMA issuer
     // The whole warp walks along, converged; one elected lane issues.
+    regs_dec<kRegsOther>();
     bool ok = true;
     {
       constexpr int kBf = BF16 ? 1 : 0;
       constexpr uint32_t idesc_s = make_idesc_f16(kKeys, kQ, kBf, 0);                // S^T, dP^T
       constexpr uint32_t idesc_kv = make_idesc_f16(kKeys, D, kBf, 1);                // dV, dK (B M/N-major)
       constexpr uint32_t idesc_q = make_idesc_f16(128, 64, kBf, 1, 1);               // dQ, dQ^T (A and B M/N-major)
-      uint32_t lt = 0, lp = 0, use[2] = {0, 0};
+      uint32_t lt = 0, lp = 0, use0 = 0, use1 = 0;  // uses of the stages (no array: g is not known at compile time)
       int li = 0;
       // The step whose products are still to be issued.
       struct {
@@ -596,8 +605,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // The step staged; the stage's columns free: its last P read by
             // the dV product (D = 64), and its dQ^T read out (D = 128).
+            const uint32_t use = g ? use1 : use0;
             if (!wait_all(ctl.ld_full[slot], (lt / kRing) & 1) ||
-                (use[g] > 0 && !wait_all(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use[g] - 1) & 1))) {
+                (use > 0 && !wait_all(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use - 1) & 1))) {
               ok = false;
               break;
             }
@@ -630,8 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             pend.first = t == 0;
             pend.pair_end = g == 1 || t + 1 == n;
             pend.kv_free = t + 1 == n ? kv : -1;
-            pend.use = use[g];
-            ++use[g];
+            pend.use = use;
+            if (g) ++use1;
+            else ++use0;
           }
           if (!ok) break;
           ++li;
@@ -663,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kScanWarp) {
     // ================================================================ scanner
+    regs_dec<kRegsOther>();
     // Item j's live list: bit v set when some query row of step v keeps a key
     // of the item's tile.  A step's words of the tile are 1 KiB in a row, 32
     // bytes per lane; 8 steps per batch of loads.
@@ -718,12 +730,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) fail();
   } else if (warp < kEwWarps) {
     // ================================================================ element-wise
+    regs_inc<kRegsEw>();
     // Thread t = key t of the tile (TMEM lane); stage g = warp / 4.
     const int g = warp >> 2;
     const int t = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float c2 = scale * kLog2e;
     const uint64_t c2x2 = f2(c2, c2);
+    float* s_win = reinterpret_cast<float*>(smem + C::kOffBias) + warp * 96;  // kBias: bias by relative position
     bool ok = true;
     uint32_t lt0 = 0, lp0 = 0, use = 0;
     // Mask bits of this key for the 64 queries of the next step of this stage.
@@ -754,7 +768,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // kBias: this warp's 32-key block, and the bias gradient of blocks
       // beyond the last bucket's start, per head.
       int key0 = 0, off = 0, far_head = -1;
-      float far_lo = 0.f, far_hi = 0.f;
+      float far_lo = 0.f, far_hi = 0.f, add_lo = 0.f, add_hi = 0.f;
+      const float* head_row = nullptr;
       if constexpr (kBias) {
         key0 = it.kt * kKeys + (warp & 3) * 32;
         off = x.bias_offsets == nullptr
@@ -789,6 +804,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (head != far_head) {
             flush_far();
             far_head = head;
+            head_row = x.bias + static_cast<int64_t>(head) * x.bias_len;
+            add_lo = __ldg(head_row);
+            add_hi = __ldg(head_row + x.bias_len - 1);
+          }
+        }
+        // kBias: relative positions of the step's block c are d0 - 32 c + lane
+        // - e.  When it comes near the diagonal band, the 95 values of the
+        // step go to this warp's window: value of d at d - d0 + 64.
+        const int d0 = key0 - q0 - off;
+        bool step_near = false;
+        float win[3];
+        if constexpr (kBias) {
+          step_near = d0 + 31 > x.bias_lo && d0 - 63 < x.bias_hi;
+          if (step_near) {
+            const float* src = head_row + (d0 - x.bias_lo + kBiasPad + lane);
+#pragma unroll
+            for (int u = 0; u < 3; ++u) win[u] = __ldg(src + (u - 2) * 32);
           }
         }
         // The next step's words, a step ahead; at the last one those of the
@@ -816,25 +848,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                           (C::kPairDQ ? static_cast<int>((lp0 + (tt >> 1)) & 1) * 2 + g : g) * C::kDSBytes + t * 128;
         ok = wait_all(ctl.ld_full[b], (lt / kRing) & 1) && wait_all(ctl.st_full[g], use & 1);
         if (!ok) break;
+        if constexpr (kBias) {
+          if (step_near) {
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 3; ++u) s_win[32 * u + lane] = win[u];
+            __syncwarp();
+          }
+        }
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           const uint32_t word = c == 0 ? words.x : words.y;
           float s[32], dp[32];
           tmem_ld32f(t_lane + col_s(g) + c * 32, s);
           tmem_ld32f(t_lane + col_dp(g) + c * 32, dp);
-          // kBias: relative positions of the block are d0 + lane - e; the
-          // bias of a block beyond (bias_lo, bias_hi) is one value.
-          float badd = 0.f;
-          const float* brow = nullptr;
-          int d0 = 0;
-          bool near = false;
-          if constexpr (kBias) {
-            d0 = key0 - (q0 + c * 32) - off;
-            const float* head_row = x.bias + static_cast<int64_t>(head) * x.bias_len;
-            near = d0 + 31 > x.bias_lo && d0 - 31 < x.bias_hi;
-            brow = head_row + (near ? d0 - x.bias_lo + kBiasPad + lane : 0);
-            badd = near ? 0.f : __ldg(head_row + (d0 < x.bias_hi ? 0 : x.bias_len - 1));
-          }
+          // kBias: the bias of a block beyond (bias_lo, bias_hi) is one value.
+          const int dc = d0 - 32 * c;
+          const bool near = kBias && dc + 31 > x.bias_lo && dc - 31 < x.bias_hi;
+          const float badd = dc < x.bias_hi ? add_lo : add_hi;
+          const float* brow = s_win + 64 - 32 * c + lane;
           tmem_wait_ld();
           uint32_t pw[16], dw[16];
 #pragma unroll
@@ -845,8 +877,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint64_t l01 = f2(l4.x, l4.y), l23 = f2(l4.z, l4.w);
             if constexpr (kBias) {
               if (near) {
-                l01 = add2(l01, f2(__ldg(brow - e), __ldg(brow - e - 1)));
-                l23 = add2(l23, f2(__ldg(brow - e - 2), __ldg(brow - e - 3)));
+                l01 = add2(l01, f2(brow[-e], brow[-e - 1]));
+                l23 = add2(l23, f2(brow[-e - 2], brow[-e - 3]));
               } else {
                 l01 = add2(l01, f2(badd, badd));
                 l23 = add2(l23, f2(badd, badd));
@@ -893,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float sum = 0.f;
 #pragma unroll
               for (int e = 0; e < 32; ++e) sum += s[e];
-              if (d0 < x.bias_hi) far_lo += sum;
+              if (dc < x.bias_hi) far_lo += sum;
               else far_hi += sum;
             }
           }
@@ -910,15 +942,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       arrive_warp(ctl.item_free[sl]);
     }
     if (!ok && lane == 0) fail();
-  } else {
+  } else if (warp < kScanWarp) {
     // ================================================================ epilogue
+    regs_dec<kRegsOther>();
     const int w = (warp - kEpiWarp + 2) & 3;  // a warp reads the TMEM lanes of its index mod 4
     const int t = w * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(w * 32) << 16);
     uint8_t* s_dq = smem + C::kOffDQ + w * 4096;
     const int n_rows = x.hb * x.Nq;  // rows of the accumulator's block that holds a step
     bool ok = true;
-    uint32_t lp = 0, use[2] = {0, 0}, li = 0;
+    uint32_t lp = 0, use0 = 0, use1 = 0;
     // The staged box (32 rows of 32 columns) is added at (col, row0, block);
     // rows past the block are clipped by the TMA unit.
     auto add_box = [&](int col, int row0, int block) {
@@ -975,9 +1008,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tt = 0; tt < n; ++tt) {
           const int v = next_live(ctl.live_bits[sl], cw, cx);
           const int g = tt & 1;
-          ok = wait_all(ctl.dq_full[g], use[g] & 1);
+          ok = wait_all(ctl.dq_full[g], (g ? use1 : use0) & 1);
           if (!ok) break;
-          ++use[g];
+          if (g) ++use1;
+          else ++use0;
           float u[64];
           tmem_ld32f(t_lane + col_dp(g), u);
           tmem_ld32f(t_lane + col_dp(g) + 32, u + 32);
@@ -1027,15 +1061,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (n > 0) {
-        arrive_warp(ctl.acc_free);
-        ++li;
-      }
+      if (n > 0) arrive_warp(ctl.acc_free);
       arrive_warp(ctl.item_free[sl]);
     }
     // The reduce-adds must finish (and stop reading shared memory) before the CTA exits.
     if (lane == 0) bulk_wait_group0();
     if (!ok && lane == 0) fail();
+  } else {
+    regs_dec<kRegsOther>();
   }
 
   tc_fence_before();
