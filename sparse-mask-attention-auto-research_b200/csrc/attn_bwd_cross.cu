@@ -48,6 +48,7 @@
 // an error there shifts a whole row of dS.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "attn_math.cuh"
 #include "rel_bias.cuh"
@@ -135,6 +136,7 @@ struct BwdGeo {
   int B, H, Hkv, Nq, Nk;
   int tn, hb, gh, rows;    // rows = tn * hb; gh = G / hb
   int QT1;                 // 64-row steps of Nq
+  uint32_t qt_magic;       // v / QT1 = umulhi(v, qt_magic) for v < 2^16, or 0: QT1 = 1
   const uint32_t* words;   // packed mask rows (16-byte aligned), or nullptr: every key is kept
   int64_t word_stride[3];  // batch, head, query, in words (0: broadcast)
   int one_row;             // all query rows of an item have the same mask row
@@ -388,11 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     it.h0 = it.hkv * (x.gh * x.hb);
     return it;
   };
-  auto step_head = [&](int v) { return v / x.QT1 * x.hb; };  // relative to h0
-  auto step_q0 = [&](int v) { return v % x.QT1 * kQ; };
+  auto step_block = [&](int v) { return x.qt_magic != 0u ? static_cast<int>(__umulhi(v, x.qt_magic)) : v; };
+  auto step_head = [&](int v) { return step_block(v) * x.hb; };  // relative to h0
+  auto step_q0 = [&](int v) { return (v - step_block(v) * x.QT1) * kQ; };
   // The 128 words (by key) of step v of an item, where the mask is by key.
   auto step_words = [&](const Item& it, int v) {
-    const int ht = v / x.QT1;
+    const int ht = step_block(v);
     return x.words_t + it.b * x.t_stride[0] + (it.hkv * x.gh + ht) * x.t_stride[1] + (v - ht * x.QT1) * x.t_stride[2] +
            it.kt * kKeys;
   };
@@ -603,11 +606,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = false;
               break;
             }
+            const uint32_t use = g ? use1 : use0;
+            uint64_t& cols_free = C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g];
             // The step staged; the stage's columns free: its last P read by
             // the dV product (D = 64), and its dQ^T read out (D = 128).
-            const uint32_t use = g ? use1 : use0;
-            if (!wait_all(ctl.ld_full[slot], (lt / kRing) & 1) ||
-                (use > 0 && !wait_all(C::kPairDQ ? ctl.pt_free[g] : ctl.dq_free[g], (use - 1) & 1))) {
+            if (!wait_all(ctl.ld_full[slot], (lt / kRing) & 1) || (use > 0 && !wait_all(cols_free, (use - 1) & 1))) {
               ok = false;
               break;
             }
@@ -865,40 +868,49 @@ __global__ void __launch_bounds__(kThreads, 1)
           // kBias: the bias of a block beyond (bias_lo, bias_hi) is one value.
           const int dc = d0 - 32 * c;
           const bool near = kBias && dc + 31 > x.bias_lo && dc - 31 < x.bias_hi;
-          const float badd = dc < x.bias_hi ? add_lo : add_hi;
-          const float* brow = s_win + 64 - 32 * c + lane;
           tmem_wait_ld();
           uint32_t pw[16], dw[16];
+          // P and dS of the block; kB: 0 no bias, 1 one value, 2 the window's.
+          // (Told apart outside the loop, which schedules as one block then.)
+          auto block = [&](auto kind) {
+            constexpr int kB = decltype(kind)::value;
+            const uint64_t badd = f2(dc < x.bias_hi ? add_lo : add_hi, dc < x.bias_hi ? add_lo : add_hi);
+            const float* brow = s_win + 64 - 32 * c + lane;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 l4 = *reinterpret_cast<const float4*>(t_lse + c * 32 + e);
-            const float4 d4 = *reinterpret_cast<const float4*>(t_delta + c * 32 + e);
-            // y = s * scale * log2(e) + bias - lse2 and ds = p * (dp - Delta), two queries per instruction.
-            uint64_t l01 = f2(l4.x, l4.y), l23 = f2(l4.z, l4.w);
-            if constexpr (kBias) {
-              if (near) {
+            for (int e = 0; e < 32; e += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(t_lse + c * 32 + e);
+              const float4 d4 = *reinterpret_cast<const float4*>(t_delta + c * 32 + e);
+              // y = s * scale * log2(e) + bias - lse2 and ds = p * (dp - Delta), two queries per instruction.
+              uint64_t l01 = f2(l4.x, l4.y), l23 = f2(l4.z, l4.w);
+              if constexpr (kB == 1) {
+                l01 = add2(l01, badd);
+                l23 = add2(l23, badd);
+              } else if constexpr (kB == 2) {
                 l01 = add2(l01, f2(brow[-e], brow[-e - 1]));
                 l23 = add2(l23, f2(brow[-e - 2], brow[-e - 3]));
-              } else {
-                l01 = add2(l01, f2(badd, badd));
-                l23 = add2(l23, f2(badd, badd));
+              }
+              float y[4], p[4], ds[4];
+              f2_split(fma2(f2(s[e], s[e + 1]), c2x2, l01), y[0], y[1]);
+              f2_split(fma2(f2(s[e + 2], s[e + 3]), c2x2, l23), y[2], y[3]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) p[u] = (word & (1u << (e + u))) ? ex2f(y[u]) : 0.f;
+              f2_split(mul2(f2(p[0], p[1]), add2(f2(dp[e], dp[e + 1]), f2(d4.x, d4.y))), ds[0], ds[1]);
+              f2_split(mul2(f2(p[2], p[3]), add2(f2(dp[e + 2], dp[e + 3]), f2(d4.z, d4.w))), ds[2], ds[3]);
+              pw[e / 2] = pack2<BF16>(p[0], p[1]);
+              pw[e / 2 + 1] = pack2<BF16>(p[2], p[3]);
+              dw[e / 2] = pack2<BF16>(ds[0], ds[1]);
+              dw[e / 2 + 1] = pack2<BF16>(ds[2], ds[3]);
+              if constexpr (kB != 0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[e + u] = ds[u];  // the scores are used up
               }
             }
-            float y[4], p[4], ds[4];
-            f2_split(fma2(f2(s[e], s[e + 1]), c2x2, l01), y[0], y[1]);
-            f2_split(fma2(f2(s[e + 2], s[e + 3]), c2x2, l23), y[2], y[3]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = (word & (1u << (e + u))) ? ex2f(y[u]) : 0.f;
-            f2_split(mul2(f2(p[0], p[1]), add2(f2(dp[e], dp[e + 1]), f2(d4.x, d4.y))), ds[0], ds[1]);
-            f2_split(mul2(f2(p[2], p[3]), add2(f2(dp[e + 2], dp[e + 3]), f2(d4.z, d4.w))), ds[2], ds[3]);
-            pw[e / 2] = pack2<BF16>(p[0], p[1]);
-            pw[e / 2 + 1] = pack2<BF16>(p[2], p[3]);
-            dw[e / 2] = pack2<BF16>(ds[0], ds[1]);
-            dw[e / 2 + 1] = pack2<BF16>(ds[2], ds[3]);
-            if constexpr (kBias) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) s[e + u] = ds[u];  // the scores are used up
-            }
+          };
+          if constexpr (kBias) {
+            if (near) block(std::integral_constant<int, 2>{});
+            else block(std::integral_constant<int, 1>{});
+          } else {
+            block(std::integral_constant<int, 0>{});
           }
           // P over S^T columns this warp has read (chunk c writes 16 c ..,
           // which chunks <= c have read).
@@ -922,11 +934,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dst[32 + lane] = neg;
               }
             } else {
-              float sum = 0.f;
+              uint64_t sum[4];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) sum += s[e];
-              if (dc < x.bias_hi) far_lo += sum;
-              else far_hi += sum;
+              for (int e = 0; e < 4; ++e) sum[e] = f2(s[2 * e], s[2 * e + 1]);
+#pragma unroll
+              for (int e = 4; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], f2(s[2 * e], s[2 * e + 1]));
+              float a, b2;
+              f2_split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b2);
+              if (dc < x.bias_hi) far_lo += a + b2;
+              else far_hi += a + b2;
             }
           }
         }
@@ -1000,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<float4*>(s_dq + lane * 128 + ((c ^ (lane & 7)) * 16)) =
                   make_float4(y[0] * scale, y[1] * scale, y[2] * scale, y[3] * scale);
             }
-            add_box(32 * h, row0, block0 + v / x.QT1);
+            add_box(32 * h, row0, block0 + step_block(v));
           }
         }
       } else {
@@ -1025,43 +1041,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 32; ++q)
               *reinterpret_cast<float*>(s_dq + q * 128 + (((lane >> 2) ^ (q & 7)) * 16) + (lane & 3) * 4) =
                   u[32 * h + q] * scale;
-            add_box(32 * w, row0 + 32 * h, block0 + v / x.QT1);
+            add_box(32 * w, row0 + 32 * h, block0 + step_block(v));
           }
         }
       }
       if (!ok) break;
       // dV and dK of this key tile (lane t = key); zero when no step was live.
       // The dq_full wait of the item's last step covered all of its products.
+      // D = 64 reads both out before it stores, so that the next item's first
+      // products wait no longer than that; D = 128 has no registers for it.
       const int key = it.kt * kKeys + t;
-#pragma unroll 1
-      for (int h = 0; h < D / 32; ++h) {
-        uint32_t vw[16], kw[16];
+      const int64_t at = ((static_cast<int64_t>(it.b) * x.Hkv + it.hkv) * x.Nk + key) * D;
+      auto read_acc = [&](uint32_t col, float mul, uint32_t (&w)[16]) {
+        float u[32];
+        tmem_ld32f(t_lane + col, u);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(u[2 * e] * mul, u[2 * e + 1] * mul);
+      };
+      auto store_row = [&](uint16_t* dst, const uint32_t (&w)[16]) {
+        if (key >= x.Nk) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      };
+      if constexpr (D == 64) {
+        uint32_t w[4][16] = {};
         if (n > 0) {
-          float u[32];
-          tmem_ld32f(t_lane + kColDV + h * 32, u);
-          tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) vw[e] = pack2<BF16>(u[2 * e], u[2 * e + 1]);
-          tmem_ld32f(t_lane + C::kColDK + h * 32, u);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) kw[e] = pack2<BF16>(u[2 * e] * scale, u[2 * e + 1] * scale);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) vw[e] = kw[e] = 0u;
-        }
-        if (key < x.Nk) {
-          const int64_t at = ((static_cast<int64_t>(it.b) * x.Hkv + it.hkv) * x.Nk + key) * D + h * 32;
-          uint4* dvr = reinterpret_cast<uint4*>(dv + at);
-          uint4* dkr = reinterpret_cast<uint4*>(dk + at);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            dvr[q] = make_uint4(vw[4 * q], vw[4 * q + 1], vw[4 * q + 2], vw[4 * q + 3]);
-            dkr[q] = make_uint4(kw[4 * q], kw[4 * q + 1], kw[4 * q + 2], kw[4 * q + 3]);
+          for (int h = 0; h < 2; ++h) {
+            read_acc(kColDV + h * 32, 1.f, w[h]);
+            read_acc(C::kColDK + h * 32, scale, w[2 + h]);
           }
+          arrive_warp(ctl.acc_free);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          store_row(dv + at + h * 32, w[h]);
+          store_row(dk + at + h * 32, w[2 + h]);
+        }
+      } else {
+#pragma unroll 1
+        for (int h = 0; h < D / 32; ++h) {
+          uint32_t vw[16] = {}, kw[16] = {};
+          if (n > 0) {
+            read_acc(kColDV + h * 32, 1.f, vw);
+            read_acc(C::kColDK + h * 32, scale, kw);
+          }
+          store_row(dv + at + h * 32, vw);
+          store_row(dk + at + h * 32, kw);
+        }
+        if (n > 0) arrive_warp(ctl.acc_free);
       }
-      if (n > 0) arrive_warp(ctl.acc_free);
       arrive_warp(ctl.item_free[sl]);
     }
     // The reduce-adds must finish (and stop reading shared memory) before the CTA exits.
@@ -1169,6 +1200,9 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
   x->gh = G / x->hb;
   x->rows = x->tn * x->hb;
   x->QT1 = (x->Nq + kQ - 1) / kQ;
+  // ceil(2^32 / QT1): exact for v < 2^16, as v * (the rounding of it, below
+  // QT1 / 2^32 relative) stays below 1 / QT1 for QT1 <= 2^16.
+  x->qt_magic = x->QT1 > 1 ? static_cast<uint32_t>((uint64_t{0xFFFFFFFF} + x->QT1) / x->QT1) : 0u;
   x->words = p.words;
   for (int i = 0; i < 3; ++i) x->word_stride[i] = p.word_stride[i];
   x->one_row = p.words != nullptr && (x->Nq == 1 || p.word_stride[2] == 0) && (G == 1 || p.word_stride[1] == 0);
