@@ -64,10 +64,10 @@ constexpr int kTmemCols = 512;
 constexpr int kEwWarps = 8, kLoaderWarp = 8, kMmaWarp = 9, kEpiWarp = 10, kScanWarp = 14;
 constexpr int kThreads = 16 * 32;  // warp 15 only fills its warpgroup
 // Register split after start-up: the launch gives every thread 128; the two
-// warpgroups of loader, MMA, epilogue and scanner drop to 104 and the
-// element-wise ones rise to 152: 256 x (104 + 152) = 512 x 128.
-constexpr int kRegsOther = 104;
-constexpr int kRegsEw = 152;
+// warpgroups of loader, MMA, epilogue and scanner drop to 112 and the
+// element-wise ones rise to 144: 256 x (112 + 144) = 512 x 128.
+constexpr int kRegsOther = 112;
+constexpr int kRegsEw = 144;
 static_assert(256 * (kRegsOther + kRegsEw) <= kThreads * 128, "register split");
 // Items whose live lists the scanner publishes ahead, and words of a list: one
 // bit per step, up to 2048 steps of the heads that share a key head.
@@ -144,6 +144,9 @@ struct BwdGeo {
   // rows, strides in such words for batch, head block (ht) and 64-query step.
   const uint2* words_t;
   int64_t t_stride[3];
+  // And which 32-key words of a step keep a pair: 4 bytes (0 / 1) per key tile,
+  // strides t_stride / 128 per tile.
+  const uint32_t* live_t;
   // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
   const float* bias;
   const int32_t* bias_offsets;
@@ -190,12 +193,13 @@ __device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
 }
 
 // words (rows of queries) -> words_t (BwdGeo): one warp per (batch, head block,
-// step, 32 keys), its 64 rows' words transposed.  Bound by reading and writing
+// step, 32 keys), its 64 rows' words transposed, and whether they keep any
+// pair (live_t, so that the scanner reads 4 bytes per step).  Bound by reading and writing
 // the packed mask once, mostly in L2.
 constexpr int kTransposeWarps = 8;
 __global__ void __launch_bounds__(kTransposeWarps * 32)
-    transpose_words_kernel(const __grid_constant__ BwdGeo x, uint2* __restrict__ out, int Bm, int Hm, int key_words,
-                           int64_t total) {
+    transpose_words_kernel(const __grid_constant__ BwdGeo x, uint2* __restrict__ out, uint8_t* __restrict__ live, int Bm,
+                           int Hm, int key_words, int64_t total) {
   pdl_launch_dependents();
   pdl_wait_prior_grid();
   const int lane = threadIdx.x & 31;
@@ -219,6 +223,8 @@ __global__ void __launch_bounds__(kTransposeWarps * 32)
     v[u] = transpose_bits(v[u], lane);
   }
   out[w * 32 + lane] = make_uint2(v[0], v[1]);
+  const bool any = __any_sync(0xffffffffu, (v[0] | v[1]) != 0u);
+  if (lane == 0) live[w] = any ? 1 : 0;
 }
 
 // Per row: -Delta, Delta = sum_d dO[row, d] * (O[row, d] + its rounding
@@ -679,8 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ================================================================ scanner
     regs_dec<kRegsOther>();
     // Item j's live list: bit v set when some query row of step v keeps a key
-    // of the item's tile.  A step's words of the tile are 1 KiB in a row, 32
-    // bytes per lane; 8 steps per batch of loads.
+    // of the item's tile; a lane looks at one step of 32.
     bool ok = true;
     for (int j = 0; j < n_items; ++j) {
       const int sl = j % kSlots;
@@ -703,22 +708,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           mine[1] = low_bits(VT - 32 * (lane + 32));
         }
       } else {
-        for (int v0 = 0; v0 < VT; v0 += 8) {
-          uint4 m[8][2];
+        for (int v0 = 0; v0 < VT; v0 += 128) {
+          uint32_t f[4];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const uint4* src = reinterpret_cast<const uint4*>(step_words(it, min(v0 + u, VT - 1))) + lane * 2;
-            m[u][0] = __ldg(src);
-            m[u][1] = __ldg(src + 1);
+          for (int u = 0; u < 4; ++u) {
+            const int v = v0 + 32 * u + lane;
+            const int64_t tile = (step_words(it, min(v, VT - 1)) - x.words_t) / kKeys;
+            f[u] = v < VT ? __ldg(x.live_t + tile) : 0u;
           }
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int v = v0 + u;
-            const uint32_t o = m[u][0].x | m[u][0].y | m[u][0].z | m[u][0].w | m[u][1].x | m[u][1].y | m[u][1].z | m[u][1].w;
-            const bool any = __any_sync(0xffffffffu, o != 0u) && v < VT;
-            if (any && lane == ((v >> 5) & 31)) {
-              if (v < 1024) mine[0] |= 1u << (v & 31);
-              else mine[1] |= 1u << (v & 31);
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t bits = __ballot_sync(0xffffffffu, f[u] != 0u);
+            const int w = (v0 >> 5) + u;
+            if (lane == (w & 31)) {
+              if (w < 32) mine[0] = bits;
+              else mine[1] = bits;
             }
           }
         }
@@ -989,6 +993,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at(j);
       const int block0 = (it.b * x.Hkv + it.hkv) * x.gh;
       const int n = static_cast<int>(ctl.n_live[sl]);
+      // dV and dK of this key tile (lane t = key), once the item's last products
+      // are complete, which the dq_full wait of its last step covers: ahead of
+      // that step's dQ, since the next item's first products wait for it.  Zero
+      // when no step was live.
+      auto write_acc = [&]() {
+        // D = 64 reads both out before it stores, so that the next item's first
+        // products wait no longer than that; D = 128 has no registers for it.
+        const int key = it.kt * kKeys + t;
+        const int64_t at = ((static_cast<int64_t>(it.b) * x.Hkv + it.hkv) * x.Nk + key) * D;
+        auto read_acc = [&](uint32_t col, float mul, uint32_t (&w)[16]) {
+          float u[32];
+          tmem_ld32f(t_lane + col, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(u[2 * e] * mul, u[2 * e + 1] * mul);
+        };
+        auto store_row = [&](uint16_t* dst, const uint32_t (&w)[16]) {
+          if (key >= x.Nk) return;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        };
+        if constexpr (D == 64) {
+          uint32_t w[4][16] = {};
+          if (n > 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              read_acc(kColDV + h * 32, 1.f, w[h]);
+              read_acc(C::kColDK + h * 32, scale, w[2 + h]);
+            }
+            arrive_warp(ctl.acc_free);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            store_row(dv + at + h * 32, w[h]);
+            store_row(dk + at + h * 32, w[2 + h]);
+          }
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < D / 32; ++h) {
+            uint32_t vw[16] = {}, kw[16] = {};
+            if (n > 0) {
+              read_acc(kColDV + h * 32, 1.f, vw);
+              read_acc(C::kColDK + h * 32, scale, kw);
+            }
+            store_row(dv + at + h * 32, vw);
+            store_row(dk + at + h * 32, kw);
+          }
+          if (n > 0) arrive_warp(ctl.acc_free);
+        }
+      };
+      if (n == 0) write_acc();
       int cw = 0;
       uint32_t cx = ctl.live_bits[sl][0];
       if constexpr (C::kPairDQ) {
@@ -999,6 +1055,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int b = lp & 1;
           ok = wait_all(ctl.dq_full[b], (lp >> 1) & 1);
           if (!ok) break;
+          if (tt + 2 >= n) write_acc();
           float u[64];
           tmem_ld32f(t_lane + C::col_dq(b), u);
           tmem_ld32f(t_lane + C::col_dq(b) + 32, u + 32);
@@ -1028,6 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if (g) ++use1;
           else ++use0;
+          if (tt + 1 == n) write_acc();
           float u[64];
           tmem_ld32f(t_lane + col_dp(g), u);
           tmem_ld32f(t_lane + col_dp(g) + 32, u + 32);
@@ -1046,53 +1104,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
-      // dV and dK of this key tile (lane t = key); zero when no step was live.
-      // The dq_full wait of the item's last step covered all of its products.
-      // D = 64 reads both out before it stores, so that the next item's first
-      // products wait no longer than that; D = 128 has no registers for it.
-      const int key = it.kt * kKeys + t;
-      const int64_t at = ((static_cast<int64_t>(it.b) * x.Hkv + it.hkv) * x.Nk + key) * D;
-      auto read_acc = [&](uint32_t col, float mul, uint32_t (&w)[16]) {
-        float u[32];
-        tmem_ld32f(t_lane + col, u);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(u[2 * e] * mul, u[2 * e + 1] * mul);
-      };
-      auto store_row = [&](uint16_t* dst, const uint32_t (&w)[16]) {
-        if (key >= x.Nk) return;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-      };
-      if constexpr (D == 64) {
-        uint32_t w[4][16] = {};
-        if (n > 0) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            read_acc(kColDV + h * 32, 1.f, w[h]);
-            read_acc(C::kColDK + h * 32, scale, w[2 + h]);
-          }
-          arrive_warp(ctl.acc_free);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          store_row(dv + at + h * 32, w[h]);
-          store_row(dk + at + h * 32, w[2 + h]);
-        }
-      } else {
-#pragma unroll 1
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t vw[16] = {}, kw[16] = {};
-          if (n > 0) {
-            read_acc(kColDV + h * 32, 1.f, vw);
-            read_acc(C::kColDK + h * 32, scale, kw);
-          }
-          store_row(dv + at + h * 32, vw);
-          store_row(dk + at + h * 32, kw);
-        }
-        if (n > 0) arrive_warp(ctl.acc_free);
-      }
       arrive_warp(ctl.item_free[sl]);
     }
     // The reduce-adds must finish (and stop reading shared memory) before the CTA exits.
@@ -1229,9 +1240,10 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
 }
 
 // Offsets, in floats, within the scratch of a backward: the FP32 accumulator of
-// dq at 0, -Delta and -lse2, the mask by key, partial sums of the bias gradient.
+// dq at 0, -Delta and -lse2, the mask by key and its live bytes, partial sums of
+// the bias gradient.
 struct Scratch {
-  int64_t delta, words, bias, end;
+  int64_t delta, words, live, bias, end;
 };
 Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
@@ -1240,7 +1252,9 @@ Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
   s.delta = rows * p.D;
   s.words = s.delta + up(2 * rows);
   const int64_t Bm = p.word_stride[0] != 0 ? p.B : 1, Hm = p.word_stride[1] != 0 ? p.H / x.hb : 1;
-  s.bias = s.words + 2 * Bm * Hm * x.QT1 * x.t_stride[2];
+  const int64_t masked = Bm * Hm * x.QT1 * x.t_stride[2];  // 0 where the mask is not by key
+  s.live = s.words + 2 * masked;
+  s.bias = s.live + up(masked / kKeys);
   s.end = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0);
   return s;
 }
@@ -1290,9 +1304,11 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
     const int key_words = static_cast<int>(KT * 4);
     const int64_t total = static_cast<int64_t>(Bm) * Hm * x.QT1 * key_words;
     uint2* words_t = reinterpret_cast<uint2*>(g.scratch + at.words);
+    uint8_t* live = reinterpret_cast<uint8_t*>(g.scratch + at.live);
     e = launch_pdl(transpose_words_kernel, static_cast<unsigned>((total + kTransposeWarps - 1) / kTransposeWarps),
-                   kTransposeWarps * 32, 0, p.stream, x, words_t, Bm, Hm, key_words, total);
+                   kTransposeWarps * 32, 0, p.stream, x, words_t, live, Bm, Hm, key_words, total);
     x.words_t = words_t;
+    x.live_t = reinterpret_cast<const uint32_t*>(live);
   }
   if (e == cudaSuccess)
     e = launch_pdl(cross_delta_kernel<D, BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
