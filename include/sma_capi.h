@@ -224,7 +224,8 @@ typedef struct sma_attn_args {
   float* lse;  /* [B, H, Nq] natural-log sum of exponentials, or NULL */
   /* Of the 128-row tile entries: room for the packed mask, int32 words
    * [B, H, Nq, 4 * ceil(Nk / 128)] with length 1 for an axis whose mask_stride
-   * is 0 (bit b of word w: column 32 w + b, 0 past Nk). */
+   * is 0 (bit b of word w: column 32 w + b, 0 past Nk), and for the live key
+   * tiles behind it, [B, H, ceil(Nq / 128), ceil(Nk / 2048)] more words. */
   void* words;
   float* bias_distance; /* room for H * SMA_BIAS_DISTANCE_LEN floats */
   void* out_lo;         /* O minus its rounded value, like out, or NULL */

@@ -6,10 +6,10 @@
 //   dV = P^T dO,  dS = P * (dO V^T - Delta),  Delta_i = sum_d dO_id O_id
 //   dQ = scale * dS K,  dK = scale * dS^T Q,  dtable[bucket, h] = sum of dS over the bucket's pairs
 //
-// Kernels, in stream order: transpose_words_kernel (the packed mask by key,
-// where query rows have masks of their own), cross_delta_kernel (Delta, and
-// clears the FP32 dQ accumulator), cross_bwd_kernel, cross_dq_kernel
-// (accumulator -> dq) and, with a bias, bias_reduce_kernel.
+// Kernels, in stream order: cross_prepare_kernel (Delta, zeros in the FP32 dQ
+// accumulator, and the packed mask by key, where query rows have masks of
+// their own), cross_bwd_kernel, cross_dq_kernel (accumulator -> dq) and, with a
+// bias, bias_reduce_kernel.
 //
 // cross_bwd_kernel is persistent, one CTA per SM, over items (batch, key head,
 // 128-key tile).  K and V of the item stay in shared memory, dK and dV
@@ -194,24 +194,22 @@ __device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
 
 // words (rows of queries) -> words_t (BwdGeo): one warp per (batch, head block,
 // step, 32 keys), its 64 rows' words transposed, and whether they keep any
-// pair (live_t, so that the scanner reads 4 bytes per step).  Bound by reading and writing
-// the packed mask once, mostly in L2.
-constexpr int kTransposeWarps = 8;
-__global__ void __launch_bounds__(kTransposeWarps * 32)
-    transpose_words_kernel(const __grid_constant__ BwdGeo x, uint2* __restrict__ out, uint8_t* __restrict__ live, int Bm,
-                           int Hm, int key_words, int64_t total) {
-  pdl_launch_dependents();
-  pdl_wait_prior_grid();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kTransposeWarps + (threadIdx.x >> 5);
-  if (w >= total) return;
+// pair (live_t, so that the scanner reads 4 bytes per step).
+struct Transpose {
+  uint2* out;
+  uint8_t* live;
+  int Hm, key_words;
+  int64_t total;  // warps; 0: nothing to do
+};
+__device__ __forceinline__ void transpose_words(const BwdGeo& x, const Transpose& tr, int64_t w, int lane) {
+  if (w >= tr.total) return;
   // [Bm][Hm head blocks][QT1][key_words]
-  const int kw = static_cast<int>(w % key_words);
-  int64_t rest = w / key_words;
+  const int kw = static_cast<int>(w % tr.key_words);
+  int64_t rest = w / tr.key_words;
   const int qt = static_cast<int>(rest % x.QT1);
   rest /= x.QT1;
-  const int hm = static_cast<int>(rest % Hm);
-  const int64_t b = rest / Hm;
+  const int hm = static_cast<int>(rest % tr.Hm);
+  const int64_t b = rest / tr.Hm;
   uint32_t v[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -222,24 +220,44 @@ __global__ void __launch_bounds__(kTransposeWarps * 32)
                : 0u;
     v[u] = transpose_bits(v[u], lane);
   }
-  out[w * 32 + lane] = make_uint2(v[0], v[1]);
+  tr.out[w * 32 + lane] = make_uint2(v[0], v[1]);
   const bool any = __any_sync(0xffffffffu, (v[0] | v[1]) != 0u);
-  if (lane == 0) live[w] = any ? 1 : 0;
+  if (lane == 0) tr.live[w] = any ? 1 : 0;
 }
 
-// Per row: -Delta, Delta = sum_d dO[row, d] * (O[row, d] + its rounding
-// residual) in FP32, and -lse * log2(e) (negated, so that the element-wise
-// pass adds them in packed pairs); D/8 threads per row, each of which also
-// clears its 8 elements of the FP32 dQ accumulator.  Bound by HBM: three
-// 16-bit reads and a 32-bit write per element.
+constexpr int kZeroRounds = 4;
+
+// What the backward needs before it starts, in one launch.  Blocks below
+// `delta_blocks`, D/8 threads per row: -Delta, Delta = sum_d dO[row, d] *
+// (O[row, d] + its rounding residual) in FP32, and -lse * log2(e) (negated, so
+// that the element-wise pass adds them in packed pairs), and zeros in the FP32
+// dQ accumulator.  The next `zero_blocks`: zeros in the bias gradient's partial
+// sums (blocks that no live step visits count as 0).  The others: the mask by
+// key, a warp each.  Bound by HBM:
+// three 16-bit reads and a 32-bit write per element, and the packed mask once
+// in and out.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256)
-    cross_delta_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ out, const uint4* __restrict__ out_lo,
-                       const float* __restrict__ lse, float* __restrict__ neg_delta, float* __restrict__ neg_lse2,
-                       float4* __restrict__ dq_acc, int64_t rows) {
+    cross_prepare_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ out, const uint4* __restrict__ out_lo,
+                         const float* __restrict__ lse, float* __restrict__ neg_delta, float* __restrict__ neg_lse2,
+                         float4* __restrict__ dq_acc, int64_t rows, unsigned delta_blocks, float4* __restrict__ zero,
+                         int64_t zeros, unsigned zero_blocks, const __grid_constant__ Transpose tr, const __grid_constant__ BwdGeo x) {
   constexpr int kPerRow = D / 8;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
+  if (blockIdx.x >= delta_blocks + zero_blocks) {
+    transpose_words(x, tr, static_cast<int64_t>(blockIdx.x - delta_blocks - zero_blocks) * 8 + (threadIdx.x >> 5),
+                    threadIdx.x & 31);
+    return;
+  }
+  if (blockIdx.x >= delta_blocks) {
+#pragma unroll
+    for (int u = 0; u < kZeroRounds; ++u) {
+      const int64_t i = (static_cast<int64_t>(blockIdx.x - delta_blocks) * kZeroRounds + u) * 256 + threadIdx.x;
+      if (i < zeros) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = gid / kPerRow;
   float acc = 0.f;
@@ -251,9 +269,9 @@ __global__ void __launch_bounds__(256)
     const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 x = unpack2<BF16>(aw[e]), y = unpack2<BF16>(bw[e]), z = unpack2<BF16>(cw[e]);
-      acc = fmaf(x.x, y.x + z.x, acc);
-      acc = fmaf(x.y, y.y + z.y, acc);
+      const float2 x2 = unpack2<BF16>(aw[e]), y = unpack2<BF16>(bw[e]), z = unpack2<BF16>(cw[e]);
+      acc = fmaf(x2.x, y.x + z.x, acc);
+      acc = fmaf(x2.y, y.y + z.y, acc);
     }
   }
 #pragma unroll
@@ -1148,35 +1166,44 @@ __global__ void __launch_bounds__(kReduceThreads)
     d_hi = first == 0 && !s.two_sided ? kFar : -first;
   }
   float acc = 0.f;
-  for (int b = 0; b < x.B; ++b) {
+  // A warp per batch and stretch of key blocks, so that their loads overlap.
+  constexpr int kWarps = kReduceThreads / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int parts = x.B < kWarps ? (kWarps + x.B - 1) / x.B : 1;
+  for (int unit = warp; unit < x.B * parts; unit += kWarps) {
+    const int b = unit / parts, part = unit - b * parts;
+    const int kb0 = x.KB * part / parts, kb1 = x.KB * (part + 1) / parts;
     const int off = x.bias_offsets == nullptr
                         ? x.bias_offset
                         : max(-kMaxBiasOffset, min(kMaxBiasOffset, __ldg(x.bias_offsets + b)));
     const int j_max = bias_block_max(x.bias_hi, off);
     const int j_min = -bias_block_max(-x.bias_lo, -off);
     const int lo = max(d_lo, 32 * j_min - off - 31), hi = min(d_hi, 32 * j_max - off + 31);
-    const int64_t n = hi >= lo ? static_cast<int64_t>(hi - lo + 1) * x.KB : 0;
+    const int64_t n = hi >= lo ? static_cast<int64_t>(hi - lo + 1) * (kb1 - kb0) : 0;
     const float* near_bh = x.near_part + (static_cast<int64_t>(b) * x.H + h) * x.KB * x.slots * 64;
-    for (int64_t w = threadIdx.x; w < n; w += kReduceThreads) {
-      const int kb = static_cast<int>(w / (hi - lo + 1));
-      const int d = lo + static_cast<int>(w - static_cast<int64_t>(kb) * (hi - lo + 1));
+#pragma unroll 4
+    for (int64_t w = lane; w < n; w += 32) {
+      const int di = static_cast<int>(w / (kb1 - kb0));
+      const int kb = kb0 + static_cast<int>(w - static_cast<int64_t>(di) * (kb1 - kb0));
       // d = 32 j - off + k: k in [0, 31] of block j, or k - 32 of block j + 1.
-      const int y = d + off;
+      const int y = lo + di + off;
       const int j = y >= 0 ? y / 32 : -((-y + 31) / 32);
       const int k = y - 32 * j;
+      float v[2] = {0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int jj = j + u, qb = kb - jj;
-        if (jj < j_min || jj > j_max || qb < 0 || qb >= x.QB || (u == 1 && k == 0)) continue;
         const int slot = x.slot_by_query ? qb : j_max - jj;
-        acc += __ldg(near_bh + (static_cast<int64_t>(kb) * x.slots + slot) * 64 + (u == 0 ? k : k + 32));
+        if (jj >= j_min && jj <= j_max && qb >= 0 && qb < x.QB && (u == 0 || k != 0))
+          v[u] = __ldg(near_bh + (static_cast<int64_t>(kb) * x.slots + slot) * 64 + (u == 0 ? k : k + 32));
       }
+      acc += v[0] + v[1];
     }
     const bool low_end = !high && i == s.side - 1;
     const bool high_end = s.two_sided ? high && i == s.side - 1 : i == 0;
     if (low_end || high_end) {
       const float* far_bh = x.far_part + (static_cast<int64_t>(b) * x.H + h) * x.KB * 4;
-      for (int w = threadIdx.x; w < 2 * x.KB; w += kReduceThreads) {
+      for (int w = 2 * kb0 + lane; w < 2 * kb1; w += 32) {
         if (low_end) acc += __ldg(far_bh + 2 * w);
         if (high_end) acc += __ldg(far_bh + 2 * w + 1);
       }
@@ -1255,7 +1282,7 @@ Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
   const int64_t masked = Bm * Hm * x.QT1 * x.t_stride[2];  // 0 where the mask is not by key
   s.live = s.words + 2 * masked;
   s.bias = s.live + up(masked / kKeys);
-  s.end = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0);
+  s.end = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0);  // a multiple of 4
   return s;
 }
 
@@ -1289,31 +1316,35 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
   static std::atomic<bool> smem_set[kMaxDevices] = {};
   auto kern = cross_bwd_kernel<D, BF16, kBias>;
   cudaError_t e = ensure_smem_limit(kern, kSmemBytes, dp.device, smem_set);
-  if (e == cudaSuccess && kBias) {
-    // Blocks that no live step visits count as 0.
-    const Scratch s = scratch_layout(p, x);
-    x.near_part = g.scratch + s.bias;
-    x.far_part = x.near_part + p.B * p.H * x.KB * x.slots * 64;
-    e = cudaMemsetAsync(x.near_part, 0, static_cast<size_t>(s.end - s.bias) * sizeof(float), p.stream);
-  }
   const Scratch at = scratch_layout(p, x);
   float* neg_delta = g.scratch + at.delta;
   float4* dq_accum = reinterpret_cast<float4*>(g.scratch);
-  if (e == cudaSuccess && x.t_stride[2] != 0) {
-    const int Bm = p.word_stride[0] != 0 ? x.B : 1, Hm = p.word_stride[1] != 0 ? x.H / x.hb : 1;
-    const int key_words = static_cast<int>(KT * 4);
-    const int64_t total = static_cast<int64_t>(Bm) * Hm * x.QT1 * key_words;
-    uint2* words_t = reinterpret_cast<uint2*>(g.scratch + at.words);
-    uint8_t* live = reinterpret_cast<uint8_t*>(g.scratch + at.live);
-    e = launch_pdl(transpose_words_kernel, static_cast<unsigned>((total + kTransposeWarps - 1) / kTransposeWarps),
-                   kTransposeWarps * 32, 0, p.stream, x, words_t, live, Bm, Hm, key_words, total);
-    x.words_t = words_t;
-    x.live_t = reinterpret_cast<const uint32_t*>(live);
+  if (kBias) {
+    x.near_part = g.scratch + at.bias;
+    x.far_part = x.near_part + p.B * p.H * x.KB * x.slots * 64;
+  }
+  const int64_t zeros = (at.end - at.bias) / 4;
+  const int64_t zero_blocks = (zeros + 256 * kZeroRounds - 1) / (256 * kZeroRounds);
+  Transpose tr{};
+  if (x.t_stride[2] != 0) {
+    tr.out = reinterpret_cast<uint2*>(g.scratch + at.words);
+    tr.live = reinterpret_cast<uint8_t*>(g.scratch + at.live);
+    tr.Hm = p.word_stride[1] != 0 ? x.H / x.hb : 1;
+    tr.key_words = static_cast<int>(KT * 4);
+    tr.total = int64_t{p.word_stride[0] != 0 ? p.B : 1} * tr.Hm * x.QT1 * tr.key_words;
+    x.words_t = tr.out;
+    x.live_t = reinterpret_cast<const uint32_t*>(tr.live);
+  }
+  if (row_blocks + zero_blocks + (tr.total + 7) / 8 > 0x7FFFFFFFll) {
+    *msg = "backward: batch*heads too large";
+    return kErrArg;
   }
   if (e == cudaSuccess)
-    e = launch_pdl(cross_delta_kernel<D, BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
-                   static_cast<const uint4*>(g.dout), static_cast<const uint4*>(p.out),
-                   static_cast<const uint4*>(p.out_lo), p.lse, neg_delta, neg_delta + rows, dq_accum, rows);
+    e = launch_pdl(cross_prepare_kernel<D, BF16>, static_cast<unsigned>(row_blocks + zero_blocks + (tr.total + 7) / 8), 256, 0,
+                   p.stream, static_cast<const uint4*>(g.dout), static_cast<const uint4*>(p.out),
+                   static_cast<const uint4*>(p.out_lo), p.lse, neg_delta, neg_delta + rows, dq_accum, rows,
+                   static_cast<unsigned>(row_blocks), reinterpret_cast<float4*>(g.scratch + at.bias), zeros,
+                   static_cast<unsigned>(zero_blocks), tr, x);
   if (e == cudaSuccess)
     e = launch_pdl(kern, static_cast<unsigned>(std::min<int64_t>(items, dp.sms)), kThreads, kSmemBytes, p.stream, mq, mk,
                    mv, mdo, mdq, neg_delta + rows, neg_delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),

@@ -176,6 +176,10 @@ struct Geo {
   const uint32_t* words;   // 16-byte aligned rows of W words (W % 4 == 0), or nullptr
   int64_t word_stride[3];  // batch, head, query, in words
   int row_shared;          // every row of a tile has the same mask row
+  // Live key tiles of every 128-row tile, from the packer: bit t of word k is
+  // key tile 32 k + t; strides for batch, head block (h0 / hb) and query tile.
+  const uint32_t* occ;
+  int64_t occ_stride[3];
   const int32_t* lengths;
   int kv_shared;           // all batches read the keys of batch 0
   uint16_t* out_lo;        // O minus its rounded value, in the inputs' type, or nullptr
@@ -828,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       xt = rr - hb_t * x.tn;
       xb = hb_t / x.hb;
       xh = hb_t - xb * x.hb;
-      need_scan = x.words != nullptr || x.lengths != nullptr;
+      need_scan = x.words == nullptr && x.lengths != nullptr;
     }
     // Whether this thread's row of `it` is a row of the problem.
     auto row_ok = [&](const Item& it) -> bool {
@@ -890,9 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // This thread's packed-mask row of `it` into L1 (a prefetch holds no registers).
     auto prefetch_rows_l1 = [&](const Item& it) {
-      if constexpr (kX) {
-        if (x.words == nullptr || x.row_shared) return;
-      }
+      if constexpr (kX) return;
       if (!row_ok(it)) return;
       const uintptr_t a0 = reinterpret_cast<uintptr_t>(row_ptr(it));
       const uintptr_t a1 = a0 + static_cast<uintptr_t>(W) * 4u;
@@ -905,31 +907,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto scan_post = [&](const Item& it, int j) {
       const int nw = (KT + 31) >> 5;
       if constexpr (kX) {
-        if (x.words == nullptr) {  // lengths: the tiles below the row's limit
-          const int tiles = row_ok(it) ? x.KTp + (max(row_limit(it, it.q0 + xt), 0) + kBN - 1) / kBN : 0;
-          for (int k = 0; k < nw; ++k) {
-            const uint32_t bits = __reduce_or_sync(0xffffffffu, low_bits(tiles - 32 * k));
-            if (lane == 0 && bits != 0u) atomicOr(&cc.scan_bits[j % kSlots][k], bits);
-          }
-          return;
+        // Only lengths are scanned (masks come with the packer's bits): the
+        // tiles below the row's limit.
+        const int tiles = row_ok(it) ? x.KTp + (max(row_limit(it, it.q0 + xt), 0) + kBN - 1) / kBN : 0;
+        for (int k = 0; k < nw; ++k) {
+          const uint32_t bits = __reduce_or_sync(0xffffffffu, low_bits(tiles - 32 * k));
+          if (lane == 0 && bits != 0u) atomicOr(&cc.scan_bits[j % kSlots][k], bits);
         }
-        if (x.row_shared) {  // one mask row for the tile: its 16-byte groups are shared out to the threads
-          const uint4* row16 = reinterpret_cast<const uint4*>(row_ptr(it));
-          for (int g0 = wq * 32; g0 < G4; g0 += 128) {
-            const int gi = g0 + lane;
-            // 32 groups: 32 tiles (one word, D = 64) or 64 tiles (two words, D = 128).
-            const int k = gi / kGroupsPerWord;
-            uint32_t bits = 0u;
-            if (gi < G4) bits = group_live<D>(__ldg(row16 + gi), gi, k, N);
-            constexpr int kPer = kGroupsPerWord;  // 32 or 16 lanes per word
-            const uint32_t lo = __reduce_or_sync(0xffffffffu, lane < kPer ? bits : 0u);
-            const uint32_t hi = __reduce_or_sync(0xffffffffu, lane < kPer ? 0u : bits);
-            const int k0 = g0 / kGroupsPerWord;
-            if (lane == 0 && lo != 0u) atomicOr(&cc.scan_bits[j % kSlots][k0], lo);
-            if (kPer == 16 && lane == 0 && hi != 0u) atomicOr(&cc.scan_bits[j % kSlots][k0 + 1], hi);
-          }
-          return;
-        }
+        return;
       }
       const uint32_t* mrow = row_ptr(it);
       const bool in_rows = row_ok(it);
@@ -1049,7 +1034,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           tiles = cc.scan_bits[slot][lane];
           cc.scan_bits[slot][lane] = 0u;  // ready for the item four later
-          if (kX && !need_scan) tiles = 0xFFFFFFFFu;  // every key is kept
+          if constexpr (kX) {
+            if (x.words != nullptr) {
+              const Item itj = item_at(c, j);
+              tiles = __ldg(x.occ + itj.b0 * x.occ_stride[0] + itj.h0 / x.hb * x.occ_stride[1] +
+                            itj.q0 / kBM * x.occ_stride[2] + lane);
+            } else if (x.lengths == nullptr) {
+              tiles = 0xFFFFFFFFu;  // every key is kept
+            }
+          }
         }
         if (KT - lane * 32 < 32) tiles &= (1u << (KT - lane * 32)) - 1u;
       }
@@ -1325,7 +1318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // D = 128 loads short rows (up to kEpiGroups 16-byte groups) outright
       // below, before it writes O.
       bool scan_regs = !kBoolIn && !C::kStageO && vec && G4 <= kEpiGroups;
-      if constexpr (kX) scan_regs = scan_regs && x.words != nullptr && !x.row_shared;
+      if constexpr (kX) scan_regs = false;
       if (!kBoolIn && do_scan && need_scan && !scan_regs) prefetch_rows_l1(itn);
       const float inv = (l_out > 0.f) ? (1.f / l_out) : 0.f;
       const float lse_row = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -FLT_MAX;

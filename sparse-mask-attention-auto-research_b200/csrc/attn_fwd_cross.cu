@@ -8,49 +8,91 @@ namespace {
 
 // ---------------------------------------------------------------- mask packer
 // bool bytes with any batch / head / query strides -> words [Bm, Hm, Qm, W],
-// W = 4 ceil(Nk / 128) (whole 128-key tiles; bits at columns >= Nk are 0).
-// One thread per word.  A word's 32 bytes start at any address: the aligned
-// 16-byte vectors that cover them are packed to bits first, and the bits are
-// shifted into place.  Bound by HBM: every mask byte is read once (a vector
-// shared by two words the second time from L1).  Vectors that would reach
-// outside the mask's own span [lo, hi) are read byte by byte.
+// W = 4 ceil(Nk / 128) (whole 128-key tiles; bits at columns >= Nk are 0), and
+// for every 128-row tile of the attention kernel (Geo's rows) the bits of its
+// live key tiles, which then needs no scan of the words.  One CTA per tile and
+// stretch of 8 key tiles or more; a thread packs the words of one column in
+// every kPackThreads / columns-th row and notes whether it saw one live.
+//
+// A word's 32 bytes start at any address: the aligned 16-byte vectors that
+// cover them are packed to bits first, and the bits are shifted into place.
+// Bound by HBM: every mask byte is read once (a vector shared by two words the
+// second time from L1).  Vectors that would reach outside the mask's own span
+// [lo, hi) are read byte by byte.
 constexpr int kPackThreads = 256;
-constexpr int kPackRounds = 4;
+constexpr int kPackWords = 256;   // words of a row per CTA, at most
+constexpr int kPackRounds = 4;    // words per thread with their loads in flight
 
-__device__ __forceinline__ uint32_t pack_word(const uint8_t* a, const uint8_t* lo, const uint8_t* hi, int valid) {
-  const uint32_t keep = valid >= 32 ? 0xFFFFFFFFu : (1u << valid) - 1u;
-  const int sh = static_cast<int>(reinterpret_cast<uintptr_t>(a) & 15u);
-  const uint8_t* v = a - sh;
-  const int bytes = sh == 0 ? 32 : 48;
-  if (v >= lo && v + bytes <= hi) {
-    const uint4* p = reinterpret_cast<const uint4*>(v);
-    unsigned long long bits = pack16_any(__ldg(p)) | (pack16_any(__ldg(p + 1)) << 16);
-    if (sh != 0) bits |= static_cast<unsigned long long>(pack16_any(__ldg(p + 2))) << 32;
-    return static_cast<uint32_t>(bits >> sh) & keep;
-  }
-  uint32_t w = 0u;
-  for (int i = 0; i < min(valid, 32); ++i) w |= (a[i] != 0 ? 1u : 0u) << i;
-  return w;
-}
+struct PackParams {
+  const uint8_t* mask;
+  const uint8_t* hi;          // end of the mask's span
+  int64_t sb, sh, sq;
+  uint32_t* words;
+  uint8_t* occ;               // [Bm][Hb][QT][occ_words * 4], 8 key tiles per byte
+  int Hm, Qm, Nk, W;
+  int hb, tn, rows;           // heads and queries of a tile, as far as the mask has them
+  int Hb, QT;                 // head blocks, query tiles
+  int chunks, chunk_log2;     // stretches of a row, 2^chunk_log2 words each
+  int occ_words, tile_log2;   // words of live bits per tile; packed words per key tile
+};
 
-__global__ void __launch_bounds__(kPackThreads)
-    pack_rows_kernel(const uint8_t* __restrict__ mask, const uint8_t* hi, uint32_t* __restrict__ words, int64_t sb,
-                     int64_t sh, int64_t sq, int Hm, int Qm, int Nk, int W, int64_t total) {
+__global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_constant__ PackParams p) {
   pdl_launch_dependents();
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kPackThreads * kPackRounds) + threadIdx.x;
+  __shared__ uint32_t live[kPackWords / 2 / 32];  // a key tile is 2 or 4 words
+  const int chunk = blockIdx.x % p.chunks;
+  int rest = blockIdx.x / p.chunks;
+  const int qt = rest % p.QT;
+  rest /= p.QT;
+  const int hblk = rest % p.Hb;
+  const int64_t b = rest / p.Hb;
+  if (threadIdx.x < kPackWords / 2 / 32) live[threadIdx.x] = 0u;
+  pdl_wait_prior_grid();
+  const int c = threadIdx.x & ((1 << p.chunk_log2) - 1), w = (chunk << p.chunk_log2) + c;
+  const int valid = p.Nk - 32 * w;
+  const int step = kPackThreads >> p.chunk_log2;
+  uint32_t any = 0u;
+  for (int r0 = threadIdx.x >> p.chunk_log2; w < p.W && r0 < p.rows; r0 += step * kPackRounds) {
+    // All loads first: the two or three aligned vectors of each word.
+    uint4 x[kPackRounds][3];
+    const uint8_t* src[kPackRounds];
+    int64_t at[kPackRounds];
+    bool whole[kPackRounds];
 #pragma unroll
-  for (int u = 0; u < kPackRounds; ++u) {
-    const int64_t idx = first + u * kPackThreads;
-    if (idx >= total) return;
-    const int64_t row = idx / W;
-    const int w = static_cast<int>(idx - row * W);
-    const int64_t bh = row / Qm;
-    const int q = static_cast<int>(row - bh * Qm);
-    const int64_t b = bh / Hm;
-    const int64_t h = bh - b * Hm;
-    const int valid = Nk - 32 * w;
-    words[idx] = valid > 0 ? pack_word(mask + b * sb + h * sh + q * sq + 32 * w, mask, hi, valid) : 0u;
+    for (int u = 0; u < kPackRounds; ++u) {
+      const int r = r0 + u * step;
+      const int hr = p.hb > 1 ? r / p.tn : 0, t = qt * kBM + r - hr * p.tn;
+      const int64_t h = static_cast<int64_t>(hblk) * p.hb + hr;
+      const bool in = r < p.rows && t < p.Qm;
+      at[u] = in ? ((b * p.Hm + h) * p.Qm + t) * p.W + w : -1;
+      src[u] = p.mask + b * p.sb + h * p.sh + t * p.sq + 32 * w;
+      const int sh = static_cast<int>(reinterpret_cast<uintptr_t>(src[u]) & 15u);
+      const uint8_t* v = src[u] - sh;
+      whole[u] = in && valid > 0 && v >= p.mask && v + (sh != 0 ? 48 : 32) <= p.hi;
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      x[u][0] = whole[u] ? __ldcs(reinterpret_cast<const uint4*>(v)) : zero;
+      x[u][1] = whole[u] ? __ldcs(reinterpret_cast<const uint4*>(v) + 1) : zero;
+      x[u][2] = whole[u] && sh != 0 ? __ldcs(reinterpret_cast<const uint4*>(v) + 2) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < kPackRounds; ++u) {
+      const int sh = static_cast<int>(reinterpret_cast<uintptr_t>(src[u]) & 15u);
+      const unsigned long long bits = pack16_any(x[u][0]) | (pack16_any(x[u][1]) << 16) |
+                                      static_cast<unsigned long long>(pack16_any(x[u][2])) << 32;
+      uint32_t word = static_cast<uint32_t>(bits >> sh) & (valid >= 32 ? 0xFFFFFFFFu : (1u << max(valid, 0)) - 1u);
+      if (at[u] >= 0 && !whole[u])
+        for (int i = 0; i < min(valid, 32); ++i) word |= (src[u][i] != 0 ? 1u : 0u) << i;
+      if (at[u] >= 0) p.words[at[u]] = word;
+      any |= word;
+    }
   }
+  __syncthreads();
+  if (any != 0u) atomicOr(&live[(c >> p.tile_log2) >> 5], 1u << ((c >> p.tile_log2) & 31));
+  __syncthreads();
+  // Bytes of live bits of a chunk (a row in one chunk may have fewer than 8 tiles, and writes all of its words).
+  const int bytes = p.chunks == 1 ? p.occ_words * 4 : 1 << (p.chunk_log2 - p.tile_log2 - 3);
+  const int k = chunk * bytes + threadIdx.x;
+  if (threadIdx.x < bytes && k < p.occ_words * 4)
+    p.occ[((b * p.Hb + hblk) * p.QT + qt) * (p.occ_words * 4) + k] = reinterpret_cast<const uint8_t*>(live)[threadIdx.x];
 }
 
 // ---------------------------------------------------------------- bias by relative position
@@ -296,13 +338,8 @@ int launch(const CrossParams& p, const Keys& keys, Geo x, int pieces, Partial in
   return kOk;
 }
 
-// One launch over `keys`.  `partial`: takes in / leaves a piece of every row
-// (always the split kernel, whose merge does that).  `with_prefix`: p's prefix
-// stands in front of the keys.
-int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool partial, Partial in, Partial out,
-                 const char** msg) {
-  DeviceProps dp;
-  if (!device_props(&dp, msg)) return kErrCuda;
+// The rows of a tile.
+Geo tile_geometry(const CrossParams& p, bool shared_keys) {
   Geo x{};
   x.B = static_cast<int>(p.B);
   x.H = static_cast<int>(p.H);
@@ -313,14 +350,100 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool 
   for (int h = 1; h <= G; ++h)
     if (G % h == 0 && h * x.tn <= kBM) x.hb = h;
   x.gh = G / x.hb;
-  x.nb = keys.shared ? std::max(1, std::min<int>(x.B, kBM / (x.tn * x.hb))) : 1;
+  x.nb = shared_keys ? std::max(1, std::min<int>(x.B, kBM / (x.tn * x.hb))) : 1;
   x.rows = x.tn * x.hb * x.nb;
+  return x;
+}
+
+// The packed mask of p: its words, and behind them the live-tile bits.
+struct PackLayout {
+  int64_t words;         // their number
+  int64_t Bm, Hm, Qm;    // lengths of the axes the mask has, 1 for the others
+  int64_t Hb, QT;        // head blocks and query tiles it has
+  int64_t occ_words;
+};
+PackLayout pack_layout(const CrossParams& p, const Geo& x) {
+  PackLayout l{};
+  l.Bm = p.word_stride[0] != 0 ? p.B : 1;
+  l.Hm = p.word_stride[1] != 0 ? p.H : 1;
+  l.Qm = p.word_stride[2] != 0 ? p.Nq : 1;
+  l.words = l.Bm * l.Hm * l.Qm * ((p.Nk + 127) / 128 * 4);
+  l.Hb = p.word_stride[1] != 0 ? p.H / x.hb : 1;
+  l.QT = p.word_stride[2] != 0 ? (p.Nq + kBM - 1) / kBM : 1;
+  const int64_t bn = p.D == 64 ? 128 : 64;
+  l.occ_words = ((p.Nk + bn - 1) / bn + 31) / 32;
+  return l;
+}
+
+int launch_pack(const CrossParams& p, const char** msg) {
+  const Geo x = tile_geometry(p, false);
+  const PackLayout l = pack_layout(p, x);
+  PackParams k{};
+  k.mask = p.mask;
+  k.sb = p.mask_stride[0];
+  k.sh = p.mask_stride[1];
+  k.sq = p.mask_stride[2];
+  k.hi = p.mask + (l.Bm - 1) * k.sb + (l.Hm - 1) * k.sh + (l.Qm - 1) * k.sq + p.Nk;
+  k.words = p.words;
+  k.occ = reinterpret_cast<uint8_t*>(p.words + l.words);
+  k.Hm = static_cast<int>(l.Hm);
+  k.Qm = static_cast<int>(l.Qm);
+  k.Nk = static_cast<int>(p.Nk);
+  k.W = static_cast<int>((p.Nk + 127) / 128 * 4);
+  k.hb = p.word_stride[1] != 0 ? x.hb : 1;
+  k.tn = p.word_stride[2] != 0 ? x.tn : 1;
+  k.rows = k.hb * k.tn;
+  k.Hb = static_cast<int>(l.Hb);
+  k.QT = static_cast<int>(l.QT);
+  k.occ_words = static_cast<int>(l.occ_words);
+  k.tile_log2 = p.D == 64 ? 2 : 1;
+  // The longest stretch (fewest CTAs) that still gives every SM a few CTAs; 8
+  // key tiles at least.
+  DeviceProps dp;
+  if (!device_props(&dp, msg)) return kErrCuda;
+  const int64_t tiles = l.Bm * l.Hb * l.QT;
+  k.chunk_log2 = 8;
+  while (k.chunk_log2 > k.tile_log2 + 3 && tiles * (((k.W - 1) >> k.chunk_log2) + 1) < 6 * dp.sms) --k.chunk_log2;
+  while ((1 << (k.chunk_log2 - 1)) >= k.W) --k.chunk_log2;
+  k.chunks = ((k.W - 1) >> k.chunk_log2) + 1;
+  const int64_t blocks = tiles * k.chunks;
+  if (blocks > 0x7FFFFFFFll) {
+    *msg = "attention: mask too large";
+    return kErrArg;
+  }
+  const cudaError_t e =
+      launch_pdl(pack_tiles_kernel, static_cast<unsigned>(blocks), kPackThreads, 0, p.stream, k);
+  if (e != cudaSuccess) {
+    *msg = cudaGetErrorString(e);
+    return kErrLaunch;
+  }
+  return kOk;
+}
+
+// One launch over `keys`.  `partial`: takes in / leaves a piece of every row
+// (always the split kernel, whose merge does that).  `with_prefix`: p's prefix
+// stands in front of the keys.
+int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool partial, Partial in, Partial out,
+                 const char** msg) {
+  DeviceProps dp;
+  if (!device_props(&dp, msg)) return kErrCuda;
+  Geo x = tile_geometry(p, keys.shared);
   x.kv_shared = keys.shared ? 1 : 0;
   x.out_lo = static_cast<uint16_t*>(p.out_lo);
   if (!keys.shared) {
     x.words = p.words;
     for (int i = 0; i < 3; ++i) x.word_stride[i] = p.word_stride[i];
     x.row_shared = p.words != nullptr && (x.Nq == 1 || p.word_stride[2] == 0) && (x.hb == 1 || p.word_stride[1] == 0);
+    if (p.words != nullptr) {
+      const PackLayout l = pack_layout(p, x);
+      x.occ = p.words + l.words;
+      int64_t step = l.occ_words;
+      x.occ_stride[2] = p.word_stride[2] != 0 ? step : 0;
+      step *= l.QT;
+      x.occ_stride[1] = p.word_stride[1] != 0 ? step : 0;
+      step *= l.Hb;
+      x.occ_stride[0] = p.word_stride[0] != 0 ? step : 0;
+    }
     x.lengths = p.lengths;
   }
   const int bn = p.D == 64 ? 128 : 64;
@@ -351,28 +474,6 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool 
 
 }  // namespace
 
-int launch_pack_rows(const uint8_t* mask, const int64_t* stride, uint32_t* words, int64_t Bm, int64_t Hm, int64_t Qm,
-                     int64_t Nk, cudaStream_t stream, const char** msg) {
-  const int64_t W = (Nk + 127) / 128 * 4;
-  const int64_t total = Bm * Hm * Qm * W;
-  if (total == 0) return kOk;
-  const int64_t blocks = (total + kPackThreads * kPackRounds - 1) / (kPackThreads * kPackRounds);
-  if (blocks > 0x7FFFFFFFll) {
-    *msg = "pack_mask: input too large";
-    return kErrArg;
-  }
-  const uint8_t* hi = mask + (Bm - 1) * stride[0] + (Hm - 1) * stride[1] + (Qm - 1) * stride[2] + Nk;
-  pack_rows_kernel<<<static_cast<unsigned>(blocks), kPackThreads, 0, stream>>>(
-      mask, hi, words, stride[0], stride[1], stride[2], static_cast<int>(Hm), static_cast<int>(Qm),
-      static_cast<int>(Nk), static_cast<int>(W), total);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    *msg = cudaGetErrorString(e);
-    return kErrLaunch;
-  }
-  return kOk;
-}
-
 int launch_fill(float* x, int64_t n, float v, cudaStream_t stream) {
   if (n <= 0) return kOk;
   fill_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(x, n, v);
@@ -402,8 +503,7 @@ int launch_bias_expand(const CrossParams& p, const char** msg) {
 
 int launch_attn_cross(const CrossParams& p, const char** msg) {
   if (p.mask != nullptr) {
-    const int rc = launch_pack_rows(p.mask, p.mask_stride, p.words, p.word_stride[0] ? p.B : 1,
-                                    p.word_stride[1] ? p.H : 1, p.word_stride[2] ? p.Nq : 1, p.Nk, p.stream, msg);
+    const int rc = launch_pack(p, msg);
     if (rc != kOk) return rc;
   }
   if (p.bias.table != nullptr) {

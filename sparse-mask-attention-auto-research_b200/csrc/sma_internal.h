@@ -117,7 +117,8 @@ struct CrossParams {
   void* out;                  // [B, H, Nq, D] contiguous
   float* lse;                 // [B, H, Nq] or nullptr
   // attn_fwd_cross.cu and attn_bwd_cross.cu: the packed mask ([.., W] words with
-  // strides {batch, head, query}, 0: broadcast; nullptr keeps every key), the
+  // strides {batch, head, query}, 0: broadcast, and behind them the live-tile
+  // bits; nullptr keeps every key), the
   // bias by relative position, [H][bias_hi - bias_lo + 1 + 2 kBiasPad], and
   // O minus its rounded value, in the inputs' type (nullptr: not wanted).
   uint32_t* words;
@@ -146,9 +147,6 @@ inline void bias_range(const BiasSpec& s, int* lo, int* hi) {
 // on either side, so that a tile which overlaps (lo, hi) never leaves it.
 constexpr int kBiasPad = 256;
 
-// Bool bytes -> words [Bm, Hm, Qm, 4 * ceil(Nk / 128)] (attn_fwd_cross.cu).
-int launch_pack_rows(const uint8_t* mask, const int64_t* stride, uint32_t* words, int64_t Bm, int64_t Hm, int64_t Qm,
-                     int64_t Nk, cudaStream_t stream, const char** msg);
 // Fills p.bias_distance from p.bias.
 int launch_bias_expand(const CrossParams& p, const char** msg);
 // Many query rows (attn_fwd_cross.cu), Nk <= kMaxSeqLen.

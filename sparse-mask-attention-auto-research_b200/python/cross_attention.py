@@ -26,7 +26,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib, sparse_attn_cuda
-from .sparse_attn_cuda import _require, _strided
+from .sparse_attn_cuda import _empty, _require, _strided
 
 _DTYPES = (torch.float16, torch.bfloat16)
 
@@ -94,7 +94,7 @@ class CrossAttentionFunction(Function):
             ctx.bias = bias._replace(table=None, offsets=None)
         else:
             ctx.bias = None
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty(q)
         saved, ctx.mask_strides = sparse_attn_cuda.cross_forward(q, k, v, out, scale, mask, bias, training=True)
         ctx.scale = scale
         ctx.save_for_backward(q, k, v, out, saved, table, offsets)
@@ -128,7 +128,7 @@ def _attention(q, k, v, mask, scale, bias):
         _require(steps <= _MAX_STEPS, f"with gradients at most {_MAX_STEPS} steps of 64 queries may share a key head")
         return CrossAttentionFunction.apply(q, k, v, table, mask, scale, bias)
     q, k, v = _strided(q), _strided(k), _strided(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _empty(q)
     if _few_rows(q, k):
         sparse_attn_cuda.rows_forward(q, k, v, out, scale, mask=mask, bias=bias)
     else:
@@ -250,7 +250,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths=None, scale=Non
     if dtype == torch.float32:
         q, k_prefix, v_prefix, k, v = (t.bfloat16() for t in (q, k_prefix, v_prefix, k, v))
     q, k_prefix, v_prefix, k, v = (_strided(t) for t in (q, k_prefix, v_prefix, k, v))
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _empty(q)
     prefix = (k_prefix, v_prefix)
     if B == 1 or k_prefix.shape[1] == 0 or S > _lib.SMA_MAX_SEQ_LEN:
         sparse_attn_cuda.rows_forward(q, k, v, out, scale, lengths=lengths, prefix=prefix)

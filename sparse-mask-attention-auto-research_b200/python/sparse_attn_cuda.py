@@ -219,6 +219,11 @@ def _strided(t):
     return t.contiguous()
 
 
+def _empty(t):
+    """A contiguous tensor like `t` (empty_like costs half of empty's host time)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _mask_strides(mask):
     """`mask` with a contiguous last axis, and its strides along the others (0
     where it is broadcast)."""
@@ -295,11 +300,13 @@ def _saved_layout(q, k, mask_strides, bias, training):
     words = distance = lse = out_lo = 0
     if mask_strides is not None:
         words = end
-        rows = 1
-        for n, s in zip((B, H, Nq), mask_strides):
+        rows, tiles = 1, 1
+        for n, s, per in zip((B, H, Nq), mask_strides, (1, 1, 128)):
             if s:
                 rows *= n
-        end += rows * ((k.shape[2] + 127) // 128 * 16)
+                tiles *= (n + per - 1) // per
+        Nk = k.shape[2]
+        end += rows * ((Nk + 127) // 128 * 16) + (tiles * ((Nk + 2047) // 2048) * 4 + 15) // 16 * 16
     if bias is not None:
         distance = end
         n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 513
@@ -342,8 +349,7 @@ def cross_backward(dout, q, k, v, out, scale, saved, mask_strides=None, bias=Non
     args = _attn_args(q, k, v, out, scale, 0, mask_strides or (0, 0, 0), bias=bias, lse=base + lse,
                       words=words and base + words, bias_distance=distance and base + distance, out_lo=base + out_lo)
     lib = _lib.load()
-    dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
-    dv = torch.empty_like(dk)
+    dq, dk, dv = _empty(q), _empty(k), _empty(k)
     with _device_guard(q.device):
         dtable = None if bias is None else torch.empty_like(bias.table)
         floats = lib.sma_cross_attn_bwd_scratch(args)
