@@ -258,9 +258,10 @@ SMA_API int sma_rows_attn_fwd(const sma_attn_args* args, void* stream);
 SMA_API int sma_cross_attn_fwd(const sma_attn_args* args, void* stream);
 
 /*
- * Attention behind a prefix shared by the batch, the prefix read once for all:
- * its tiles hold the rows of several sequences.  P > 0, Nk <= SMA_MAX_SEQ_LEN,
- * `lengths` or nothing for the sequences' own keys, no mask, no bias, no lse.
+ * Attention behind a prefix shared by the batch.  Where it pays, the prefix is
+ * read once for all sequences (its tiles hold the rows of several).  P > 0,
+ * Nk <= SMA_MAX_SEQ_LEN, `lengths` or nothing for the sequences' own keys, no
+ * mask, no bias, no lse.  Own keys behind a sequence's length may hold anything.
  */
 SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
 

@@ -233,10 +233,6 @@ int choose_pieces(int64_t items, int64_t tiles, int64_t chains, bool merge_anywa
   return best;
 }
 
-// A shared prefix is taken in one pass per sequence when a key head has more
-// rows than this: the rows of one sequence then fill most of a tile.
-constexpr int kOnePassRows = 64;
-
 // The keys of one launch: k and v with their strides {batch, head, row}.
 struct Keys {
   const void* k;
@@ -514,10 +510,21 @@ int launch_attn_cross(const CrossParams& p, const char** msg) {
   return launch_tiles(p, keys, false, false, {}, {}, msg);
 }
 
-// Either one pass over prefix and own keys per sequence, or the prefix once for
-// the batch: the sequences' own keys leave a piece of every row (FP32), then
-// the prefix is attended with the rows of several sequences in one tile, and
-// its merge takes those pieces in.
+// Three ways, by their cost in us (measured on a B200, see below):
+//   rows    the streaming kernel, prefix and own keys per 16 rows: little
+//           work, or little to share;
+//   tiles   128-row tiles, prefix and own keys in one pass per sequence: the
+//           rows of one sequence fill most of a tile;
+//   shared  the prefix once for the batch: the sequences' own keys leave a
+//           piece of every row (FP32), then the prefix is attended with the
+//           rows of several sequences in one tile, and its merge takes those
+//           pieces in.
+// rows: 8 + 1 per 8.5 MB of keys streamed (from L2 where the prefix is read
+// again): B16 Hkv8 P1024 D128 17.1 (shared: 21.1), P4096 39.7 (31.0).  The two
+// others: 23 + 7.3 ns (D = 64) or 12.5 ns per 128 x 128 tile, and for `shared`
+// the own keys streamed at 6 MB per us (one tile of 16 rows) or 8 us for one
+// more launch of tiles: B64 Hkv8 G4 P256 D128 23.1 (rows: 17.4), P1024
+// with S256 30.7 (43.5).
 int launch_shared_prefix(const CrossParams& p, const char** msg) {
   DeviceProps dp;
   if (!device_props(&dp, msg)) return kErrCuda;
@@ -526,8 +533,23 @@ int launch_shared_prefix(const CrossParams& p, const char** msg) {
   const Keys own_keys{p.k, p.v, p.k_stride, p.v_stride, p.Nk, false};
   const int64_t bn = p.D == 64 ? 128 : 64;
   const int64_t own_tiles = (p.Nk + bn - 1) / bn, prefix_tiles = (p.P + bn - 1) / bn;
-  if (group_rows > kOnePassRows && own_tiles + prefix_tiles <= kMaxSeqLen / bn)
-    return launch_tiles(p, own_keys, true, false, {}, {}, msg);
+  {
+    const Geo once = tile_geometry(p, true), own = tile_geometry(p, false);
+    const double heads = static_cast<double>(p.B * p.Hkv), ns = p.D == 64 ? 7.3e-3 : 12.5e-3;
+    const double q_tiles = static_cast<double>((p.Nq + kBM - 1) / kBM);
+    const double per_key = 4.0 * static_cast<double>(p.D) * 1e-6;  // MB of K and V
+    const double rows_us = 8.0 + heads * static_cast<double>((group_rows + kRowsTile - 1) / kRowsTile) *
+                                     static_cast<double>(p.P + p.Nk) * per_key / 8.5;
+    const double tile_us = ns * q_tiles * static_cast<double>(bn) / 128.0;  // per group and key tile
+    const double own_us = heads * own.gh * tile_us * static_cast<double>(own_tiles);
+    const double tiles_us = 23.0 + own_us + heads * own.gh * tile_us * static_cast<double>(prefix_tiles);
+    const double shared_us = 23.0 + static_cast<double>((p.B + once.nb - 1) / once.nb * p.Hkv) * once.gh * tile_us *
+                                        static_cast<double>(prefix_tiles) +
+                             (group_rows <= kRowsTile ? heads * static_cast<double>(p.Nk) * per_key / 6.0 : 8.0 + own_us);
+    if (rows_us <= tiles_us && rows_us <= shared_us) return launch_attn_rows(p, msg);
+    if (tiles_us <= shared_us && own_tiles + prefix_tiles <= kMaxSeqLen / bn)
+      return launch_tiles(p, own_keys, true, false, {}, {}, msg);
+  }
   void* ws = nullptr;
   Partial part;
   int rc = kOk;

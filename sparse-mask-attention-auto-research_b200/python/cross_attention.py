@@ -70,13 +70,29 @@ def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-# Query rows per key head (queries times the heads that share one) up to which
-# the streaming kernel is taken; above, the 128-row tiles.
-_ROWS = 16
+def _few_rows(q, k, mask, bias):
+    """Whether the streaming kernel is taken (16 rows of a key head at a time,
+    the keys read again for every 16) instead of the 128-row tiles.
 
-
-def _few_rows(q, k):
-    return q.shape[1] // max(k.shape[1], 1) * q.shape[2] <= _ROWS or k.shape[2] > _lib.SMA_MAX_SEQ_LEN
+    With no mask, or one that all rows of a key head share, and R rows per key
+    head in T tiles of 128, the first takes (measured on a B200) about 8 us +
+    B Hkv Nk D ceil(R / 16) * 0.57e-6 us, the second (which also packs the
+    mask) 18 us + B Hkv Nk D T * 0.9e-6 us (D = 64) or 0.77e-6 us (D = 128).
+    For instance B8 Hkv8 Nk1000 D64: 12.8 against 22.3 us at 64 rows, 22.9
+    against 25.0 at 128; B16 H12 Nk1500 D128: 31 against 50 us at 16 rows, 58
+    against 49 at 24.  Masks of the rows' own and a bias cost the first more:
+    B16 H12 Nk500 D64 with a mask 19.4 against 20.9 us at 16 rows, 35.5 against
+    21.0 at 32, so there it is taken for one tile of 16 rows only."""
+    B, H, Nq, D = q.shape
+    Hkv, Nk = k.shape[1:3]
+    if Nk > _lib.SMA_MAX_SEQ_LEN:
+        return True
+    rows = H // max(Hkv, 1) * Nq
+    if rows <= 16 or rows > 128:
+        return rows <= 16
+    if bias is not None or (mask is not None and (mask.shape[1] != 1 or mask.shape[2] != 1)):
+        return False
+    return B * Hkv * Nk * D * ((0.6 if D == 64 else 0.75) * ((rows + 15) // 16) - 1.0) <= 15e6
 
 
 class CrossAttentionFunction(Function):
@@ -129,7 +145,7 @@ def _attention(q, k, v, mask, scale, bias):
         return CrossAttentionFunction.apply(q, k, v, table, mask, scale, bias)
     q, k, v = _strided(q), _strided(k), _strided(v)
     out = _empty(q)
-    if _few_rows(q, k):
+    if _few_rows(q, k, mask, bias):
         sparse_attn_cuda.rows_forward(q, k, v, out, scale, mask=mask, bias=bias)
     else:
         sparse_attn_cuda.cross_forward(q, k, v, out, scale, mask, bias)
@@ -252,7 +268,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths=None, scale=Non
     q, k_prefix, v_prefix, k, v = (_strided(t) for t in (q, k_prefix, v_prefix, k, v))
     out = _empty(q)
     prefix = (k_prefix, v_prefix)
-    if B == 1 or k_prefix.shape[1] == 0 or S > _lib.SMA_MAX_SEQ_LEN:
+    if k_prefix.shape[1] == 0 or S > _lib.SMA_MAX_SEQ_LEN:
         sparse_attn_cuda.rows_forward(q, k, v, out, scale, lengths=lengths, prefix=prefix)
     else:
         sparse_attn_cuda.prefix_forward(q, k, v, out, scale, prefix, lengths)
