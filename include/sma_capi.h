@@ -224,8 +224,9 @@ typedef struct sma_attn_args {
   float* lse;  /* [B, H, Nq] natural-log sum of exponentials, or NULL */
   /* Of the 128-row tile entries: room for the packed mask, int32 words
    * [B, H, Nq, 4 * ceil(Nk / 128)] with length 1 for an axis whose mask_stride
-   * is 0 (bit b of word w: column 32 w + b, 0 past Nk), and for the live key
-   * tiles behind it, [B, H, ceil(Nq / 128), ceil(Nk / 2048)] more words. */
+   * is 0 (bit b of word w: column 32 w + b, 0 past Nk), and behind it, for
+   * every 128-row tile, the keys that some row keeps and the live key tiles:
+   * [B, H, ceil(Nq / 128), 4 * ceil(Nk / 128) + ceil(Nk / 2048)] more. */
   void* words;
   float* bias_distance; /* room for H * SMA_BIAS_DISTANCE_LEN floats */
   void* out_lo;         /* O minus its rounded value, like out, or NULL */
@@ -250,10 +251,9 @@ SMA_API int sma_rows_attn_fwd(const sma_attn_args* args, void* stream);
  * into `words` first, and a bias laid out in bias_distance (the backward reads
  * both, with the lse and out_lo, which training needs).  Queries of the heads
  * that share a key head fill a tile together when Nq <= 64.
- * Nk <= SMA_MAX_SEQ_LEN, no prefix; otherwise as sma_rows_attn_fwd, except
- * that a key which only some rows of a tile keep must hold finite values (a
- * key that a mask row shared by the tile, or the length, leaves out may hold
- * anything).  Rows that keep no key get out = 0 and lse = -FLT_MAX.
+ * Nk <= SMA_MAX_SEQ_LEN, no prefix; otherwise as sma_rows_attn_fwd: a key
+ * that none of a tile's rows keeps may hold any values, one that some keep
+ * must be finite.  Rows that keep no key get out = 0 and lse = -FLT_MAX.
  */
 SMA_API int sma_cross_attn_fwd(const sma_attn_args* args, void* stream);
 
@@ -274,7 +274,8 @@ SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
  *   dtable[bucket, h] = sum of dS over the pairs in the bucket.
  * scratch: sma_cross_attn_bwd_scratch(args) floats.
  * At most 2048 steps of 64 query rows per key head (SMA_ERR_UNSUPPORTED_N).
- * All values of K, V, Q and dO must be finite.  dq is accumulated by atomic
+ * Q, dO and every key must be finite, except that the keys a mask leaves to no
+ * query (B and Nk its only axes: padding) may hold anything.  dq is accumulated by atomic
  * adds in FP32, so its last bits can differ from run to run; dk, dv and
  * dtable do not.
  */

@@ -765,6 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* s_win = reinterpret_cast<float*>(smem + C::kOffBias) + warp * 96;  // kBias: bias by relative position
     bool ok = true;
     uint32_t lt0 = 0, lp0 = 0, use = 0;
+    int li = 0;
     // Mask bits of this key for the 64 queries of the next step of this stage.
     uint2 next_words = make_uint2(0u, 0u);
     bool have_words = false;
@@ -801,6 +802,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                   ? x.bias_offset
                   : max(-kMaxBiasOffset, min(kMaxBiasOffset, __ldg(x.bias_offsets + it.b)));
       }
+      // Where the item has one mask row, the K rows of keys it leaves out (they
+      // may hold anything) are cleared before the first dQ product, which runs
+      // over all keys.
+      if (g == 0 && n > 0 && x.words != nullptr && x.one_row) {
+        ok = wait_all(ctl.kv_full[li % C::kKVBufs], (li / C::kKVBufs) & 1);
+        if (!ok) break;
+        if (next_words.x == 0u) {
+          uint8_t* krow = smem + C::kOffK + (li % C::kKVBufs) * C::kKVBytes + t * 128;
+#pragma unroll
+          for (int e = 0; e < D / 8; ++e)
+            *reinterpret_cast<uint4*>(krow + (e >> 3) * (kKeys * 128) + (e & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();  // ahead of this thread's arrival on p_full
+      }
+      if (n > 0) ++li;
       auto flush_far = [&]() {
         if constexpr (kBias) {
           if (far_head < 0) return;
@@ -933,6 +949,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             else block(std::integral_constant<int, 1>{});
           } else {
             block(std::integral_constant<int, 0>{});
+          }
+          // A key that keeps no query of the block has dS = 0 whatever its V holds.
+          if (word == 0u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dw[e] = 0u;
+            if constexpr (kBias) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[e] = 0.f;
+            }
           }
           // P over S^T columns this warp has read (chunk c writes 16 c ..,
           // which chunks <= c have read).

@@ -175,11 +175,13 @@ struct Geo {
   int gh;                  // tiles of a head group, G / hb
   const uint32_t* words;   // 16-byte aligned rows of W words (W % 4 == 0), or nullptr
   int64_t word_stride[3];  // batch, head, query, in words
-  int row_shared;          // every row of a tile has the same mask row
   // Live key tiles of every 128-row tile, from the packer: bit t of word k is
   // key tile 32 k + t; strides for batch, head block (h0 / hb) and query tile.
   const uint32_t* occ;
   int64_t occ_stride[3];
+  // And which keys some row of the tile keeps: W words per tile, strides alike.
+  const uint32_t* kept;
+  int64_t kept_stride[3];
   const int32_t* lengths;
   int kv_shared;           // all batches read the keys of batch 0
   uint16_t* out_lo;        // O minus its rounded value, in the inputs' type, or nullptr
@@ -858,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return words + (static_cast<int64_t>(it.bh) * N + it.q0 + r) * W;
       }
     };
-    // kX with lengths: keys this row keeps, and the most that a row of the tile keeps.
+    // kX with lengths: the keys that query t of this thread's batch keeps.
     auto row_limit = [&](const Item& it, int t) -> int {
       if constexpr (kX) {
         const int len = max(0, min(N, __ldg(x.lengths + min(it.b0 + xb, x.B - 1))));
@@ -867,25 +869,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         return N;
       }
     };
+    // kX: which of keys 32 (r / 32) .. +31 of tile kt some row of the tile keeps.
+    uint32_t kept = 0xFFFFFFFFu;
     auto low_bits = [](int n) -> uint32_t { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u); };
-    // Mask words of key tile kt for this thread's row of `it` (0 for padding
-    // rows, except that with a row shared by the tile every thread has it).
-    auto fetch_words = [&](const Item& it, int kt, uint32_t (&mw)[kWords]) {
+    // What fetch_words needs of an item, worked out once for it (kX).
+    struct RowMask {
+      const uint32_t* words = nullptr;  // the row's packed mask, or nullptr: no row of the problem
+      const uint32_t* kept = nullptr;   // this warp's word of tile 0's kept keys
+      int limit = 0, kept_limit = 0;    // without a mask: own keys the row keeps, and any row of the tile
+    };
+    auto row_mask = [&](const Item& it) {
+      RowMask m;
+      if constexpr (kX) {
+        const bool in = row_ok(it);
+        if (x.words != nullptr) {
+          if (in) m.words = row_ptr(it);
+          m.kept = x.kept + it.b0 * x.kept_stride[0] + it.h0 / x.hb * x.kept_stride[1] +
+                   it.q0 / kBM * x.kept_stride[2] + (r >> 5);
+        } else if (x.lengths != nullptr) {
+          const int first = row_limit(it, 0);
+          m.limit = in ? first + it.q0 + xt : N;
+          m.kept_limit = first + min(it.q0 + x.tn, x.Nq) - 1;
+        } else {
+          m.limit = m.kept_limit = N;
+        }
+        if (!in) m.limit = 0x7FFFFFFF;
+      }
+      return m;
+    };
+    // Mask words of key tile kt for this thread's row of `it`.  Rows past the
+    // problem's, never stored: 0, or with kX all ones, which spares a warp
+    // that holds some the element-wise select.
+    auto fetch_words = [&](const Item& it, const RowMask& m, int kt, uint32_t (&mw)[kWords]) {
       if constexpr (kX) {
         if (x.words == nullptr) {
-          int limit = x.P;  // of the tile's own sequence: the prefix, or the row's keys
-          if (kt >= x.KTp) {
-            kt -= x.KTp;
-            limit = x.lengths != nullptr ? row_limit(it, it.q0 + xt) : N;
-          }
+          const bool pre = kt < x.KTp;
+          const int key0 = (pre ? kt : kt - x.KTp) * kBN;
+          const int limit = pre && m.limit != 0x7FFFFFFF ? x.P : m.limit;
+          kept = pre ? 0xFFFFFFFFu : low_bits(m.kept_limit - key0 - (r & ~31));
 #pragma unroll
-          for (int w = 0; w < kWords; ++w) mw[w] = row_ok(it) ? low_bits(limit - kt * kBN - 32 * w) : 0u;
+          for (int w = 0; w < kWords; ++w) mw[w] = low_bits(limit - key0 - 32 * w);
           return;
         }
-      }
-      bool load = row_ok(it);
-      if constexpr (kX) load = load || x.row_shared;
-      if (load) {
+        if ((r >> 5) < kWords) kept = __ldg(m.kept + kt * kWords);
+        if (m.words != nullptr) {
+          load_tile_words<D, kBoolIn>(m.words, kt, W, N, vec != 0, mw);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) mw[w] = 0xFFFFFFFFu;
+        }
+      } else if (row_ok(it)) {
         load_tile_words<D, kBoolIn>(row_ptr(it), kt, W, N, vec != 0, mw);
       } else {
 #pragma unroll
@@ -1096,7 +1129,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     uint32_t mw[kWords] = {};
-    bool have_mw = false;  // mw already holds tile 0 of the current item
+    bool have_mw = false;  // mw (and cur_mask) already hold tile 0 of the current item
+    RowMask cur_mask;
     for (int i = 0; i < n_items; ++i) {
       const int slot = i % kSlots;
       const Item it = item_at(c, i);
@@ -1119,7 +1153,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         bias_off = x.bias_offsets == nullptr
                        ? x.bias_offset
                        : max(-kMaxBiasOffset, min(kMaxBiasOffset, __ldg(x.bias_offsets + min(it.b0 + xb, x.B - 1))));
-      if (n > 0 && !have_mw) fetch_words(it, kt0, mw);
+      if (!have_mw) cur_mask = row_mask(it);
+      if (n > 0 && !have_mw) fetch_words(it, cur_mask, kt0, mw);
       have_mw = false;
       float m_run = -INFINITY, l_run = 0.f, l_out = 0.f;
 
@@ -1153,32 +1188,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
         if constexpr (kX) {
           // V rows of keys that no row of the tile keeps (padding, unused
-          // slots) are cleared, so that P = 0 times what they hold is 0.  Only
-          // masks that are the same for the whole tile are known to leave a
-          // key to no row without looking at the other rows.
-          bool dead = false, some = false;
-          if (x.words != nullptr && x.row_shared) {
-            uint32_t all = mw[0];
-#pragma unroll
-            for (int ch = 1; ch < kWords; ++ch) all &= mw[ch];
-            some = all != 0xFFFFFFFFu;
-            if (some) {
-              uint32_t word = mw[0];
-#pragma unroll
-              for (int ch = 1; ch < kWords; ++ch) word = (r >> 5) == ch ? mw[ch] : word;
-              dead = r < kBN && ((word >> (r & 31)) & 1u) == 0u;
-            }
-          } else if (x.lengths != nullptr && kt_cur >= x.KTp) {
-            const int most = row_limit(it, min(it.q0 + x.tn, x.Nq) - 1) - (kt_cur - x.KTp) * kBN;
-            some = most < kBN;
-            dead = r < kBN && r >= most;
-          }
-          if (some) {
+          // slots) are cleared, so that P = 0 times what they hold is 0: warp w
+          // looks after keys 32 w .. +31.
+          if (kept != 0xFFFFFFFFu && r < kBN) {
             if (!wait_all(cc.v_full[g % kStages], (g / kStages) & 1)) {
               ok = false;
               break;
             }
-            if (dead) {
+            if (((kept >> lane) & 1u) == 0u) {
               uint8_t* vrow = smem + c * C::kChainBytes + C::kQBufs * C::kQBytes + kStages * C::kKVBytes +
                               (g % kStages) * C::kKVBytes + r * 128;
 #pragma unroll
@@ -1232,9 +1249,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The next tile's mask words, a whole tile of exponentials ahead of their use.
         if (t + 1 < n) {
           kt_next = next_live(cc.live_bits[slot], lw, lx);
-          fetch_words(it, kt_next, mw);
+          fetch_words(it, cur_mask, kt_next, mw);
         } else if (next_kt >= 0) {
-          fetch_words(item_at(c, i + 1), next_kt, mw);
+          const Item it1 = item_at(c, i + 1);
+          cur_mask = row_mask(it1);
+          fetch_words(it1, cur_mask, next_kt, mw);
           have_mw = true;
         }
 

@@ -10,7 +10,8 @@ namespace {
 // bool bytes with any batch / head / query strides -> words [Bm, Hm, Qm, W],
 // W = 4 ceil(Nk / 128) (whole 128-key tiles; bits at columns >= Nk are 0), and
 // for every 128-row tile of the attention kernel (Geo's rows) the bits of its
-// live key tiles, which then needs no scan of the words.  One CTA per tile and
+// live key tiles, which then needs no scan of the words, and the keys that some
+// row of the tile keeps (the others' V is cleared there).  One CTA per tile and
 // stretch of 8 key tiles or more; a thread packs the words of one column in
 // every kPackThreads / columns-th row and notes whether it saw one live.
 //
@@ -29,6 +30,7 @@ struct PackParams {
   int64_t sb, sh, sq;
   uint32_t* words;
   uint8_t* occ;               // [Bm][Hb][QT][occ_words * 4], 8 key tiles per byte
+  uint32_t* kept;             // [Bm][Hb][QT][W]
   int Hm, Qm, Nk, W;
   int hb, tn, rows;           // heads and queries of a tile, as far as the mask has them
   int Hb, QT;                 // head blocks, query tiles
@@ -39,6 +41,7 @@ struct PackParams {
 __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_constant__ PackParams p) {
   pdl_launch_dependents();
   __shared__ uint32_t live[kPackWords / 2 / 32];  // a key tile is 2 or 4 words
+  __shared__ uint32_t kept[kPackWords];
   const int chunk = blockIdx.x % p.chunks;
   int rest = blockIdx.x / p.chunks;
   const int qt = rest % p.QT;
@@ -46,6 +49,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_c
   const int hblk = rest % p.Hb;
   const int64_t b = rest / p.Hb;
   if (threadIdx.x < kPackWords / 2 / 32) live[threadIdx.x] = 0u;
+  kept[threadIdx.x] = 0u;
+  static_assert(kPackThreads == kPackWords, "one thread per column");
   pdl_wait_prior_grid();
   const int c = threadIdx.x & ((1 << p.chunk_log2) - 1), w = (chunk << p.chunk_log2) + c;
   const int valid = p.Nk - 32 * w;
@@ -86,8 +91,13 @@ __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_c
     }
   }
   __syncthreads();
-  if (any != 0u) atomicOr(&live[(c >> p.tile_log2) >> 5], 1u << ((c >> p.tile_log2) & 31));
+  if (any != 0u) {
+    atomicOr(&live[(c >> p.tile_log2) >> 5], 1u << ((c >> p.tile_log2) & 31));
+    atomicOr(&kept[c], any);
+  }
   __syncthreads();
+  if (threadIdx.x < (1 << p.chunk_log2) && w < p.W)
+    p.kept[((b * p.Hb + hblk) * p.QT + qt) * p.W + w] = kept[c];
   // Bytes of live bits of a chunk (a row in one chunk may have fewer than 8 tiles, and writes all of its words).
   const int bytes = p.chunks == 1 ? p.occ_words * 4 : 1 << (p.chunk_log2 - p.tile_log2 - 3);
   const int k = chunk * bytes + threadIdx.x;
@@ -351,9 +361,10 @@ Geo tile_geometry(const CrossParams& p, bool shared_keys) {
   return x;
 }
 
-// The packed mask of p: its words, and behind them the live-tile bits.
+// The packed mask of p: its words, the kept keys of every tile, and the
+// live-tile bits, one behind the other.
 struct PackLayout {
-  int64_t words;         // their number
+  int64_t words, kept;   // numbers of words
   int64_t Bm, Hm, Qm;    // lengths of the axes the mask has, 1 for the others
   int64_t Hb, QT;        // head blocks and query tiles it has
   int64_t occ_words;
@@ -366,6 +377,7 @@ PackLayout pack_layout(const CrossParams& p, const Geo& x) {
   l.words = l.Bm * l.Hm * l.Qm * ((p.Nk + 127) / 128 * 4);
   l.Hb = p.word_stride[1] != 0 ? p.H / x.hb : 1;
   l.QT = p.word_stride[2] != 0 ? (p.Nq + kBM - 1) / kBM : 1;
+  l.kept = l.Bm * l.Hb * l.QT * ((p.Nk + 127) / 128 * 4);
   const int64_t bn = p.D == 64 ? 128 : 64;
   l.occ_words = ((p.Nk + bn - 1) / bn + 31) / 32;
   return l;
@@ -381,7 +393,8 @@ int launch_pack(const CrossParams& p, const char** msg) {
   k.sq = p.mask_stride[2];
   k.hi = p.mask + (l.Bm - 1) * k.sb + (l.Hm - 1) * k.sh + (l.Qm - 1) * k.sq + p.Nk;
   k.words = p.words;
-  k.occ = reinterpret_cast<uint8_t*>(p.words + l.words);
+  k.kept = p.words + l.words;
+  k.occ = reinterpret_cast<uint8_t*>(p.words + l.words + l.kept);
   k.Hm = static_cast<int>(l.Hm);
   k.Qm = static_cast<int>(l.Qm);
   k.Nk = static_cast<int>(p.Nk);
@@ -429,16 +442,16 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool 
   if (!keys.shared) {
     x.words = p.words;
     for (int i = 0; i < 3; ++i) x.word_stride[i] = p.word_stride[i];
-    x.row_shared = p.words != nullptr && (x.Nq == 1 || p.word_stride[2] == 0) && (x.hb == 1 || p.word_stride[1] == 0);
     if (p.words != nullptr) {
+      const int64_t W = (p.Nk + 127) / 128 * 4;
       const PackLayout l = pack_layout(p, x);
-      x.occ = p.words + l.words;
-      int64_t step = l.occ_words;
-      x.occ_stride[2] = p.word_stride[2] != 0 ? step : 0;
-      step *= l.QT;
-      x.occ_stride[1] = p.word_stride[1] != 0 ? step : 0;
-      step *= l.Hb;
-      x.occ_stride[0] = p.word_stride[0] != 0 ? step : 0;
+      x.kept = p.words + l.words;
+      x.occ = p.words + l.words + l.kept;
+      const int64_t tiles[3] = {l.QT * l.Hb, l.QT, 1};
+      for (int i = 0; i < 3; ++i) {
+        x.occ_stride[i] = p.word_stride[i] != 0 ? tiles[i] * l.occ_words : 0;
+        x.kept_stride[i] = p.word_stride[i] != 0 ? tiles[i] * W : 0;
+      }
     }
     x.lengths = p.lengths;
   }

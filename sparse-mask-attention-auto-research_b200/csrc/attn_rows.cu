@@ -629,6 +629,10 @@ int launch(const CrossParams& a, const char** msg) {
   p.RT = (p.R + kRows - 1) / kRows;
   p.mask_rows = a.mask != nullptr && (a.Nq == 1 || a.mask_stride[2] == 0) && (p.G == 1 || a.mask_stride[1] == 0) ? 1 : 0;
   p.scale_log2 = a.scale * kLog2e;
+  if (a.H / a.Hkv * a.Nq > 0x7FFFFFFFll - kRows) {
+    *msg = "attention: too many query rows";
+    return kErrArg;
+  }
   const int64_t items = a.B * a.Hkv * p.RT;
   constexpr int kChunk = C::kChunk;
   const int64_t chunks = (a.P + kChunk - 1) / kChunk + (a.Nk + kChunk - 1) / kChunk;

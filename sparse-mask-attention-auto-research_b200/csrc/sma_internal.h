@@ -117,8 +117,8 @@ struct CrossParams {
   void* out;                  // [B, H, Nq, D] contiguous
   float* lse;                 // [B, H, Nq] or nullptr
   // attn_fwd_cross.cu and attn_bwd_cross.cu: the packed mask ([.., W] words with
-  // strides {batch, head, query}, 0: broadcast, and behind them the live-tile
-  // bits; nullptr keeps every key), the
+  // strides {batch, head, query}, 0: broadcast, and behind them the kept keys
+  // and the live-tile bits of every tile; nullptr keeps every key), the
   // bias by relative position, [H][bias_hi - bias_lo + 1 + 2 kBiasPad], and
   // O minus its rounded value, in the inputs' type (nullptr: not wanted).
   uint32_t* words;

@@ -306,7 +306,8 @@ def _saved_layout(q, k, mask_strides, bias, training):
                 rows *= n
                 tiles *= (n + per - 1) // per
         Nk = k.shape[2]
-        end += rows * ((Nk + 127) // 128 * 16) + (tiles * ((Nk + 2047) // 2048) * 4 + 15) // 16 * 16
+        W = (Nk + 127) // 128 * 4
+        end += (rows + tiles) * W * 4 + (tiles * ((Nk + 2047) // 2048) * 4 + 15) // 16 * 16
     if bias is not None:
         distance = end
         n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 513

@@ -247,3 +247,20 @@ def test_results_do_not_change_from_run_to_run():
     want = cross_attention(q, k, v)
     for _ in range(20):
         assert torch.equal(cross_attention(q, k, v), want)
+
+
+@pytest.mark.parametrize("Nq,D", [(3, 64), (100, 64), (300, 128)])
+def test_keys_that_no_row_keeps_may_hold_anything(Nq, D):
+    """Masks with rows of their own (causal and padded, say): keys that no
+    query keeps may be infinite or NaN."""
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    q = heads(gen, 2, 2, Nq, D, BF16)
+    k, v = (heads(gen, 2, 2, 400, D, BF16) for _ in range(2))
+    m = torch.rand(2, 2, Nq, 400, generator=gen, device=DEV) < 0.5
+    m[0, ..., 333:] = False
+    m[1, ..., :130] = False
+    m[1, 0, :, 200] = False
+    want = cross_attention(q, k, v, m)
+    gone = ~m.any(2)[..., None]
+    got = cross_attention(q, k.masked_fill(gone, float("nan")), v.masked_fill(gone, float("-inf")), m)
+    assert torch.equal(got, want)

@@ -241,3 +241,33 @@ def test_too_many_query_tiles_are_refused():
     k = torch.empty(1, 1, 8, 64, device=DEV).half()
     with pytest.raises(RuntimeError, match="2048"):
         cross_attention(q, k, k)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("Nq,D", [(5, 64), (200, 64), (130, 128)])
+def test_padding_may_hold_anything(Nq, D, bias):
+    """Keys and values behind a padding mask may be infinite or NaN: their
+    gradients are 0 and nothing else changes."""
+    gen = torch.Generator(device=DEV).manual_seed(25)
+    q, dout = heads(gen, 2, 4, Nq, D, BF16), heads(gen, 2, 4, Nq, D, BF16)
+    k, v = (heads(gen, 2, 2, 300, D, BF16) for _ in range(2))
+    table = torch.randn(32, 4, generator=gen, device=DEV).bfloat16()
+    m = torch.zeros(2, 1, 1, 300, dtype=torch.bool, device=DEV)
+    m[0, ..., :133] = True
+    m[1, ..., 7:290] = True
+    gone = ~m.view(2, 1, 300, 1)
+
+    def run(k, v):
+        leaves = [t.clone().requires_grad_(True) for t in ((q, k, v, table) if bias else (q, k, v))]
+        out = relative_bias_attention(*leaves, m) if bias else cross_attention(*leaves, m)
+        return out.detach(), torch.autograd.grad(out, leaves, dout)
+
+    out0, want = run(k, v)
+    out1, got = run(k.masked_fill(gone, float("nan")), v.masked_fill(gone, float("inf")))
+    assert torch.equal(out0, out1)
+    for i, (a, b) in enumerate(zip(got, want)):
+        if i == 0:  # dq: FP32 adds in another order
+            assert torch.allclose(a.float(), b.float(), rtol=2.0**-7, atol=1e-4)
+        else:
+            assert torch.equal(a, b)
+    assert torch.all(got[1].masked_select(gone.expand_as(k)) == 0) and torch.all(got[2].masked_select(gone.expand_as(v)) == 0)
