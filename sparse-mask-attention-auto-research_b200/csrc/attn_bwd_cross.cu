@@ -12,7 +12,11 @@
 // bias, bias_reduce_kernel.
 //
 // cross_bwd_kernel is persistent, one CTA per SM, over items (batch, key head,
-// 128-key tile).  K and V of the item stay in shared memory, dK and dV
+// 128-key tile), handed out as CTAs come free (masks leave items of very
+// different length).  The last ones, which would not fill a round of the SMs,
+// are cut along their query steps into parts that do; the parts leave dK and dV
+// in FP32, which cross_dq_kernel adds in order, so that dK and dV do not depend
+// on which CTA did what.  K and V of the item stay in shared memory, dK and dV
 // accumulate in TMEM over all query heads that share the key head, and the CTA
 // walks the item's live steps of 64 query rows (those whose mask block keeps
 // a pair).  Two steps are in flight, each with its own S^T / dP^T columns and
@@ -69,11 +73,14 @@ constexpr int kThreads = 16 * 32;  // warp 15 only fills its warpgroup
 constexpr int kRegsOther = 112;
 constexpr int kRegsEw = 144;
 static_assert(256 * (kRegsOther + kRegsEw) <= kThreads * 128, "register split");
-// Items whose live lists the scanner publishes ahead, and words of a list: one
-// bit per step, up to 2048 steps of the heads that share a key head.
-constexpr int kSlots = 4;
+// Items whose live lists the scanner claims and publishes ahead (no more than
+// the one being worked on and the next, since a claimed item waits for its
+// CTA), and words of a list: one bit per step, up to 2048 steps of the heads
+// that share a key head.
+constexpr int kSlots = 2;
 constexpr int kListWords = 64;
 constexpr int kMaxSteps = 32 * kListWords;
+constexpr int kMaxParts = 8;  // of an item
 
 // TMEM columns: S^T of stage g, dP^T of stage g, dV, dK, and for D = 64 two dQ buffers.
 __host__ __device__ constexpr uint32_t col_s(int g) { return 64u * g; }
@@ -116,6 +123,7 @@ struct Ctl {
   uint64_t drain;
   uint32_t live_bits[kSlots][kListWords];
   uint32_t n_live[kSlots];
+  int unit[kSlots];                // which item or part, -1: no more
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
@@ -154,11 +162,26 @@ struct BwdGeo {
   // Its gradient by relative position: dS summed along the diagonals of every
   // 32 x 32 block that overlaps (bias_lo, bias_hi), [B*H][KB][slots][64]
   // (entry d - 32 (kb - qb) + off, mod 64), and the sums of the blocks beyond
-  // on either side, [B*H][KB][2 (stage)][2 (low, high)].
+  // on either side, [B*H][KB][kMaxParts * 2 (stage)][2 (low, high)].
   float* near_part;
   float* far_part;
   int KB, QB, slots, slot_by_query;
+  // Units of work: `whole` items, then `cut` items in `parts` parts each, whose
+  // dV and dK [cut * parts][128 keys][2 D] FP32 go to part_acc.  CTA c starts
+  // with unit c; the others go to whoever asks next (`next`, cleared before).
+  int grid, whole, cut, parts;
+  int tile_major;          // items by key tile, then (batch, key head), instead of the other way round
+  float* part_acc;
+  int* next;
 };
+
+// (batch, key head) and key tile of item w.
+__device__ __forceinline__ void item_place(const BwdGeo& x, int KT, int w, int& bh, int& kt) {
+  const int fast = x.tile_major ? x.B * x.Hkv : KT;
+  const int slow = w / fast;
+  kt = x.tile_major ? slow : w - slow * fast;
+  bh = x.tile_major ? w - slow * fast : slow;
+}
 
 // Block difference j = kb - qb of the 32 x 32 blocks that overlap (lo, hi):
 // their relative positions are 32 j - off + [-31, 31].  The largest such j.
@@ -259,6 +282,7 @@ __global__ void __launch_bounds__(256)
     return;
   }
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (gid == 0) *x.next = 0;
   const int64_t row = gid / kPerRow;
   float acc = 0.f;
   if (row < rows) {
@@ -284,15 +308,43 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dq[i] = acc[i] in the input dtype, 8 elements per thread.
-template <bool BF16>
-__global__ void __launch_bounds__(256) cross_dq_kernel(const float4* __restrict__ acc, uint4* __restrict__ dq, int64_t n8) {
+// Blocks below `dq_blocks`: dq[i] = acc[i] in the input dtype, 8 elements per
+// thread.  The others: dV and dK of the items cut in parts, the parts added in
+// order, 8 elements per thread.  Bound by HBM.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256)
+    cross_dq_kernel(const float4* __restrict__ acc, uint4* __restrict__ dq, int64_t n8, unsigned dq_blocks,
+                    uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int KT, const __grid_constant__ BwdGeo x) {
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n8) return;
-  const float4 a = __ldcs(acc + 2 * i), b = __ldcs(acc + 2 * i + 1);
-  dq[i] = make_uint4(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w), pack2<BF16>(b.x, b.y), pack2<BF16>(b.z, b.w));
+  if (blockIdx.x < dq_blocks) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= n8) return;
+    const float4 a = __ldcs(acc + 2 * i), b = __ldcs(acc + 2 * i + 1);
+    dq[i] = make_uint4(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w), pack2<BF16>(b.x, b.y), pack2<BF16>(b.z, b.w));
+    return;
+  }
+  constexpr int kPerRow = 2 * D / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x - dq_blocks) * 256 + threadIdx.x;
+  const int64_t row = i / kPerRow;
+  const int c = static_cast<int>(i - row * kPerRow);
+  const int item = static_cast<int>(row / kKeys), t = static_cast<int>(row - static_cast<int64_t>(item) * kKeys);
+  if (item >= x.cut) return;
+  int bh, kt;
+  item_place(x, KT, x.whole + item, bh, kt);
+  const int key = kt * kKeys + t;
+  if (key >= x.Nk) return;
+  float sum[8] = {};
+  for (int part = 0; part < x.parts; ++part) {
+    const float4* src = reinterpret_cast<const float4*>(
+        x.part_acc + ((static_cast<int64_t>(item) * x.parts + part) * kKeys + t) * (2 * D) + c * 8);
+    const float4 a = __ldcs(src), b = __ldcs(src + 1);
+    sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w;
+    sum[4] += b.x, sum[5] += b.y, sum[6] += b.z, sum[7] += b.w;
+  }
+  uint16_t* dst = (c < D / 8 ? dv : dk) + (static_cast<int64_t>(bh) * x.Nk + key) * D + (c < D / 8 ? c : c - D / 8) * 8;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<BF16>(sum[0], sum[1]), pack2<BF16>(sum[2], sum[3]),
+                                              pack2<BF16>(sum[4], sum[5]), pack2<BF16>(sum[6], sum[7]));
 }
 
 // Sums of a 32 x 32 block along its diagonals.  ds[e] is lane t's element of
@@ -328,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                      const __grid_constant__ CUtensorMap tm_dq, const float* __restrict__ neg_lse2,
                      const float* __restrict__ neg_delta, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int KT,
-                     int total_items, float scale, const __grid_constant__ BwdGeo x, uint32_t* err_word,
+                     float scale, const __grid_constant__ BwdGeo x, uint32_t* err_word,
                      uint64_t timeout_ns) {
   using C = Cfg<D>;
   constexpr int kRing = C::kRing;
@@ -345,14 +397,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* s_lse = reinterpret_cast<float*>(smem + C::kOffLse);
   float* s_delta = reinterpret_cast<float*>(smem + C::kOffDelta);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // CTA c takes items c, c + G, ...: the CTAs running at one time share the
-  // Q and dO of a few heads in L2.  Counters over all items of the CTA, the
-  // same in every role: j items (list slot j % kSlots), li items with a live
-  // step (K/V buffer li % kKVBufs), lt live steps (ring slot lt % kRing), the
-  // uses of each stage (step t of an item uses stage t & 1) and lp pairs of
-  // steps of one item (D = 64: dQ buffer lp & 1).
-  const int G = static_cast<int>(gridDim.x);
-  const int n_items = (total_items - static_cast<int>(blockIdx.x) + G - 1) / G;
+  // Counters over all units of the CTA, the same in every role: j units (list
+  // slot j % kSlots), li units with a live step (K/V buffer li % kKVBufs), lt
+  // live steps (ring slot lt % kRing), the uses of each stage (step t of a unit
+  // uses stage t & 1) and lp pairs of steps of one unit (D = 64: dQ buffer
+  // lp & 1).
+  const int units = x.whole + x.cut * x.parts;
   const int VT = x.gh * x.QT1;
   volatile uint32_t* abort_flag = &ctl.abort_flag;
 
@@ -400,15 +450,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     ctl.abort_flag = 1;
     atomicOr(err_word, kDevErrTimeout);
   };
-  // Batch, key head and key tile of item j, and the first head of the group.
+  // Batch, key head and key tile of a unit, and the first head of the group.
   struct Item {
     int b, hkv, kt, h0;
+    int part;  // -1: a whole item
   };
-  auto item_at = [&](int j) -> Item {
-    const int w = static_cast<int>(blockIdx.x) + j * G;
-    const int bh = w / KT;
+  auto item_of = [&](int unit) -> Item {
     Item it;
-    it.kt = w - bh * KT;
+    int w = unit;
+    it.part = -1;
+    if (unit >= x.whole) {
+      const int i = (unit - x.whole) / x.parts;
+      it.part = unit - x.whole - i * x.parts;
+      w = x.whole + i;
+    }
+    int bh;
+    item_place(x, KT, w, bh, it.kt);
     it.b = bh / x.Hkv;
     it.hkv = bh - it.b * x.Hkv;
     it.h0 = it.hkv * (x.gh * x.hb);
@@ -507,15 +564,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++lt;
       return true;
     };
-    for (int j = 0; ok && j < n_items; ++j) {
+    for (int j = 0; ok; ++j) {
       const int sl = j % kSlots;
       if (!wait_all(ctl.item_full[sl], (j / kSlots) & 1)) {
         ok = false;
         break;
       }
+      if (ctl.unit[sl] < 0) break;
       const int n = static_cast<int>(ctl.n_live[sl]);
       if (n > 0) {
-        const Item it = item_at(j);
+        const Item it = item_of(ctl.unit[sl]);
         ok = issue_kv(it);
         int cw = 0;
         uint32_t cx = ctl.live_bits[sl][0];
@@ -609,12 +667,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (pend.kv_free >= 0) mma_commit_warp(smem_u32(&ctl.kv_free[pend.kv_free]));
         return true;
       };
-      for (int j = 0; ok && j < n_items; ++j) {
+      for (int j = 0; ok; ++j) {
         const int sl = j % kSlots;
         if (!wait_all(ctl.item_full[sl], (j / kSlots) & 1)) {
           ok = false;
           break;
         }
+        if (ctl.unit[sl] < 0) break;
         const int n = static_cast<int>(ctl.n_live[sl]);
         if (n > 0) {
           const int kv = li % C::kKVBufs;
@@ -677,12 +736,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // next item's first S^T, if that item has a live step; its list
           // needs nothing of this item.
           bool keep = false;
-          if (C::kKVBufs == 2 && j + 1 < n_items) {
-            if (!wait_all(ctl.item_full[(j + 1) % kSlots], ((j + 1) / kSlots) & 1)) {
+          if (C::kKVBufs == 2) {
+            const int sl1 = (j + 1) % kSlots;
+            if (!wait_all(ctl.item_full[sl1], ((j + 1) / kSlots) & 1)) {
               ok = false;
               break;
             }
-            keep = ctl.n_live[(j + 1) % kSlots] > 0u;
+            keep = ctl.unit[sl1] >= 0 && ctl.n_live[sl1] > 0u;
           }
           if (!keep && !flush()) {
             ok = false;
@@ -705,13 +765,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Item j's live list: bit v set when some query row of step v keeps a key
     // of the item's tile; a lane looks at one step of 32.
     bool ok = true;
-    for (int j = 0; j < n_items; ++j) {
+    for (int j = 0;; ++j) {
       const int sl = j % kSlots;
       if (j >= kSlots && !wait_all(ctl.item_free[sl], ((j / kSlots) - 1) & 1)) {
         ok = false;
         break;
       }
-      const Item it = item_at(j);
+      int unit = static_cast<int>(blockIdx.x);
+      if (j > 0) {
+        if (lane == 0) unit = x.grid + atomicAdd(x.next, 1);
+        unit = __shfl_sync(0xffffffffu, unit, 0);
+      }
+      if (unit >= units) {
+        if (lane == 0) {
+          ctl.unit[sl] = -1;
+          mbar_arrive(smem_u32(&ctl.item_full[sl]));
+        }
+        break;
+      }
+      const Item it = item_of(unit);
       uint32_t mine[2] = {0u, 0u};  // words lane and lane + 32 of the list
       if (x.words_t == nullptr) {
         // No mask, or one mask row for the whole item: all steps or none.
@@ -745,10 +817,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (it.part >= 0) {
+        // The part's share of the n live steps, by rank: [part n / parts, (part + 1) n / parts).
+        int before[2], all = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int incl = __popc(mine[h]);
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+          }
+          before[h] = all + incl - __popc(mine[h]);
+          all += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        const int lo = all * it.part / x.parts, hi = all * (it.part + 1) / x.parts;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int from = max(lo - before[h], 0), to = min(hi - before[h], __popc(mine[h]));
+          uint32_t left = mine[h], keep = 0u;
+          for (int i = 0; i < to; ++i) {
+            const uint32_t low = left & (0u - left);
+            if (i >= from) keep |= low;
+            left ^= low;
+          }
+          mine[h] = keep;
+        }
+      }
       ctl.live_bits[sl][lane] = mine[0];
       ctl.live_bits[sl][lane + 32] = mine[1];
       const int n = __reduce_add_sync(0xffffffffu, __popc(mine[0]) + __popc(mine[1]));
-      if (lane == 0) ctl.n_live[sl] = static_cast<uint32_t>(n);
+      if (lane == 0) {
+        ctl.n_live[sl] = static_cast<uint32_t>(n);
+        ctl.unit[sl] = unit;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_full[sl]));
     }
@@ -779,12 +881,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto fetch_words = [&](const Item& it, int v) {
       return x.words_t != nullptr ? __ldg(step_words(it, v) + t) : item_bit(it);
     };
-    for (int j = 0; ok && j < n_items; ++j) {
+    for (int j = 0; ok; ++j) {
       const int sl = j % kSlots;
       ok = wait_all(ctl.item_full[sl], (j / kSlots) & 1);
-      if (!ok) break;
+      if (!ok || ctl.unit[sl] < 0) break;
       const int n = static_cast<int>(ctl.n_live[sl]);
-      const Item it = item_at(j);
+      const Item it = item_of(ctl.unit[sl]);
       int cw = 0;
       uint32_t cx = ctl.live_bits[sl][0];
       if (g == 1) next_live(ctl.live_bits[sl], cw, cx);
@@ -826,7 +928,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             far_hi += __shfl_xor_sync(0xffffffffu, far_hi, o);
           }
           if (lane == 0) {
-            float* dst = x.far_part + (((static_cast<int64_t>(it.b) * x.H + far_head) * x.KB + key0 / 32) * 2 + g) * 2;
+            float* dst = x.far_part + (((static_cast<int64_t>(it.b) * x.H + far_head) * x.KB + key0 / 32) * (2 * kMaxParts) +
+                                       2 * max(it.part, 0) + g) * 2;
             dst[0] = far_lo;
             dst[1] = far_hi;
           }
@@ -870,16 +973,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           next_live(ctl.live_bits[sl], cw, cx);  // the other stage's
           v_next = next_live(ctl.live_bits[sl], cw, cx);
           if (x.words_t != nullptr) next_words = fetch_words(it, v_next);
-        } else if (j + 1 < n_items) {
+        } else {
           const int sl1 = (j + 1) % kSlots;
           ok = wait_all(ctl.item_full[sl1], ((j + 1) / kSlots) & 1);
           if (!ok) break;
-          if (static_cast<int>(ctl.n_live[sl1]) > g) {
+          if (ctl.unit[sl1] >= 0 && static_cast<int>(ctl.n_live[sl1]) > g) {
             int w1 = 0;
             uint32_t x1 = ctl.live_bits[sl1][0];
             if (g == 1) next_live(ctl.live_bits[sl1], w1, x1);
             const int v1 = next_live(ctl.live_bits[sl1], w1, x1);
-            next_words = fetch_words(item_at(j + 1), v1);
+            next_words = fetch_words(item_of(ctl.unit[sl1]), v1);
             have_words = true;
           }
         }
@@ -1029,11 +1132,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) bulk_wait_group_read0();
       __syncwarp();
     };
-    for (int j = 0; ok && j < n_items; ++j) {
+    for (int j = 0; ok; ++j) {
       const int sl = j % kSlots;
       ok = wait_all(ctl.item_full[sl], (j / kSlots) & 1);
-      if (!ok) break;
-      const Item it = item_at(j);
+      if (!ok || ctl.unit[sl] < 0) break;
+      const int unit = ctl.unit[sl];
+      const Item it = item_of(unit);
       const int block0 = (it.b * x.Hkv + it.hkv) * x.gh;
       const int n = static_cast<int>(ctl.n_live[sl]);
       // dV and dK of this key tile (lane t = key), once the item's last products
@@ -1058,7 +1162,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 4; ++q)
             reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
         };
-        if constexpr (D == 64) {
+        if (it.part >= 0) {
+          float* dst = x.part_acc + (static_cast<int64_t>(unit - x.whole) * kKeys + t) * (2 * D);
+#pragma unroll 1
+          for (int h = 0; h < 2 * D / 32; ++h) {  // dV, then dK
+            const float mul = h < D / 32 ? 1.f : scale;
+            float u[32] = {};
+            if (n > 0) {
+              tmem_ld32f(t_lane + kColDV + h * 32, u);
+              tmem_wait_ld();
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              reinterpret_cast<float4*>(dst + h * 32)[q] =
+                  make_float4(u[4 * q] * mul, u[4 * q + 1] * mul, u[4 * q + 2] * mul, u[4 * q + 3] * mul);
+          }
+          if (n > 0) arrive_warp(ctl.acc_free);
+        } else if constexpr (D == 64) {
           uint32_t w[4][16] = {};
           if (n > 0) {
 #pragma unroll
@@ -1227,8 +1347,8 @@ __global__ void __launch_bounds__(kReduceThreads)
     const bool low_end = !high && i == s.side - 1;
     const bool high_end = s.two_sided ? high && i == s.side - 1 : i == 0;
     if (low_end || high_end) {
-      const float* far_bh = x.far_part + (static_cast<int64_t>(b) * x.H + h) * x.KB * 4;
-      for (int w = 2 * kb0 + lane; w < 2 * kb1; w += 32) {
+      const float* far_bh = x.far_part + (static_cast<int64_t>(b) * x.H + h) * x.KB * (4 * kMaxParts);
+      for (int w = 2 * kMaxParts * kb0 + lane; w < 2 * kMaxParts * kb1; w += 32) {
         if (low_end) acc += __ldg(far_bh + 2 * w);
         if (high_end) acc += __ldg(far_bh + 2 * w + 1);
       }
@@ -1247,7 +1367,8 @@ __global__ void __launch_bounds__(kReduceThreads)
 }
 
 // Fills the geometry; false when the steps of a key head exceed the list.
-bool geometry(const CrossParams& p, BwdGeo* x) {
+bool geometry(const CrossParams& p, const DeviceProps& dp, BwdGeo* x) {
+  const int sms = dp.sms;
   const int G = static_cast<int>(p.H / p.Hkv);
   x->B = static_cast<int>(p.B);
   x->H = static_cast<int>(p.H);
@@ -1288,14 +1409,31 @@ bool geometry(const CrossParams& p, BwdGeo* x) {
     x->slot_by_query = slots > x->QB ? 1 : 0;
     x->slots = std::min(slots, x->QB);
   }
-  return static_cast<int64_t>(x->gh) * x->QT1 <= kMaxSteps;
+  // Whole rounds of items, and the rest in parts that make up most of a round,
+  // of 4 steps or more: a part costs some steps in itself (start, read-out and
+  // the final sum).
+  const int64_t items = p.B * p.Hkv * ((p.Nk + kKeys - 1) / kKeys), steps = static_cast<int64_t>(x->gh) * x->QT1;
+  x->cut = static_cast<int>(items % sms);
+  x->parts = x->cut > 0 ? static_cast<int>(std::max<int64_t>(
+                              1, std::min<int64_t>({sms / x->cut, int64_t{kMaxParts}, steps / 4})))
+                        : 1;
+  if (x->parts == 1) x->cut = 0;
+  // By key tile where Q, dO and the dQ accumulator of all heads stay in L2
+  // meanwhile: under a causal mask the items with the most steps come first
+  // and the shortest last (B4 H16 N1024 D64 with a bias: 81 us, by head 93).
+  // Else by head, whose
+  // Q and dO the CTAs then share at one time.
+  x->tile_major = 8 * p.B * p.H * p.Nq * p.D <= dp.l2_bytes / 2 ? 1 : 0;
+  x->whole = static_cast<int>(items - x->cut);
+  x->grid = static_cast<int>(std::min<int64_t>(sms, x->whole + int64_t{x->cut} * x->parts));
+  return steps <= kMaxSteps;
 }
 
 // Offsets, in floats, within the scratch of a backward: the FP32 accumulator of
 // dq at 0, -Delta and -lse2, the mask by key and its live bytes, partial sums of
-// the bias gradient.
+// the bias gradient, dV and dK of parts of items, the next unit.
 struct Scratch {
-  int64_t delta, words, live, bias, end;
+  int64_t delta, words, live, bias, parts, next, end;
 };
 Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
@@ -1307,12 +1445,14 @@ Scratch scratch_layout(const CrossParams& p, const BwdGeo& x) {
   const int64_t masked = Bm * Hm * x.QT1 * x.t_stride[2];  // 0 where the mask is not by key
   s.live = s.words + 2 * masked;
   s.bias = s.live + up(masked / kKeys);
-  s.end = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4) : 0);  // a multiple of 4
+  s.parts = s.bias + (p.bias.table != nullptr ? p.B * p.H * x.KB * (int64_t{64} * x.slots + 4 * kMaxParts) : 0);
+  s.next = s.parts + int64_t{x.cut} * x.parts * kKeys * 2 * p.D;
+  s.end = s.next + 4;
   return s;
 }
 
 template <int D, bool BF16, bool kBias>
-int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg) {
+int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, int device, const char** msg) {
   using C = Cfg<D>;
   constexpr size_t kSmemBytes = smem_bytes<D>();
   const int64_t KT = (p.Nk + kKeys - 1) / kKeys;
@@ -1336,11 +1476,9 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
     *msg = tensor_map_error("backward", rc);
     return kErrCuda;
   }
-  DeviceProps dp;
-  if (!device_props(&dp, msg)) return kErrCuda;
   static std::atomic<bool> smem_set[kMaxDevices] = {};
   auto kern = cross_bwd_kernel<D, BF16, kBias>;
-  cudaError_t e = ensure_smem_limit(kern, kSmemBytes, dp.device, smem_set);
+  cudaError_t e = ensure_smem_limit(kern, kSmemBytes, device, smem_set);
   const Scratch at = scratch_layout(p, x);
   float* neg_delta = g.scratch + at.delta;
   float4* dq_accum = reinterpret_cast<float4*>(g.scratch);
@@ -1348,7 +1486,9 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
     x.near_part = g.scratch + at.bias;
     x.far_part = x.near_part + p.B * p.H * x.KB * x.slots * 64;
   }
-  const int64_t zeros = (at.end - at.bias) / 4;
+  x.part_acc = g.scratch + at.parts;
+  x.next = reinterpret_cast<int*>(g.scratch + at.next);
+  const int64_t zeros = (at.parts - at.bias) / 4;
   const int64_t zero_blocks = (zeros + 256 * kZeroRounds - 1) / (256 * kZeroRounds);
   Transpose tr{};
   if (x.t_stride[2] != 0) {
@@ -1371,12 +1511,14 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
                    static_cast<unsigned>(row_blocks), reinterpret_cast<float4*>(g.scratch + at.bias), zeros,
                    static_cast<unsigned>(zero_blocks), tr, x);
   if (e == cudaSuccess)
-    e = launch_pdl(kern, static_cast<unsigned>(std::min<int64_t>(items, dp.sms)), kThreads, kSmemBytes, p.stream, mq, mk,
+    e = launch_pdl(kern, static_cast<unsigned>(x.grid), kThreads, kSmemBytes, p.stream, mq, mk,
                    mv, mdo, mdq, neg_delta + rows, neg_delta, static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv),
-                   static_cast<int>(KT), static_cast<int>(items), p.scale, x, p.err_word, p.timeout_ns);
+                   static_cast<int>(KT), p.scale, x, p.err_word, p.timeout_ns);
+  const int64_t part_blocks = (int64_t{x.cut} * kKeys * (2 * D / 8) + 255) / 256;
   if (e == cudaSuccess)
-    e = launch_pdl(cross_dq_kernel<BF16>, static_cast<unsigned>(row_blocks), 256, 0, p.stream,
-                   dq_accum, static_cast<uint4*>(g.dq), rows * D / 8);
+    e = launch_pdl(cross_dq_kernel<D, BF16>, static_cast<unsigned>(row_blocks + part_blocks), 256, 0, p.stream, dq_accum,
+                   static_cast<uint4*>(g.dq), rows * D / 8, static_cast<unsigned>(row_blocks),
+                   static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv), static_cast<int>(KT), x);
   if (e == cudaSuccess && kBias) {
     const dim3 grid(static_cast<unsigned>(p.H), static_cast<unsigned>(p.bias.side * (p.bias.two_sided ? 2 : 1)));
     bias_reduce_kernel<BF16><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, g.dtable);
@@ -1390,26 +1532,33 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, const char** msg
 }
 
 template <int D, bool BF16>
-int launch_b(const CrossParams& p, const CrossGrads& g, const BwdGeo& x, const char** msg) {
-  return p.bias.table != nullptr ? launch<D, BF16, true>(p, g, x, msg) : launch<D, BF16, false>(p, g, x, msg);
+int launch_b(const CrossParams& p, const CrossGrads& g, const BwdGeo& x, int device, const char** msg) {
+  return p.bias.table != nullptr ? launch<D, BF16, true>(p, g, x, device, msg)
+                                 : launch<D, BF16, false>(p, g, x, device, msg);
 }
 
 }  // namespace
 
 int64_t cross_bwd_scratch_floats(const CrossParams& p) {
   BwdGeo x{};
-  geometry(p, &x);
+  DeviceProps dp;
+  const char* msg = nullptr;
+  if (!device_props(&dp, &msg)) return -1;
+  geometry(p, dp, &x);
   return scratch_layout(p, x).end;
 }
 
 int launch_attn_cross_bwd(const CrossParams& p, const CrossGrads& g, const char** msg) {
   BwdGeo x{};
-  if (!geometry(p, &x)) {
+  DeviceProps dp;
+  if (!device_props(&dp, msg)) return kErrCuda;
+  if (!geometry(p, dp, &x)) {
     *msg = "backward: more than 2048 steps of 64 query rows share a key head";
     return kErrUnsupportedN;
   }
-  if (p.D == 128) return p.dtype == 1 ? launch_b<128, true>(p, g, x, msg) : launch_b<128, false>(p, g, x, msg);
-  return p.dtype == 1 ? launch_b<64, true>(p, g, x, msg) : launch_b<64, false>(p, g, x, msg);
+  const int dev = dp.device;
+  if (p.D == 128) return p.dtype == 1 ? launch_b<128, true>(p, g, x, dev, msg) : launch_b<128, false>(p, g, x, dev, msg);
+  return p.dtype == 1 ? launch_b<64, true>(p, g, x, dev, msg) : launch_b<64, false>(p, g, x, dev, msg);
 }
 
 }  // namespace sma
