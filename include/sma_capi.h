@@ -202,7 +202,7 @@ SMA_API int sma_attn_bwd_noalloc(int dtype, const void* q, const void* k, const 
 #define SMA_MAX_BIAS_SIDE 128
 #define SMA_MAX_BIAS_DISTANCE 65536 /* largest last start, where bias_distance is used */
 /* Floats per head of bias_distance, `last` being the last bucket's start. */
-#define SMA_BIAS_DISTANCE_LEN(last, two_sided) (((two_sided) ? 2 : 1) * (int64_t)(last) + 1 + 512)
+#define SMA_BIAS_DISTANCE_LEN(last, two_sided) (16 * ((((two_sided) ? 2 : 1) * (int64_t)(last) + 516) / 4 + 1))
 typedef struct sma_attn_args {
   int32_t dtype;
   float scale;

@@ -155,10 +155,12 @@ struct BwdGeo {
   // And which 32-key words of a step keep a pair: 4 bytes (0 / 1) per key tile,
   // strides t_stride / 128 per tile.
   const uint32_t* live_t;
-  // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
+  // Bias in units of log2 by relative position, bias_len values a head
+  // (bias_stride in sma_internal.h).
   const float* bias;
   const int32_t* bias_offsets;
   int bias_offset, bias_lo, bias_hi, bias_len;
+  int64_t bias_stride;
   // Its gradient by relative position: dS summed along the diagonals of every
   // 32 x 32 block that overlaps (bias_lo, bias_hi), [B*H][KB][slots][64]
   // (entry d - 32 (kb - qb) + off, mod 64), and the sums of the blocks beyond
@@ -948,9 +950,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (head != far_head) {
             flush_far();
             far_head = head;
-            head_row = x.bias + static_cast<int64_t>(head) * x.bias_len;
+            head_row = x.bias + static_cast<int64_t>(head) * x.bias_stride;
             add_lo = __ldg(head_row);
-            add_hi = __ldg(head_row + x.bias_len - 1);
+            add_hi = __ldg(head_row + bias_at(x.bias_len - 1));
           }
         }
         // kBias: relative positions of the step's block c are d0 - 32 c + lane
@@ -962,9 +964,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kBias) {
           step_near = d0 + 31 > x.bias_lo && d0 - 63 < x.bias_hi;
           if (step_near) {
-            const float* src = head_row + (d0 - x.bias_lo + kBiasPad + lane);
+            const float* src = head_row + bias_at(d0 - x.bias_lo + kBiasPad + lane);
 #pragma unroll
-            for (int u = 0; u < 3; ++u) win[u] = __ldg(src + (u - 2) * 32);
+            for (int u = 0; u < 3; ++u) win[u] = __ldg(src + (u - 2) * (32 * 4));
           }
         }
         // The next step's words, a step ahead; at the last one those of the
@@ -1401,6 +1403,7 @@ bool geometry(const CrossParams& p, const DeviceProps& dp, BwdGeo* x) {
     x->bias_offset = p.bias.offset;
     bias_range(p.bias, &x->bias_lo, &x->bias_hi);
     x->bias_len = x->bias_hi - x->bias_lo + 1 + 2 * kBiasPad;
+    x->bias_stride = bias_stride(x->bias_len);
     x->KB = static_cast<int>((p.Nk + kKeys - 1) / kKeys * 4);
     x->QB = (x->Nq + 31) / 32;
     // Block differences that overlap (lo, hi): multiples of 32 in an open

@@ -185,10 +185,12 @@ struct Geo {
   const int32_t* lengths;
   int kv_shared;           // all batches read the keys of batch 0
   uint16_t* out_lo;        // O minus its rounded value, in the inputs' type, or nullptr
-  // Bias in units of log2 by relative position, [H][bias_len] (rel_bias.cuh).
+  // Bias in units of log2 by relative position, bias_len values a head
+  // (bias_stride in sma_internal.h).
   const float* bias;
   const int32_t* bias_offsets;
   int bias_offset, bias_lo, bias_hi, bias_len;
+  int64_t bias_stride;
 };
 struct NoGeo {};
 
@@ -1211,15 +1213,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s_mul = scale_log2, s_add = 0.f;
         if constexpr (kBias) {
           const int d0 = kt_cur * kBN - (it.q0 + xt) - bias_off;  // relative position of the tile's first key
-          const float* brow = x.bias + static_cast<int64_t>(it.h0 + xh) * x.bias_len;
+          const float* brow = x.bias + static_cast<int64_t>(it.h0 + xh) * x.bias_stride;
           if (__all_sync(0xffffffffu, d0 + kBN - 1 <= x.bias_lo)) {
             s_add = __ldg(brow);
           } else if (__all_sync(0xffffffffu, d0 >= x.bias_hi)) {
-            s_add = __ldg(brow + x.bias_len - 1);
+            s_add = __ldg(brow + bias_at(x.bias_len - 1));
           } else {
-            const float* b0 = brow + max(0, min(x.bias_len - kBN, d0 - x.bias_lo + kBiasPad));
+            const int p0 = max(0, min(x.bias_len - kBN, d0 - x.bias_lo + kBiasPad)), k = -p0 & 3;
+            const float4* b0 = reinterpret_cast<const float4*>(brow) + (p0 + k) + k;
+            const uint64_t sc2 = f2(scale_log2, scale_log2);
 #pragma unroll
-            for (int e = 0; e < kBN; ++e) s[e] = fmaf(s[e], scale_log2, __ldg(b0 + e));
+            for (int e = 0; e < kBN; e += 4) {
+              const float4 b = __ldg(b0 + e);
+              f2_split(fma2(f2(s[e], s[e + 1]), sc2, f2(b.x, b.y)), s[e], s[e + 1]);
+              f2_split(fma2(f2(s[e + 2], s[e + 3]), sc2, f2(b.z, b.w)), s[e + 2], s[e + 3]);
+            }
             s_mul = 1.f;
           }
         }

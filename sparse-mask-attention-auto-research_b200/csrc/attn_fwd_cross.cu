@@ -106,21 +106,33 @@ __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------- bias by relative position
-// out[h][i] = log2(e) * table[bucket(lo - kBiasPad + i)][h]: the attention
-// kernels read the bias of 128 consecutive keys from 128 consecutive floats.
+// Value i of head h is log2(e) * table[bucket(lo - kBiasPad + i)][h], laid out
+// as bias_stride (sma_internal.h) says: a row of the attention kernel reads the
+// bias of consecutive keys in vectors, at any start (B16 H12 N512 D64 with a
+// random mask, 32 buckets: 57 us, with a scalar load for every key 59).
 __global__ void __launch_bounds__(256)
-    bias_expand_kernel(const __grid_constant__ BiasSpec bias, int bf16, int lo, int len, float* __restrict__ out) {
+    bias_expand_kernel(const __grid_constant__ BiasSpec bias, int bf16, int lo, int len, int64_t stride,
+                       float* __restrict__ out) {
   __shared__ int starts[kMaxBiasSide];
+  __shared__ int bucket[260];   // of values 4 j0 - 3 .. 4 j0 + 256
+  __shared__ float value[260];
   for (int i = threadIdx.x; i < bias.side; i += 256) starts[i] = bias.starts[i];
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= len) return;
-  const int bucket = bias_bucket(bias, starts, lo - kBiasPad + i);
-  for (int h = blockIdx.y; h < bias.H; h += gridDim.y)
-    out[static_cast<int64_t>(h) * len + i] =
-        kLog2e * (bf16 ? bias_value<true>(bias, bucket, h) : bias_value<false>(bias, bucket, h));
+  const int j0 = blockIdx.x * 64;
+  for (int i = threadIdx.x; i < 260; i += 256)
+    bucket[i] = bias_bucket(bias, starts, lo - kBiasPad + max(0, min(len - 1, 4 * j0 - 3 + i)));
+  const int j = threadIdx.x >> 2, k = threadIdx.x & 3;
+  for (int h = blockIdx.y; h < bias.H; h += gridDim.y) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 260; i += 256)
+      value[i] = kLog2e * (bf16 ? bias_value<true>(bias, bucket[i], h) : bias_value<false>(bias, bucket[i], h));
+    __syncthreads();
+    const float* v = value + 4 * j + 3 - k;
+    if (16ll * (j0 + j) < stride)
+      reinterpret_cast<float4*>(out + h * stride)[4 * (j0 + j) + k] = make_float4(v[0], v[1], v[2], v[3]);
+  }
 }
 
 // ---------------------------------------------------------------- merge of a split launch
@@ -467,6 +479,7 @@ int launch_tiles(const CrossParams& p, const Keys& keys, bool with_prefix, bool 
     x.bias_offset = p.bias.offset;
     bias_range(p.bias, &x.bias_lo, &x.bias_hi);
     x.bias_len = x.bias_hi - x.bias_lo + 1 + 2 * kBiasPad;
+    x.bias_stride = bias_stride(x.bias_len);
   }
   const int64_t items = (p.B + x.nb - 1) / x.nb * p.Hkv * x.gh * ((p.Nq + kBM - 1) / kBM);
   const int pieces = choose_pieces(items, x.KTp + (keys.n + bn - 1) / bn, 2 * static_cast<int64_t>(dp.sms), partial);
@@ -493,8 +506,9 @@ int launch_bias_expand(const CrossParams& p, const char** msg) {
   int lo = 0, hi = 0;
   bias_range(p.bias, &lo, &hi);
   const int len = hi - lo + 1 + 2 * kBiasPad;
+  const int64_t stride = bias_stride(len);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((len + 255) / 256), static_cast<unsigned>(std::min<int64_t>(p.H, 1024)));
+  cfg.gridDim = dim3(static_cast<unsigned>((stride / 16 + 63) / 64), static_cast<unsigned>(std::min<int64_t>(p.H, 1024)));
   cfg.blockDim = dim3(256);
   cfg.stream = p.stream;
   cudaLaunchAttribute attr[1];
@@ -502,7 +516,7 @@ int launch_bias_expand(const CrossParams& p, const char** msg) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, bias_expand_kernel, p.bias, p.dtype, lo, len, p.bias_distance);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, bias_expand_kernel, p.bias, p.dtype, lo, len, stride, p.bias_distance);
   if (e != cudaSuccess) {
     *msg = cudaGetErrorString(e);
     return kErrLaunch;

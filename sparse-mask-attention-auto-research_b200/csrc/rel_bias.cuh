@@ -35,6 +35,10 @@ __device__ __forceinline__ int bias_bucket(const BiasSpec& s, const int* starts,
   return lo + ((s.two_sided && d > 0) ? s.side : 0);
 }
 
+// Where value i of a head's bias by relative position stands (bias_stride in
+// sma_internal.h).
+__device__ __forceinline__ int bias_at(int i) { return (i >> 2) * 16 + (i & 3); }
+
 template <bool BF16>
 __device__ __forceinline__ float bias_value(const BiasSpec& s, int bucket, int h) {
   const int64_t at = static_cast<int64_t>(bucket) * s.H + h;

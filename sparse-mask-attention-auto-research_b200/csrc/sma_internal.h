@@ -119,7 +119,7 @@ struct CrossParams {
   // attn_fwd_cross.cu and attn_bwd_cross.cu: the packed mask ([.., W] words with
   // strides {batch, head, query}, 0: broadcast, and behind them the kept keys
   // and the live-tile bits of every tile; nullptr keeps every key), the
-  // bias by relative position, [H][bias_hi - bias_lo + 1 + 2 kBiasPad], and
+  // bias by relative position, [H][bias_stride(length)], and
   // O minus its rounded value, in the inputs' type (nullptr: not wanted).
   uint32_t* words;
   int64_t word_stride[3];
@@ -143,9 +143,13 @@ inline void bias_range(const BiasSpec& s, int* lo, int* hi) {
   *lo = -s.starts[s.side - 1];
   *hi = s.two_sided ? s.starts[s.side - 1] : 0;
 }
-// Floats per head of the bias by relative position: lo .. hi and kBiasPad more
-// on either side, so that a tile which overlaps (lo, hi) never leaves it.
+// Length of the bias by relative position: lo .. hi and kBiasPad more on
+// either side, so that a tile which overlaps (lo, hi) never leaves it.
 constexpr int kBiasPad = 256;
+// It is kept four times, shifted by 0 .. 3 places, the copies interleaved by
+// 16 bytes: floats 16 j + 4 k .. + 3 are values 4 j - k .. + 3.  Any run of
+// values can so be read 16 bytes at a time, whatever its start.
+inline int64_t bias_stride(int len) { return 16 * ((static_cast<int64_t>(len) + 3) / 4 + 1); }  // floats per head
 
 // Fills p.bias_distance from p.bias.
 int launch_bias_expand(const CrossParams& p, const char** msg);

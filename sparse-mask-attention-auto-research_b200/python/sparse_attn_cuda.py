@@ -310,8 +310,8 @@ def _saved_layout(q, k, mask_strides, bias, training):
         end += (rows + tiles) * W * 4 + (tiles * ((Nk + 2047) // 2048) * 4 + 15) // 16 * 16
     if bias is not None:
         distance = end
-        n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 513
-        end += (H * n * 4 + 15) // 16 * 16
+        n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 516
+        end += H * 64 * (n // 4 + 1)
     if training:
         lse = end
         end += (B * H * Nq * 4 + 15) // 16 * 16
