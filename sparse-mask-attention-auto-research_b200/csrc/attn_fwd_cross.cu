@@ -21,7 +21,7 @@ namespace {
 // second time from L1).  Vectors that would reach outside the mask's own span
 // [lo, hi) are read byte by byte.
 // kAligned: every row starts on 16 bytes, so no word needs a third vector.  B16
-// H12 Nq512 Nk512, 50 MB of mask: 14.8 us, 3.4 TB/s (the general form: 19; two
+// H12 Nq512 Nk512, 50 MB of mask: 13.9 us, 3.6 TB/s (the general form: 19; two
 // words a thread in flight instead of four 2 us more, eight 4 us more).
 constexpr int kPackThreads = 256;
 constexpr int kPackWords = 256;   // words of a row per CTA, at most
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_c
     }
 #pragma unroll
     for (int u = 0; u < kPackRounds; ++u) {
-      uint32_t word = pack32_any(x[u][0], x[u][1]);
+      uint32_t word = bytes_are_01(x[u][0], x[u][1]) ? pack32_01(x[u][0], x[u][1]) : pack32_any(x[u][0], x[u][1]);
       if constexpr (!kAligned) {
         const int sh = static_cast<int>(reinterpret_cast<uintptr_t>(src[u]) & 15u);
         word = __funnelshift_r(word, pack16_any(x[u][2]), sh);
