@@ -1,4 +1,6 @@
-"""Build libsma.so (the C-ABI library with the sm_100a kernels) in-tree.
+"""Build libsma.so (the C-ABI library with the sm_100a kernels) and
+sma_torch.so (the PyTorch side of the operators on queries and keys of
+different lengths) in-tree.
 
 Usage:  python build.py [--verbose] [--ptxas-info]
 
@@ -6,7 +8,8 @@ Each csrc/*.cu is compiled with nvcc for sm_100a only into _build/, then
 linked into libsma.so next to this file.  The CUDA runtime is linked
 statically and the driver API (cuTensorMapEncodeTiled) is reached through
 cudaGetDriverEntryPoint, so the library loads without a GPU or libcuda and
-depends on nothing but the C/C++ runtime.
+depends on nothing but the C/C++ runtime.  sma_torch.so is host code, compiled
+against the installed PyTorch; it gets libsma.so's entry points at run time.
 """
 
 import argparse
@@ -15,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -22,6 +26,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(HERE, "_build")
 LIB_PATH = os.path.join(HERE, "libsma.so")
+OPS_PATH = os.path.join(HERE, "sma_torch.so")
 
 SOURCES = ["sma_capi.cu", "pack_mask.cu", "attn_fwd.cu", "attn_fwd_chain.cu", "tma_map.cu", "attn_bwd.cu",
            "attn_rows.cu", "attn_fwd_cross.cu", "attn_bwd_cross.cu"]
@@ -57,11 +62,35 @@ def _newest_input_mtime():
 
 
 def up_to_date():
-    return os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= _newest_input_mtime()
+    newest = _newest_input_mtime()
+    return all(os.path.exists(p) and os.path.getmtime(p) >= newest for p in (LIB_PATH, OPS_PATH))
+
+
+def _build_ops():
+    """sma_torch.so from csrc/torch_binding.cpp; returns the compiler's output."""
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    tmp = OPS_PATH + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-shared", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+           "-DTORCH_EXTENSION_NAME=sma_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], "-isystem", cuda]
+    for p in cpp_extension.include_paths():
+        cmd += ["-isystem", p]
+    cmd += [os.path.join(CSRC, "torch_binding.cpp"), "-o", tmp]
+    for p in cpp_extension.library_paths():
+        cmd += ["-L", p, f"-Wl,-rpath,{p}"]
+    cmd += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_binding.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, OPS_PATH)
+    return res.stdout + res.stderr
 
 
 def build(verbose=False, ptxas_info=False, force=False):
-    """Compile libsma.so if any source is newer than it; return its path."""
+    """Compile libsma.so and sma_torch.so if any source is newer; return libsma.so's path."""
     if not force and not ptxas_info and up_to_date():
         return LIB_PATH
     nvcc = _nvcc()
@@ -77,12 +106,16 @@ def build(verbose=False, ptxas_info=False, force=False):
             raise RuntimeError(f"nvcc failed on {src}:\n{res.stdout}\n{res.stderr}")
         return obj, res.stdout + res.stderr
 
-    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        ops = ex.submit(_build_ops)
         results = list(ex.map(compile_one, SOURCES))
+        ops_log = ops.result()
     if verbose or ptxas_info:
         for _, log in results:
             if log.strip():
                 print(log)
+        if ops_log.strip():
+            print(ops_log)
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc, "-shared", "-o", tmp] + [o for o, _ in results] + ARCH_FLAGS + ["-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -6,12 +6,15 @@ RuntimeError instead of silently computing something else.
 """
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 import threading
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("SMA_LIBRARY", os.path.join(_PKG_ROOT, "libsma.so"))
+OPS_PATH = os.path.join(_PKG_ROOT, "sma_torch.so")
 
 # Status codes (include/sma_capi.h).
 SMA_OK = 0
@@ -35,7 +38,6 @@ SMA_MAX_BIAS_DISTANCE = 65536
 # their strides; mask; its strides; lengths, bias_table, bias_starts,
 # bias_offsets; bias_offset; bias_side, bias_two_sided; out, lse, words,
 # bias_distance, out_lo.
-# Packing it as bytes costs about 1 us where a ctypes.Structure takes 5.
 ATTN_ARGS = struct.Struct("@if7q3P9q2P4qP3q4Pq2i5P")
 
 # Every symbol include/sma_capi.h declares, with (restype, argtypes).
@@ -79,6 +81,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_ops = None
 
 
 class SmaError(RuntimeError):
@@ -109,6 +112,33 @@ def load():
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def ops():
+    """The module sma_torch.so (csrc/torch_binding.cpp), loaded once and given
+    the entry points of libsma.so that it calls."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    lib = load()
+    with _lock:
+        if _ops is not None:
+            return _ops
+        if not os.path.exists(OPS_PATH):
+            raise RuntimeError(
+                f"sma_torch.so not found at {OPS_PATH}; build it with "
+                "`python sparse-mask-attention-auto-research_b200/build.py` (there is no fallback)"
+            )
+        import torch  # noqa: F401  (the module links to its libraries)
+
+        spec = importlib.util.spec_from_loader(
+            "sma_torch", importlib.machinery.ExtensionFileLoader("sma_torch", OPS_PATH), origin=OPS_PATH
+        )
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in SIGNATURES}, SmaError)
+        _ops = mod
+        return mod
 
 
 def check(code):

@@ -29,7 +29,6 @@ asynchronously, like the reference.
 
 import contextlib
 import ctypes
-import typing
 
 import torch
 
@@ -203,165 +202,6 @@ def backward(dout, q, k, v, out, lse, mask_packed, dq, dk, dv, scale):
                 dq_accum.data_ptr(), delta.data_ptr(), B, H, N, D, float(scale), _stream_ptr(q.device),
             )
         )
-
-
-def _strided(t):
-    """`t`, or a contiguous copy of it where the kernels cannot step along its
-    strides (last axis contiguous, the others positive multiples of 16 bytes,
-    a 16-byte aligned base)."""
-    if t.is_contiguous():
-        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], st[:-1])
-    ):
-        return t
-    return t.contiguous()
-
-
-def _empty(t):
-    """A contiguous tensor like `t` (empty_like costs half of empty's host time)."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _mask_strides(mask):
-    """`mask` with a contiguous last axis, and its strides along the others (0
-    where it is broadcast)."""
-    if mask.shape[3] > 1 and mask.stride(3) != 1:
-        mask = mask.contiguous()
-    return mask, tuple(0 if n == 1 else s for n, s in zip(mask.shape[:3], mask.stride()[:3]))
-
-
-class Bias(typing.NamedTuple):
-    """A relative position bias for the kernels."""
-
-    table: torch.Tensor  # [buckets, H]
-    starts: ctypes.Array  # one side's bucket starts
-    two_sided: bool
-    offset: int
-    offsets: typing.Optional[torch.Tensor]  # int32 [B], or None: offset for all
-
-
-def _attn_args(q, k, v, out, scale, mask_ptr=0, mask_strides=(0, 0, 0), lengths=None, prefix=None, bias=None, lse=0,
-               words=0, bias_distance=0, out_lo=0):
-    """sma_attn_args (include/sma_capi.h) of checked tensors and addresses."""
-    B, H, Nq, D = q.shape
-    Hkv, Nk = k.shape[1:3]
-    if prefix is not None and prefix[0].shape[1]:
-        kp, vp = prefix
-        P, pre = kp.shape[1], (kp.data_ptr(), vp.data_ptr(), *kp.stride()[:2], *vp.stride()[:2])
-    else:
-        P, pre = 0, (0, 0, 0, 0, 0, 0)
-    if bias is not None:
-        starts = bias.starts
-        add = (bias.table.data_ptr(), ctypes.addressof(starts), 0 if bias.offsets is None else bias.offsets.data_ptr(),
-               bias.offset, len(starts), int(bias.two_sided))
-    else:
-        add = (0, 0, 0, 0, 0, 0)
-    return _lib.ATTN_ARGS.pack(
-        _DTYPES[q.dtype], scale, B, H, Hkv, Nq, Nk, D, P, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
-        *k.stride()[:3], *v.stride()[:3], *pre, mask_ptr, *mask_strides, 0 if lengths is None else lengths.data_ptr(),
-        *add, out.data_ptr(), lse, words, bias_distance, out_lo,
-    )
-
-
-def rows_forward(q, k, v, out, scale, mask=None, lengths=None, prefix=None, bias=None):
-    """Attention of a few query rows per key head (sma_rows_attn_fwd): q
-    [B, H, Nq, D], k and v [B, Hkv, Nk, D], a bool ``mask`` that broadcasts to
-    [B, H, Nq, Nk] or int32 ``lengths`` [B], a shared ``prefix`` (k, v)
-    [Hkv, P, D] and a ``bias``.  Writes ``out``.  The callers
-    (cross_attention.py) check the arguments."""
-    mask_ptr, mask_st = 0, (0, 0, 0)
-    if mask is not None:
-        mask, mask_st = _mask_strides(mask)
-        mask_ptr = mask.data_ptr()
-    args = _attn_args(q, k, v, out, scale, mask_ptr, mask_st, lengths, prefix, bias)
-    lib = _lib.load()
-    with _device_guard(q.device):
-        _lib.check(lib.sma_rows_attn_fwd(args, _stream_ptr(q.device)))
-
-
-def prefix_forward(q, k, v, out, scale, prefix, lengths=None):
-    """Attention behind a shared ``prefix`` (k, v) [Hkv, P, D], read once for
-    the batch (sma_prefix_attn_fwd)."""
-    args = _attn_args(q, k, v, out, scale, lengths=lengths, prefix=prefix)
-    lib = _lib.load()
-    with _device_guard(q.device):
-        _lib.check(lib.sma_prefix_attn_fwd(args, _stream_ptr(q.device)))
-
-
-def _saved_layout(q, k, mask_strides, bias, training):
-    """Byte offsets (words, bias_distance, lse, out_lo; 0 where there is none,
-    each a multiple of 16) within the buffer a forward fills for itself and
-    its backward, and the buffer's size.  The first 16 bytes are not used, so
-    that no offset is 0."""
-    B, H, Nq, D = q.shape
-    end = 16
-    words = distance = lse = out_lo = 0
-    if mask_strides is not None:
-        words = end
-        rows, tiles = 1, 1
-        for n, s, per in zip((B, H, Nq), mask_strides, (1, 1, 128)):
-            if s:
-                rows *= n
-                tiles *= (n + per - 1) // per
-        Nk = k.shape[2]
-        W = (Nk + 127) // 128 * 4
-        end += (rows + tiles) * W * 4 + (tiles * ((Nk + 2047) // 2048) * 4 + 15) // 16 * 16
-    if bias is not None:
-        distance = end
-        n = (2 if bias.two_sided else 1) * bias.starts[len(bias.starts) - 1] + 516
-        end += H * 64 * (n // 4 + 1)
-    if training:
-        lse = end
-        end += (B * H * Nq * 4 + 15) // 16 * 16
-        out_lo = end
-        end += B * H * Nq * D * 2
-    return words, distance, lse, out_lo, end
-
-
-def cross_forward(q, k, v, out, scale, mask=None, bias=None, training=False):
-    """Attention of many query rows (sma_cross_attn_fwd).  Writes ``out``;
-    returns what cross_backward needs of this call besides the tensors:
-    (buffer, strides of the mask or None)."""
-    mask_ptr, mask_st = 0, None
-    if mask is not None:
-        mask, mask_st = _mask_strides(mask)
-        mask_ptr = mask.data_ptr()
-    words, distance, lse, out_lo, size = _saved_layout(q, k, mask_st, bias, training)
-    saved, base = None, 0
-    if size > 16:
-        saved = torch.empty(size, dtype=torch.uint8, device=q.device)
-        base = saved.data_ptr()
-    args = _attn_args(q, k, v, out, scale, mask_ptr, mask_st or (0, 0, 0), bias=bias, lse=lse and base + lse,
-                      words=words and base + words, bias_distance=distance and base + distance,
-                      out_lo=out_lo and base + out_lo)
-    lib = _lib.load()
-    with _device_guard(q.device):
-        _lib.check(lib.sma_cross_attn_fwd(args, _stream_ptr(q.device)))
-    return saved, mask_st
-
-
-def cross_backward(dout, q, k, v, out, scale, saved, mask_strides=None, bias=None):
-    """Gradients of cross_forward(training=True) (sma_cross_attn_bwd) from its
-    ``out`` and what it returned: (dq, dk, dv, dtable or None), contiguous."""
-    words, distance, lse, out_lo, _ = _saved_layout(q, k, mask_strides, bias, True)
-    base = saved.data_ptr()
-    args = _attn_args(q, k, v, out, scale, 0, mask_strides or (0, 0, 0), bias=bias, lse=base + lse,
-                      words=words and base + words, bias_distance=distance and base + distance, out_lo=base + out_lo)
-    lib = _lib.load()
-    dq, dk, dv = _empty(q), _empty(k), _empty(k)
-    with _device_guard(q.device):
-        dtable = None if bias is None else torch.empty_like(bias.table)
-        floats = lib.sma_cross_attn_bwd_scratch(args)
-        _require(floats >= 0, "backward: unsupported arguments")
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _lib.check(
-            lib.sma_cross_attn_bwd(args, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                   None if dtable is None else dtable.data_ptr(), scratch.data_ptr(),
-                                   _stream_ptr(q.device))
-        )
-    return dq, dk, dv, dtable
 
 
 def pack_mask(mask):
