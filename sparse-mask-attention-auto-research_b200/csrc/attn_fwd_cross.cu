@@ -6,6 +6,40 @@
 namespace sma {
 namespace {
 
+// ---------------------------------------------------------------- bias by relative position
+// Value i of head h is log2(e) * table[bucket(lo - kBiasPad + i)][h], laid out
+// as bias_stride (sma_internal.h) says: a row of the attention kernel reads the
+// bias of consecutive keys in vectors, at any start (B16 H12 N512 D64 with a
+// random mask, 32 buckets: 57 us, with a scalar load for every key 59).
+struct ExpandParams {
+  BiasSpec bias;
+  int bf16, lo, len;
+  int64_t stride;
+  float* out;
+  int blocks, head_blocks;  // 0 blocks: no bias
+};
+
+__device__ __forceinline__ void expand_bias(const ExpandParams& e, int block, int* starts) {
+  __shared__ int bucket[260];  // of values 4 j0 - 3 .. 4 j0 + 256
+  __shared__ float value[260];
+  for (int i = threadIdx.x; i < e.bias.side; i += 256) starts[i] = e.bias.starts[i];
+  __syncthreads();
+  pdl_wait_prior_grid();
+  const int j0 = block / e.head_blocks * 64;
+  for (int i = threadIdx.x; i < 260; i += 256)
+    bucket[i] = bias_bucket(e.bias, starts, e.lo - kBiasPad + max(0, min(e.len - 1, 4 * j0 - 3 + i)));
+  const int j = threadIdx.x >> 2, k = threadIdx.x & 3;
+  for (int h = block % e.head_blocks; h < e.bias.H; h += e.head_blocks) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 260; i += 256)
+      value[i] = kLog2e * (e.bf16 ? bias_value<true>(e.bias, bucket[i], h) : bias_value<false>(e.bias, bucket[i], h));
+    __syncthreads();
+    const float* v = value + 4 * j + 3 - k;
+    if (16ll * (j0 + j) < e.stride)
+      reinterpret_cast<float4*>(e.out + h * e.stride)[4 * (j0 + j) + k] = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 // ---------------------------------------------------------------- mask packer
 // bool bytes with any batch / head / query strides -> words [Bm, Hm, Qm, W],
 // W = 4 ceil(Nk / 128) (whole 128-key tiles; bits at columns >= Nk are 0), and
@@ -41,14 +75,22 @@ struct PackParams {
   int occ_words, tile_log2;   // words of live bits per tile; packed words per key tile
 };
 
+// With a bias, the first blocks of the launch lay that out.
 template <bool kAligned>
-__global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_constant__ PackParams p) {
+__global__ void __launch_bounds__(kPackThreads)
+    pack_tiles_kernel(const __grid_constant__ PackParams p, const __grid_constant__ ExpandParams e) {
   pdl_launch_dependents();
   constexpr int kPackRounds = kPackPackRounds, kVecs = kAligned ? 2 : 3;
   __shared__ uint32_t live[kPackWords / 2 / 32];  // a key tile is 2 or 4 words
   __shared__ uint32_t kept[kPackWords];
-  const int chunk = blockIdx.x % p.chunks;
-  int rest = blockIdx.x / p.chunks;
+  if (static_cast<int>(blockIdx.x) < e.blocks) {
+    static_assert(kPackWords >= kMaxBiasSide && kPackThreads == 256, "bucket starts; threads of expand_bias");
+    expand_bias(e, static_cast<int>(blockIdx.x), reinterpret_cast<int*>(kept));
+    return;
+  }
+  const int block = static_cast<int>(blockIdx.x) - e.blocks;
+  const int chunk = block % p.chunks;
+  int rest = block / p.chunks;
   const int qt = rest % p.QT;
   rest /= p.QT;
   const int hblk = rest % p.Hb;
@@ -111,36 +153,6 @@ __global__ void __launch_bounds__(kPackThreads) pack_tiles_kernel(const __grid_c
   const int k = chunk * bytes + threadIdx.x;
   if (threadIdx.x < bytes && k < p.occ_words * 4)
     p.occ[((b * p.Hb + hblk) * p.QT + qt) * (p.occ_words * 4) + k] = reinterpret_cast<const uint8_t*>(live)[threadIdx.x];
-}
-
-// ---------------------------------------------------------------- bias by relative position
-// Value i of head h is log2(e) * table[bucket(lo - kBiasPad + i)][h], laid out
-// as bias_stride (sma_internal.h) says: a row of the attention kernel reads the
-// bias of consecutive keys in vectors, at any start (B16 H12 N512 D64 with a
-// random mask, 32 buckets: 57 us, with a scalar load for every key 59).
-__global__ void __launch_bounds__(256)
-    bias_expand_kernel(const __grid_constant__ BiasSpec bias, int bf16, int lo, int len, int64_t stride,
-                       float* __restrict__ out) {
-  __shared__ int starts[kMaxBiasSide];
-  __shared__ int bucket[260];   // of values 4 j0 - 3 .. 4 j0 + 256
-  __shared__ float value[260];
-  for (int i = threadIdx.x; i < bias.side; i += 256) starts[i] = bias.starts[i];
-  __syncthreads();
-  pdl_launch_dependents();
-  pdl_wait_prior_grid();
-  const int j0 = blockIdx.x * 64;
-  for (int i = threadIdx.x; i < 260; i += 256)
-    bucket[i] = bias_bucket(bias, starts, lo - kBiasPad + max(0, min(len - 1, 4 * j0 - 3 + i)));
-  const int j = threadIdx.x >> 2, k = threadIdx.x & 3;
-  for (int h = blockIdx.y; h < bias.H; h += gridDim.y) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 260; i += 256)
-      value[i] = kLog2e * (bf16 ? bias_value<true>(bias, bucket[i], h) : bias_value<false>(bias, bucket[i], h));
-    __syncthreads();
-    const float* v = value + 4 * j + 3 - k;
-    if (16ll * (j0 + j) < stride)
-      reinterpret_cast<float4*>(out + h * stride)[4 * (j0 + j) + k] = make_float4(v[0], v[1], v[2], v[3]);
-  }
 }
 
 // ---------------------------------------------------------------- merge of a split launch
@@ -403,46 +415,64 @@ PackLayout pack_layout(const CrossParams& p, const Geo& x) {
   return l;
 }
 
-int launch_pack(const CrossParams& p, const char** msg) {
-  const Geo x = tile_geometry(p, false);
-  const PackLayout l = pack_layout(p, x);
-  PackParams k{};
-  k.mask = p.mask;
-  k.sb = p.mask_stride[0];
-  k.sh = p.mask_stride[1];
-  k.sq = p.mask_stride[2];
-  k.hi = p.mask + (l.Bm - 1) * k.sb + (l.Hm - 1) * k.sh + (l.Qm - 1) * k.sq + p.Nk;
-  k.words = p.words;
-  k.kept = p.words + l.words;
-  k.occ = reinterpret_cast<uint8_t*>(p.words + l.words + l.kept);
-  k.Hm = static_cast<int>(l.Hm);
-  k.Qm = static_cast<int>(l.Qm);
-  k.Nk = static_cast<int>(p.Nk);
-  k.W = static_cast<int>((p.Nk + 127) / 128 * 4);
-  k.hb = p.word_stride[1] != 0 ? x.hb : 1;
-  k.tn = p.word_stride[2] != 0 ? x.tn : 1;
-  k.rows = k.hb * k.tn;
-  k.Hb = static_cast<int>(l.Hb);
-  k.QT = static_cast<int>(l.QT);
-  k.occ_words = static_cast<int>(l.occ_words);
-  k.tile_log2 = p.D == 64 ? 2 : 1;
-  // The longest stretch (fewest CTAs) that still gives every SM a few CTAs; 8
-  // key tiles at least.
-  DeviceProps dp;
-  if (!device_props(&dp, msg)) return kErrCuda;
-  const int64_t tiles = l.Bm * l.Hb * l.QT;
-  k.chunk_log2 = 8;
-  while (k.chunk_log2 > k.tile_log2 + 3 && tiles * (((k.W - 1) >> k.chunk_log2) + 1) < 6 * dp.sms) --k.chunk_log2;
-  while ((1 << (k.chunk_log2 - 1)) >= k.W) --k.chunk_log2;
-  k.chunks = ((k.W - 1) >> k.chunk_log2) + 1;
-  const int64_t blocks = tiles * k.chunks;
-  if (blocks > 0x7FFFFFFFll) {
-    *msg = "attention: mask too large";
-    return kErrArg;
+// Packs p's mask and lays its bias out, as far as it has them.
+int launch_layout(const CrossParams& p, const char** msg) {
+  ExpandParams ex{};
+  if (p.bias.table != nullptr) {
+    int hi = 0;
+    ex.bias = p.bias;
+    ex.bf16 = p.dtype;
+    bias_range(p.bias, &ex.lo, &hi);
+    ex.len = hi - ex.lo + 1 + 2 * kBiasPad;
+    ex.stride = bias_stride(ex.len);
+    ex.out = p.bias_distance;
+    ex.head_blocks = static_cast<int>(std::min<int64_t>(p.H, 1024));
+    ex.blocks = static_cast<int>((ex.stride / 16 + 63) / 64) * ex.head_blocks;
   }
-  const bool aligned = ((reinterpret_cast<uintptr_t>(p.mask) | k.sb | k.sh | k.sq) & 15) == 0;
+  if (p.mask == nullptr && ex.blocks == 0) return kOk;
+  const Geo x = tile_geometry(p, false);
+  PackParams k{};
+  int64_t blocks = 0;
+  bool aligned = true;
+  if (p.mask != nullptr) {
+    const PackLayout l = pack_layout(p, x);
+    k.mask = p.mask;
+    k.sb = p.mask_stride[0];
+    k.sh = p.mask_stride[1];
+    k.sq = p.mask_stride[2];
+    k.hi = p.mask + (l.Bm - 1) * k.sb + (l.Hm - 1) * k.sh + (l.Qm - 1) * k.sq + p.Nk;
+    k.words = p.words;
+    k.kept = p.words + l.words;
+    k.occ = reinterpret_cast<uint8_t*>(p.words + l.words + l.kept);
+    k.Hm = static_cast<int>(l.Hm);
+    k.Qm = static_cast<int>(l.Qm);
+    k.Nk = static_cast<int>(p.Nk);
+    k.W = static_cast<int>((p.Nk + 127) / 128 * 4);
+    k.hb = p.word_stride[1] != 0 ? x.hb : 1;
+    k.tn = p.word_stride[2] != 0 ? x.tn : 1;
+    k.rows = k.hb * k.tn;
+    k.Hb = static_cast<int>(l.Hb);
+    k.QT = static_cast<int>(l.QT);
+    k.occ_words = static_cast<int>(l.occ_words);
+    k.tile_log2 = p.D == 64 ? 2 : 1;
+    // The longest stretch (fewest CTAs) that still gives every SM a few CTAs; 8
+    // key tiles at least.
+    DeviceProps dp;
+    if (!device_props(&dp, msg)) return kErrCuda;
+    const int64_t tiles = l.Bm * l.Hb * l.QT;
+    k.chunk_log2 = 8;
+    while (k.chunk_log2 > k.tile_log2 + 3 && tiles * (((k.W - 1) >> k.chunk_log2) + 1) < 6 * dp.sms) --k.chunk_log2;
+    while ((1 << (k.chunk_log2 - 1)) >= k.W) --k.chunk_log2;
+    k.chunks = ((k.W - 1) >> k.chunk_log2) + 1;
+    blocks = tiles * k.chunks;
+    if (blocks > 0x7FFFFFFFll - ex.blocks) {
+      *msg = "attention: mask too large";
+      return kErrArg;
+    }
+    aligned = ((reinterpret_cast<uintptr_t>(p.mask) | k.sb | k.sh | k.sq) & 15) == 0;
+  }
   const cudaError_t e = launch_pdl(aligned ? pack_tiles_kernel<true> : pack_tiles_kernel<false>,
-                                   static_cast<unsigned>(blocks), kPackThreads, 0, p.stream, k);
+                                   static_cast<unsigned>(ex.blocks + blocks), kPackThreads, 0, p.stream, k, ex);
   if (e != cudaSuccess) {
     *msg = cudaGetErrorString(e);
     return kErrLaunch;
@@ -511,37 +541,9 @@ int launch_fill(float* x, int64_t n, float v, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
-int launch_bias_expand(const CrossParams& p, const char** msg) {
-  int lo = 0, hi = 0;
-  bias_range(p.bias, &lo, &hi);
-  const int len = hi - lo + 1 + 2 * kBiasPad;
-  const int64_t stride = bias_stride(len);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((stride / 16 + 63) / 64), static_cast<unsigned>(std::min<int64_t>(p.H, 1024)));
-  cfg.blockDim = dim3(256);
-  cfg.stream = p.stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, bias_expand_kernel, p.bias, p.dtype, lo, len, stride, p.bias_distance);
-  if (e != cudaSuccess) {
-    *msg = cudaGetErrorString(e);
-    return kErrLaunch;
-  }
-  return kOk;
-}
-
 int launch_attn_cross(const CrossParams& p, const char** msg) {
-  if (p.mask != nullptr) {
-    const int rc = launch_pack(p, msg);
-    if (rc != kOk) return rc;
-  }
-  if (p.bias.table != nullptr) {
-    const int rc = launch_bias_expand(p, msg);
-    if (rc != kOk) return rc;
-  }
+  const int rc = launch_layout(p, msg);
+  if (rc != kOk) return rc;
   const Keys keys{p.k, p.v, p.k_stride, p.v_stride, p.Nk, false};
   return launch_tiles(p, keys, false, false, {}, {}, msg);
 }

@@ -151,8 +151,6 @@ constexpr int kBiasPad = 256;
 // values can so be read 16 bytes at a time, whatever its start.
 inline int64_t bias_stride(int len) { return 16 * ((static_cast<int64_t>(len) + 3) / 4 + 1); }  // floats per head
 
-// Fills p.bias_distance from p.bias.
-int launch_bias_expand(const CrossParams& p, const char** msg);
 // Many query rows (attn_fwd_cross.cu), Nk <= kMaxSeqLen.
 int launch_attn_cross(const CrossParams& p, const char** msg);
 // A shared prefix attended once for the batch, P > 0 (attn_fwd_cross.cu).
