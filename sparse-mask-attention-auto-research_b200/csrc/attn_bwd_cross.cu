@@ -1292,6 +1292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // the last bucket of a side the sums of the blocks beyond.  Every thread adds
 // in a fixed order and the threads are added in a fixed tree, so the result
 // does not depend on timing; FP32 throughout, rounded once to the table's type.
+// Bound by the latency of its gathers (12 us at B4 H16 N1024, 3.7 MB of sums).
 constexpr int kReduceThreads = 256;
 
 template <bool BF16>
@@ -1524,6 +1525,9 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, int device, cons
                    static_cast<uint16_t*>(g.dk), static_cast<uint16_t*>(g.dv), static_cast<int>(KT), x);
   if (e == cudaSuccess && kBias) {
     const dim3 grid(static_cast<unsigned>(p.H), static_cast<unsigned>(p.bias.side * (p.bias.two_sided ? 2 : 1)));
+    // Not launched early like the others: its few blocks would gather on the
+    // SMs that cross_dq_kernel leaves first (B4 H16 N1024 D64 causal, a whole
+    // training pass: 158 us, launched early 169).
     bias_reduce_kernel<BF16><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, g.dtable);
   }
   if (e == cudaSuccess) e = cudaGetLastError();
