@@ -57,10 +57,10 @@ void check(int code) {
 // With gradients: 64-row steps of the queries of all heads that share a key head.
 constexpr int64_t kMaxSteps = 2048;
 
+// Backward mode, or forward mode (which the node refuses).
 bool needs_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
-    if (t->requires_grad()) return true;
+    if ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()) return true;
   return false;
 }
 
@@ -365,6 +365,7 @@ Tensor relative_bias_attention(const Tensor& q, const Tensor& k, const Tensor& v
     offsets = offsets->contiguous();
   }
   const double scale = scale_of(scale_, q.size(3));
+  TORCH_CHECK(side >= 1 && side <= SMA_MAX_BIAS_SIDE, "1 to ", SMA_MAX_BIAS_SIDE, " buckets per side are supported");
   Bias bias;
   bias.on = true;
   bias.two_sided = two_sided;

@@ -77,6 +77,17 @@ def test_second_derivatives_are_refused():
         dk.sum().backward()
 
 
+def test_forward_mode_is_refused():
+    """Not dropped in silence, with or without inputs that require gradients."""
+    q, k, v, table, mask, _ = case()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for run in (lambda: cross_attention(dual, k, v, mask), lambda: relative_bias_attention(q, k, v, dual[0, :, :16, 0].t()),
+                    lambda: shared_prefix_attention(dual, k[0], v[0], k, v)):
+            with pytest.raises(RuntimeError):
+                run()
+
+
 def test_changed_inputs_are_noticed():
     q, k, v, table, mask, dout = case()
     q.requires_grad_(True)
@@ -119,6 +130,17 @@ def test_strided_and_misaligned_incoming_gradients():
     got, = torch.autograd.grad(cross_attention(q, k, v, mask).sum(), v)
     ones, = torch.autograd.grad(cross_attention(q, k, v, mask), v, torch.ones_like(dout))
     assert torch.equal(got, ones)
+
+
+def test_views_with_odd_strides_of_single_rows():
+    """Axes of length 1 may have any stride."""
+    q, k, v, table, mask, _ = case()
+    one = torch.empty_strided((1, 1, 1, 64), (7, 3, 5, 1), dtype=q.dtype, device="cuda").copy_(q[:1, :1, :1])
+    keys = torch.empty_strided((1, 1, 133, 64), (11, 9, 64, 1), dtype=q.dtype, device="cuda").copy_(k[:1, :1])
+    want = cross_attention(q[:1, :1, :1].contiguous(), k[:1, :1].contiguous(), k[:1, :1].contiguous())
+    assert torch.equal(cross_attention(one, keys, keys), want)
+    one.requires_grad_(True)
+    assert torch.autograd.grad(cross_attention(one, keys, keys).sum(), one)[0].shape == one.shape
 
 
 def test_errors_keep_their_types():
