@@ -271,3 +271,27 @@ def test_padding_may_hold_anything(Nq, D, bias):
         else:
             assert torch.equal(a, b)
     assert torch.all(got[1].masked_select(gone.expand_as(k)) == 0) and torch.all(got[2].masked_select(gone.expand_as(v)) == 0)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("mask,bias", [("none", False), ("padding", False), ("heads", False), ("padding", True)])
+def test_items_that_do_not_fill_the_last_round(mask, bias, D, dtype):
+    """A few more (batch, head, query tile) items than run at once."""
+    B, H, Nq, Nk = 10, 30, 20, 1100
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    q, k, v = (heads(gen, B, H, n, D, dtype).requires_grad_(True) for n in (Nq, Nk, Nk))
+    dout = heads(gen, B, H, Nq, D, dtype)
+    m = make_mask(gen, mask, B, H, Nq, Nk)
+    if bias:
+        table = torch.randn(32, H, generator=gen, device=DEV).to(dtype)
+        out = relative_bias_attention(q, k, v, table, m, query_offset=500)
+        add = table.double().cpu().t()[:, buckets_of(Nq, Nk, 32, 128, True, 500)]
+    else:
+        out, add = cross_attention(q, k, v, m), None
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)))
+    sparse_attn_cuda.device_status()
+    ref = RefGrads(q, k, v, dout, m, add, dtype=dtype)
+    ref.check_out(out.detach())
+    ref.check(**got)
+    again = (relative_bias_attention(q, k, v, table, m, query_offset=500) if bias else cross_attention(q, k, v, m)).detach()
+    assert torch.equal(out.detach(), again)
