@@ -44,6 +44,11 @@
 //
 // Included by attn_fwd_chain.cu (square attention: q, k and v [B, H, N, D])
 // and attn_fwd_cross.cu (kX: queries and keys of different lengths, see Geo).
+//
+// Measured with kX and no mask: B4 H32 Hkv8 Nq1024 Nk2048 D64 151 us (456
+// TFLOP/s), D128 192 us (715); H37 Nq1024 Nk16384 D64 287 us (553), D128 370 us
+// (859).  Bound by the latency of the softmax loop (two warps per SM
+// sub-partition), not by a pipe.
 #pragma once
 
 #include <algorithm>

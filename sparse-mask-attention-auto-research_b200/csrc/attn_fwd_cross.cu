@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kPackThreads)
 // the overall maximum M, O = sum w_p O_p / sum w_p l_out_p.  Writes O and the
 // LSE, or (`out_ml`) the merged row as a piece for a later merge.  One warp
 // per row, so every read is a whole row of D floats; bound by reading the
-// pieces, mostly from L2 (they have just been written).
+// pieces, mostly from L2 (they have just been written): 256 pieces of 128 rows,
+// D128 (17 MB), 10 us.
 struct MergeParams {
   const float* ws;   // [units][128][4] (max, sum, sum of rounded P, -) then [units][128][D]
   int64_t units;
