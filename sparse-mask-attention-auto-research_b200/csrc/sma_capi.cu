@@ -157,9 +157,6 @@ int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool
     if (a->bias_two_sided && a->bias_starts[a->bias_side - 1] == 0)
       return fail(sma::kErrArg, "attention: a two-sided bias needs a bucket start above 0");
   }
-  uint32_t* err = nullptr;
-  const int rc = error_word(&err);
-  if (rc != sma::kOk) return rc;
   p->dtype = a->dtype;
   p->q = a->q;
   p->k = a->k;
@@ -196,11 +193,13 @@ int cross_params(const sma_attn_args* a, void* stream, sma::CrossParams* p, bool
   p->D = a->D;
   p->P = a->P;
   p->scale = a->scale;
-  p->err_word = err;
   p->timeout_ns = g_timeout_ns.load(std::memory_order_relaxed);
   p->stream = static_cast<cudaStream_t>(stream);
   return sma::kOk;
 }
+
+// What needs the device, once all arguments have been checked.
+int device_params(sma::CrossParams* p) { return error_word(&p->err_word); }
 
 }  // namespace
 
@@ -440,7 +439,9 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
   if (p.P > 0) return fail(sma::kErrArg, "attention: no prefix here");
+  if (args->words && !args->mask) return fail(sma::kErrArg, "attention: words are packed from a mask, and there is none");
   rc = tile_params(args, &p);
+  if (rc == sma::kOk) rc = device_params(&p);
   if (rc != sma::kOk) return rc;
   if (p.Nk == 0) return write_nothing(p);
   const char* msg = nullptr;
@@ -464,6 +465,8 @@ int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, vo
   if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(scratch))
     return fail(sma::kErrArg, "backward: dout/dq/dk/dv/scratch must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(dtable) & 1u) return fail(sma::kErrArg, "backward: misaligned dtable");
+  rc = device_params(&p);
+  if (rc != sma::kOk) return rc;
   const sma::CrossGrads g{dout, dq, dk, dv, dtable, scratch};
   const char* msg = nullptr;
   rc = sma::launch_attn_cross_bwd(p, g, &msg);
@@ -488,6 +491,8 @@ int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream) {
   if (rc != sma::kOk) return rc;
   if (p.P == 0 || args->mask || args->words || args->bias_table || args->lse || args->out_lo)
     return fail(sma::kErrArg, "attention: a shared prefix takes P > 0 and no mask, bias, lse or out_lo");
+  rc = device_params(&p);
+  if (rc != sma::kOk) return rc;
   const char* msg = nullptr;
   rc = sma::launch_shared_prefix(p, &msg);
   return rc == sma::kOk ? rc : fail(rc, msg);
@@ -499,6 +504,8 @@ int sma_rows_attn_fwd(const sma_attn_args* args, void* stream) {
   bool empty = false;
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
+  rc = device_params(&p);
+  if (rc != sma::kOk) return rc;
   if (p.Nk == 0 && p.P == 0) return write_nothing(p);
   const char* msg = nullptr;
   rc = sma::launch_attn_rows(p, &msg);

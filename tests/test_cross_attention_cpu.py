@@ -34,6 +34,7 @@ def raw(**kw):
     return L.ATTN_ARGS.pack(*(d[f] for f in FIELDS))
 
 
+FAR = (ctypes.c_int32 * 2)(0, L.SMA_MAX_BIAS_DISTANCE + 1)
 BIAS = dict(table=16, starts=ctypes.addressof(STARTS), side=4)
 
 
@@ -80,6 +81,76 @@ def test_library_refuses(lib, kw, code):
 
 def test_library_refuses_no_arguments(lib):
     assert lib.sma_rows_attn_fwd(None, None) == L.SMA_ERR_ARG
+
+
+MASK = dict(mask=1, mn=64, words=16)
+TRAIN = dict(lse=16, out_lo=16)
+
+
+@pytest.mark.parametrize(
+    "kw,code",
+    [
+        (dict(D=96), L.SMA_ERR_UNSUPPORTED_D),
+        (dict(Nk=L.SMA_MAX_SEQ_LEN + 1), L.SMA_ERR_UNSUPPORTED_N),
+        (dict(P=8, kp=16, vp=16), L.SMA_ERR_ARG),
+        (dict(MASK, words=0), L.SMA_ERR_ARG),
+        (dict(MASK, words=8), L.SMA_ERR_ARG),
+        (dict(MASK, mask=0), L.SMA_ERR_ARG),  # words that nothing fills
+        (dict(MASK, lengths=16), L.SMA_ERR_ARG),
+        (dict(out_lo=8), L.SMA_ERR_ARG),
+        (dict(BIAS), L.SMA_ERR_ARG),  # no room for the bias by distance
+        (dict(BIAS, distance=8), L.SMA_ERR_ARG),
+        (dict(BIAS, starts=ctypes.addressof(FAR), side=2, distance=16), L.SMA_ERR_UNSUPPORTED_N),
+    ],
+)
+def test_tile_entry_refuses(lib, kw, code):
+    assert lib.sma_cross_attn_fwd(raw(**kw), None) == code
+    assert lib.sma_last_error()
+
+
+@pytest.mark.parametrize(
+    "kw,code",
+    [
+        (dict(), L.SMA_ERR_ARG),  # no prefix
+        (dict(P=8, kp=16, vp=16, mask=1, words=16), L.SMA_ERR_ARG),
+        (dict(P=8, kp=16, vp=16, lse=16), L.SMA_ERR_ARG),
+        (dict(P=8, kp=16, vp=16, out_lo=16), L.SMA_ERR_ARG),
+        (dict(P=8, kp=16, vp=16, Nk=L.SMA_MAX_SEQ_LEN + 1), L.SMA_ERR_UNSUPPORTED_N),
+        (dict(P=8, kp=16), L.SMA_ERR_ARG),
+    ],
+)
+def test_prefix_entry_refuses(lib, kw, code):
+    assert lib.sma_prefix_attn_fwd(raw(**kw), None) == code
+    assert lib.sma_last_error()
+
+
+@pytest.mark.parametrize(
+    "kw,pointers,code",
+    [
+        (dict(), {}, L.SMA_ERR_ARG),  # no lse, no out_lo
+        (dict(lse=16), {}, L.SMA_ERR_ARG),
+        (dict(TRAIN, Nk=0), {}, L.SMA_ERR_ARG),
+        (dict(TRAIN, Nq=0), {}, L.SMA_ERR_ARG),
+        (dict(TRAIN, lengths=16), {}, L.SMA_ERR_ARG),
+        (dict(TRAIN, P=8, kp=16, vp=16), {}, L.SMA_ERR_ARG),
+        (dict(TRAIN, Nk=L.SMA_MAX_SEQ_LEN + 1), {}, L.SMA_ERR_UNSUPPORTED_N),
+        (dict(TRAIN), dict(dout=None), L.SMA_ERR_ARG),
+        (dict(TRAIN), dict(dq=8), L.SMA_ERR_ARG),
+        (dict(TRAIN), dict(scratch=None), L.SMA_ERR_ARG),
+        (dict(TRAIN, **BIAS, distance=16), dict(dtable=None), L.SMA_ERR_ARG),
+        (dict(TRAIN, **BIAS, distance=16), dict(dtable=17), L.SMA_ERR_ARG),
+    ],
+)
+def test_backward_entry_refuses(lib, kw, pointers, code):
+    at = dict(dict(dout=16, dq=16, dk=16, dv=16, dtable=16, scratch=16), **pointers)
+    assert lib.sma_cross_attn_bwd(raw(**kw), *at.values(), None) == code
+    assert lib.sma_last_error()
+
+
+def test_backward_scratch_of_refused_arguments(lib):
+    for kw in (dict(D=96), dict(Nk=0), dict(B=0), dict(Nk=L.SMA_MAX_SEQ_LEN + 1), dict(BIAS)):
+        assert lib.sma_cross_attn_bwd_scratch(raw(**kw)) == -1
+    assert lib.sma_cross_attn_bwd_scratch(None) == -1
 
 
 def test_nothing_to_write_is_ok(lib):
