@@ -297,7 +297,8 @@ __device__ __forceinline__ void load_tile_words(const uint32_t* mrow, int kt, in
 }
 
 // Eight 32-bit words r[o .. o+7] to a 32-byte aligned global address.
-__device__ __forceinline__ void st_global_v8(void* dst, const uint32_t (&r)[16], int o) {
+template <int N>
+__device__ __forceinline__ void st_global_v8(void* dst, const uint32_t (&r)[N], int o) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(r[o]), "r"(r[o + 1]),
                "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
                : "memory");
@@ -1387,8 +1388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 32; ++q) u[q] = 0u;
           }
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            reinterpret_cast<uint4*>(po + dc * 32)[q] = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+          for (int q = 0; q < 32; q += 8) st_global_v8(po + dc * 32 + q, u, q);
         }
         *reinterpret_cast<float4*>(ml) = make_float4(m_run, l_run, l_out, 0.f);
         if constexpr (kX) continue;
