@@ -109,19 +109,19 @@ def build(verbose=False, ptxas_info=False, force=False):
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         ops = ex.submit(_build_ops)
         results = list(ex.map(compile_one, SOURCES))
-        ops_log = ops.result()
     if verbose or ptxas_info:
         for _, log in results:
             if log.strip():
                 print(log)
-        if ops_log.strip():
-            print(ops_log)
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc, "-shared", "-o", tmp] + [o for o, _ in results] + ARCH_FLAGS + ["-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    log = ops.result()  # raises what went wrong there, with libsma.so in place
+    if (verbose or ptxas_info) and log.strip():
+        print(log)
     return LIB_PATH
 
 
