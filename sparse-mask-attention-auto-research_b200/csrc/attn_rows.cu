@@ -551,49 +551,87 @@ __global__ void __launch_bounds__(kThreads, 2)
   __threadfence();
   float* weight = reinterpret_cast<float*>(smem);  // [pieces][16]
   float* total = weight + kMaxPieces * kRows;      // [16] 1 / sum of rounded P
+  float4* part = reinterpret_cast<float4*>(total + kRows);  // [kThreads]
+  static_assert(kRows * 8 == kThreads && kMaxPieces * kRows % 4 == 0, "eight threads per row; part is aligned");
   const int64_t u0 = static_cast<int64_t>(item) * p.pieces;
-  if (threadIdx.x < static_cast<unsigned>(rows)) {
-    const int r = threadIdx.x;
+  {
+    // Eight threads per row, each every eighth piece, added in a fixed tree.
+    const int r = threadIdx.x >> 3, j = threadIdx.x & 7;
+    const float* src = ws_ml + (u0 * kRows + r) * 4;
+    const int n = r < rows ? p.pieces : 0;
     float M = -INFINITY, sum = 0.f, sumr = 0.f;
-    for (int pc = 0; pc < p.pieces; ++pc) M = fmaxf(M, __ldcg(ws_ml + ((u0 + pc) * kRows + r) * 4));
-    for (int pc = 0; pc < p.pieces; ++pc) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(ws_ml + ((u0 + pc) * kRows + r) * 4));
+#pragma unroll 4
+    for (int pc = j; pc < n; pc += 8) M = fmaxf(M, __ldcg(src + pc * (kRows * 4)));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+    for (int pc = j; pc < n; pc += 8) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + pc * (kRows * 4)));
       const float f = v.x == -INFINITY ? 0.f : ex2f(v.x - M);
       weight[pc * kRows + r] = f;
       sum += f * v.y;
       sumr += f * v.z;
     }
-    total[r] = sumr > 0.f ? 1.f / sumr : 0.f;
-    write_sums(r, M, sum, sumr);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      sumr += __shfl_xor_sync(0xffffffffu, sumr, o);
+    }
+    if (j == 0 && r < rows) {
+      total[r] = sumr > 0.f ? 1.f / sumr : 0.f;
+      write_sums(r, M, sum, sumr);
+    }
   }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < rows * kVec; idx += kThreads) {
+  // Four columns of a row per thread; few rows share the pieces among `groups`
+  // threads, whose sums are added in order.
+  const int vecs = rows * kVec, groups = max(1, kThreads / vecs);
+  for (int i0 = 0; i0 < vecs; i0 += kThreads) {
+    const int idx = groups > 1 ? threadIdx.x % vecs : i0 + threadIdx.x, grp = groups > 1 ? threadIdx.x / vecs : 0;
     const int r = idx / kVec, x = idx - r * kVec;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int pc = 0; pc < p.pieces; ++pc) {
-      const float f = weight[pc * kRows + r];
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(ws_o + ((u0 + pc) * kRows + r) * D + 4 * x));
-      a.x += f * v.x;
-      a.y += f * v.y;
-      a.z += f * v.z;
-      a.w += f * v.w;
+    if (idx < vecs && grp < groups) {
+      const float* src = ws_o + (u0 * kRows + r) * D + 4 * x;
+#pragma unroll 8
+      for (int pc = grp; pc < p.pieces; pc += groups) {
+        const float f = weight[pc * kRows + r];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + static_cast<int64_t>(pc) * kRows * D));
+        a.x += f * v.x;
+        a.y += f * v.y;
+        a.z += f * v.z;
+        a.w += f * v.w;
+      }
     }
-    write_out(r, x, a, total[r]);
+    if (groups > 1) {
+      part[threadIdx.x] = a;
+      __syncthreads();
+      if (grp == 0) {
+        for (int k = 1; k < groups; ++k) {
+          const float4 v = part[k * vecs + idx];
+          a.x += v.x;
+          a.y += v.y;
+          a.z += v.z;
+          a.w += v.w;
+        }
+      }
+    }
+    if (idx < vecs && grp == 0) write_out(r, x, a, total[r]);
   }
 }
 
-// Pieces per item: units run in rounds of `slots`, a unit of C / pieces
-// chunks spread over four warps costs about C / (4 pieces) chunk times and a
-// fixed start and merge of about four; the count with the least rounds * cost
-// wins, the smallest such count on a tie.
+// Pieces of the keys per item.  Units run in rounds of `slots`; in steps of a
+// chunk per warp (0.75 to 0.8 us) a unit costs its chunks and 4 more, a split 5
+// (workspace, merge) and a little per piece.  Measured, one row per key head:
+// B1 Hkv1 Nk131072 D64 18 us in 148 pieces, 100 in 8; B1 Hkv8 Nk2048 D128 11.1 in 8, 28.4
+// whole; B16 Hkv8 Nk1024 D64 10.6 whole, 11.6 in 2; Nk2048 17.9 whole, 15.2 in 2.
 int choose_pieces(int64_t items, int64_t chunks, int64_t slots) {
   const int64_t most = std::min<int64_t>(kMaxPieces, chunks / (2 * kWarps));
   int best = 1;
   double best_cost = 0.0;
-  for (int64_t pc = 1; pc <= most; ++pc) {
+  for (int64_t pc = 1; pc <= std::max<int64_t>(most, 1); ++pc) {
     const double rounds = static_cast<double>((items * pc + slots - 1) / slots);
-    const double cost = rounds * (static_cast<double>(chunks) / static_cast<double>(kWarps * pc) + 4.0 + (pc > 1 ? 2.0 : 0.0));
+    const double steps = static_cast<double>((chunks + kWarps * pc - 1) / (kWarps * pc));
+    const double cost = rounds * (steps + 4.0) + (pc > 1 ? 5.0 + 0.04 * static_cast<double>(pc) : 0.0);
     if (pc == 1 || cost < best_cost * 0.999) {
       best = static_cast<int>(pc);
       best_cost = cost;

