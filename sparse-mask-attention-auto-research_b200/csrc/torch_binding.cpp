@@ -201,12 +201,12 @@ void set_saved(sma_attn_args* a, const Layout& l, const Tensor& saved) {
 // keys read again for every 16) instead of the 128-row tiles.
 //
 // With no mask, or one that all rows of a key head share, and R rows per key
-// head in T tiles of 128, the first takes (measured on a B200) about 8 us +
+// head in T tiles of 128, the first takes (measured on a B200) about 6 us +
 // B Hkv Nk D ceil(R / 16) * 0.57e-6 us, the second (which also packs the
-// mask) 18 us + B Hkv Nk D T * 0.9e-6 us (D = 64) or 0.77e-6 us (D = 128).
-// For instance B8 Hkv8 Nk1000 D64: 12.8 against 22.3 us at 64 rows, 22.9
-// against 25.0 at 128; B16 H12 Nk1500 D128: 31 against 50 us at 16 rows, 58
-// against 49 at 24.  Masks of the rows' own and a bias cost the first more:
+// mask) 15 us + B Hkv Nk D T * 0.9e-6 us (D = 64) or 0.77e-6 us (D = 128).
+// For instance B8 Hkv8 Nk1000 D64: 12.1 against 20.3 us at 64 rows, 19.9 at
+// 96, 21.9 at 112; B16 H12 Nk1500 D128: 31 against 48 us at 16 rows, 58
+// against 48 at 24.  Masks of the rows' own and a bias cost the first more:
 // B16 H12 Nk500 D64 with a mask 19.4 against 20.9 us at 16 rows, 35.5 against
 // 21.0 at 32, so there it is taken for one tile of 16 rows only.
 bool few_rows(const Tensor& q, const Tensor& k, const Mask& mask, const Bias& bias) {
@@ -216,7 +216,7 @@ bool few_rows(const Tensor& q, const Tensor& k, const Mask& mask, const Bias& bi
   if (rows <= 16 || rows > 128) return rows <= 16;
   if (bias.on || (mask.on() && (mask.t.size(1) != 1 || mask.t.size(2) != 1))) return false;
   const double tiles = static_cast<double>((rows + 15) / 16);
-  return static_cast<double>(B * Hkv * Nk * D) * ((D == 64 ? 0.6 : 0.75) * tiles - 1.0) <= 15e6;
+  return static_cast<double>(B * Hkv * Nk * D) * ((D == 64 ? 0.6 : 0.75) * tiles - 1.0) <= 12e6;
 }
 
 void* current_stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }

@@ -28,7 +28,6 @@ asynchronously, like the reference.
 """
 
 import contextlib
-import ctypes
 
 import torch
 
