@@ -397,8 +397,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Ctl& ctl = *reinterpret_cast<Ctl*>(smem + C::kOffCtl);
   // Per ring slot b, row i: -LSE * log2(e) and -Delta at s_lse / s_delta
-  // [b * kQ + i], 0 for rows past the problem's (whose Q and dO are 0 too, so
-  // that their P and dS reach nothing).
+  // [b * kQ + i], 0 for rows past the problem's.  Their Q and dO are 0 too, so
+  // that without a bias their P is at most 2^0 and reaches nothing; with one it
+  // would be e^bias, which no LSE holds down, and the element-wise warps clear
+  // their mask bits.
   float* s_lse = reinterpret_cast<float*>(smem + C::kOffLse);
   float* s_delta = reinterpret_cast<float*>(smem + C::kOffDelta);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -945,11 +947,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lt = lt0 + tt;
         const int b = lt % kRing;
         const int v = v_next;
-        const uint2 words = next_words;
+        uint2 words = next_words;
         int head = 0, q0 = 0;
         if constexpr (kBias) {
           head = it.h0 + step_head(v);  // hb = 1
           q0 = step_q0(v);
+          if (x.words_t == nullptr) {  // the bits by key end at the last query already
+            words.x &= low_bits(x.Nq - q0);
+            words.y &= low_bits(x.Nq - q0 - 32);
+          }
           if (head != far_head) {
             flush_far();
             far_head = head;
