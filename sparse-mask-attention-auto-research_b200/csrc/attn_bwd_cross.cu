@@ -307,9 +307,10 @@ __global__ void __launch_bounds__(256)
   for (int o = 1; o < kPerRow; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   if (row < rows && (threadIdx.x % kPerRow) == 0) {
     neg_delta[row] = -acc;
-    // -FLT_MAX (a row with no kept key) becomes +inf; such a row has no mask
-    // bit, so its P is 0 by the select and never uses this value.
-    neg_lse2[row] = -(lse[row] * kLog2e);
+    // -FLT_MAX, a row that keeps nothing: -inf, so that P = 2^-inf = 0 also where
+    // no mask says so (scores of -inf, from a table's entries).
+    const float row_lse = lse[row];
+    neg_lse2[row] = row_lse == -FLT_MAX ? -INFINITY : -(row_lse * kLog2e);
   }
 }
 

@@ -1354,7 +1354,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (kX) scan_regs = false;
       if (!kBoolIn && do_scan && need_scan && !scan_regs) prefetch_rows_l1(itn);
       const float inv = (l_out > 0.f) ? (1.f / l_out) : 0.f;
-      const float lse_row = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -FLT_MAX;
+      // kX: a sum that is NaN (of a NaN or infinite score) shows in the LSE, so
+      // that the backward does not take the row for one that keeps nothing.
+      const float lse_row = (kX ? l_run != 0.f : l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -FLT_MAX;
       // The last PV of the item (O complete); a warp-wide wait.
       auto wait_o = [&]() -> bool {
         const bool ready = ok && n > 0 && wait_all(cc.pv_done, (g - 1) & 1);

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
           pack2<BF16>(fmaf(acc[2 * e], inv, -hi.x), fmaf(acc[2 * e + 1], inv, -hi.y));
     }
   }
-  if (m.lse != nullptr && lane == 0) m.lse[row] = l > 0.f ? (M + log2f(l)) * kLn2 : -FLT_MAX;
+  if (m.lse != nullptr && lane == 0) m.lse[row] = l != 0.f ? (M + log2f(l)) * kLn2 : -FLT_MAX;
 }
 
 __global__ void __launch_bounds__(256) fill_kernel(float* x, int64_t n, float v) {

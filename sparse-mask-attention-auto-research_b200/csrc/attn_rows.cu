@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int g = rr / p.Nq;
     const int64_t at = (static_cast<int64_t>(b) * p.H + hkv * p.G + g) * p.Nq + (rr - g * p.Nq);
     if (p.part_ml != nullptr) *reinterpret_cast<float4*>(p.part_ml + at * 4) = make_float4(M, sum, sumr, 0.f);
-    if (p.lse != nullptr) p.lse[at] = sum > 0.f ? (M + log2f(sum)) * kLn2 : -FLT_MAX;
+    if (p.lse != nullptr) p.lse[at] = sum != 0.f ? (M + log2f(sum)) * kLn2 : -FLT_MAX;
   };
   const int64_t n_units = gridDim.x;
   float* ws_ml = p.ws;

@@ -1,12 +1,14 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
-they take: bias tables with large entries.  Bounds as in
+they take: bias tables with large or infinite entries.  Bounds as in
 test_cross_backward_gpu.py."""
+
+import math
 
 import pytest
 import torch
 
-from cross_ref import buckets_of
-from python import relative_bias_attention, sparse_attn_cuda
+from cross_ref import Ref, buckets_of
+from python import cross_attention, relative_bias_attention, sparse_attn_cuda
 from test_cross_attention_gpu import heads, make_mask
 from test_cross_backward_gpu import RefGrads
 
@@ -41,3 +43,51 @@ def test_large_bias_entries(Nq, mask, dtype, entry, D):
     ref = RefGrads(q, k, v, dout, m, add, dtype=dtype).with_table(bucket, 32)
     ref.check_out(out.detach())
     ref.check(dq=dq, dk=dk, dv=dv, dtable=dtable)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("Nq", [5, 70, 200])
+def test_minus_infinity_in_the_table(Nq, D, dtype):
+    """A bucket that a table closes: as if a mask closed it, also where it
+    leaves a row nothing (O = 0 and no gradient, dtable's entry 0)."""
+    B, H, Nk = 2, 2, Nq
+    gen = torch.Generator(device=DEV).manual_seed(65)
+    q, k, v, dout = (heads(gen, B, H, Nq, D, dtype) for _ in range(4))
+    table = torch.randn(32, H, generator=gen, device=DEV).to(dtype)
+    table[0] = -math.inf  # distance 0 and later keys: the first query keeps nothing
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, table)]
+    out = relative_bias_attention(*leaves, bidirectional=False)
+    got = dict(zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, dout)))
+    bucket = buckets_of(Nq, Nk, 32, 128, False)
+    add = table.masked_fill(table == -math.inf, 0.0).double().cpu().t()[:, bucket]
+    ref = RefGrads(q, k, v, dout, (bucket != 0).view(1, 1, Nq, Nk), add, dtype=dtype).with_table(bucket, 32)
+    ref.check_out(out.detach())
+    ref.check(**got)
+    with torch.no_grad():
+        one = relative_bias_attention(q[:, :, :1], k, v, table, bidirectional=False)
+        assert torch.all(one == 0)
+        two = relative_bias_attention(q[:, :, 4:5], k, v, table, bidirectional=False, query_offset=4)
+        Ref(q[:, :, 4:5], k, v, (bucket != 0)[4:5].view(1, 1, 1, Nk), add[:, 4:5]).check_out(two)
+
+
+@pytest.mark.parametrize("Nk", [150, 9000])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_row_without_a_sum_is_not_one_that_keeps_nothing(bad, D, dtype, Nk):
+    """NaN or infinity in a query: NaN in its output, its dq and the gradients
+    of every key it keeps, not zeros; other rows are as without it."""
+    gen = torch.Generator(device=DEV).manual_seed(66)
+    q, dout = heads(gen, 1, 2, 70, D, dtype), heads(gen, 1, 2, 70, D, dtype)
+    k, v = (heads(gen, 1, 2, Nk, D, dtype) for _ in range(2))
+    m = make_mask(gen, "batch", 1, 2, 70, Nk)
+    q[0, 1, 7, 3] = bad
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves, m)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    sparse_attn_cuda.device_status()
+    assert out[0, 1, 7].isnan().all() and dq[0, 1, 7].isnan().all()
+    kept = m[0, 0, 7]
+    assert dk[0, 1][kept].isnan().all() and dv[0, 1][kept].isnan().all()
+    others = torch.arange(70, device=DEV) != 7
+    assert torch.isfinite(out[0, 1][others]).all() and torch.isfinite(out[0, 0]).all()
+    assert all(torch.isfinite(t[0, 0]).all() for t in (dq, dk, dv))
