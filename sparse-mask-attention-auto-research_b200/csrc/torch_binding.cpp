@@ -291,8 +291,10 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
                           current_stream(q)));
     }
     variable_list out_grads = {dq, dk, dv, dtable};
-    // Differentiable once: what is built on these gradients says so when it is differentiated.
-    if (at::GradMode::is_enabled() && grads[0].requires_grad()) {
+    // Differentiable once: what is built on these gradients says so when it is
+    // differentiated.  They depend on q, k, v and the table even where the
+    // incoming gradient is a constant, so create_graph alone decides.
+    if (at::GradMode::is_enabled()) {
       auto error = std::make_shared<torch::autograd::DelayedError>(
           "the gradients of this attention cannot be differentiated again", static_cast<int64_t>(out_grads.size()));
       for (Tensor& t : out_grads)

@@ -1,6 +1,6 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
-they take: bias tables with large or infinite entries.  Bounds as in
-test_cross_backward_gpu.py."""
+they take: bias tables with large or infinite entries, losses on gradients.
+Bounds as in test_cross_backward_gpu.py."""
 
 import math
 
@@ -91,3 +91,27 @@ def test_a_row_without_a_sum_is_not_one_that_keeps_nothing(bad, D, dtype, Nk):
     others = torch.arange(70, device=DEV) != 7
     assert torch.isfinite(out[0, 1][others]).all() and torch.isfinite(out[0, 0]).all()
     assert all(torch.isfinite(t[0, 0]).all() for t in (dq, dk, dv))
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_second_derivatives_of_a_mixed_loss_are_refused(bias):
+    """A penalty on a gradient whose incoming gradient is a constant: it still
+    depends on q, k, v and the table, and must not be dropped in silence."""
+    gen = torch.Generator(device=DEV).manual_seed(63)
+    leaves = [heads(gen, 1, 2, n, 64, F16).requires_grad_(True) for n in (20, 30, 30)]
+    if bias:
+        leaves.append(torch.randn(16, 2, generator=gen, device=DEV).half().requires_grad_(True))
+    attend = relative_bias_attention if bias else cross_attention
+    for leaf in leaves:
+        out = attend(*leaves)
+        g, = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (out.sum() + g.square().sum()).backward()
+    # First derivatives under create_graph are as ever.
+    out = attend(*leaves)
+    plain = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+    kept = torch.autograd.grad(out.sum(), leaves, create_graph=True)
+    for i, (a, b) in enumerate(zip(plain, kept)):
+        if i:  # dq: FP32 adds in another order
+            assert torch.equal(a, b.detach())
