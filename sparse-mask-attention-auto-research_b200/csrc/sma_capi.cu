@@ -439,7 +439,9 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
   int rc = cross_params(args, stream, &p, &empty);
   if (rc != sma::kOk || empty) return rc;
   if (p.P > 0) return fail(sma::kErrArg, "attention: no prefix here");
-  if (args->words && !args->mask) return fail(sma::kErrArg, "attention: words are packed from a mask, and there is none");
+  // (A mask over no keys has no bytes and may have no address.)
+  if (args->words && !args->mask && p.Nk > 0)
+    return fail(sma::kErrArg, "attention: words are packed from a mask, and there is none");
   rc = tile_params(args, &p);
   if (rc == sma::kOk) rc = device_params(&p);
   if (rc != sma::kOk) return rc;

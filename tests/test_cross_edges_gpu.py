@@ -1,6 +1,6 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
-they take: bias tables with large or infinite entries, losses on gradients.
-Bounds as in test_cross_backward_gpu.py."""
+they take: bias tables with large or infinite entries, losses on gradients,
+no keys.  Bounds as in test_cross_backward_gpu.py."""
 
 import math
 
@@ -115,3 +115,27 @@ def test_second_derivatives_of_a_mixed_loss_are_refused(bias):
     for i, (a, b) in enumerate(zip(plain, kept)):
         if i:  # dq: FP32 adds in another order
             assert torch.equal(a, b.detach())
+
+
+@pytest.mark.parametrize("Nq", [1, 40, 200])
+@pytest.mark.parametrize("mask", ["padding", "heads", "shared"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_no_keys_under_a_mask(bias, mask, Nq):
+    """Zeros, as without a mask: with and without gradients."""
+    gen = torch.Generator(device=DEV).manual_seed(64)
+    q = heads(gen, 2, 4, Nq, 64, F16)
+    k = torch.empty(2, 2, 0, 64, device=DEV, dtype=F16)
+    table = torch.randn(16, 4, generator=gen, device=DEV).half()
+    m = make_mask(gen, mask, 2, 4, Nq, 5)[..., :0]
+
+    def run(*leaves):
+        return relative_bias_attention(*leaves, m) if bias else cross_attention(*leaves, m)
+
+    leaves = (q, k, k.clone(), table) if bias else (q, k, k.clone())
+    assert torch.equal(run(*leaves), torch.zeros_like(q))
+    leaves = [t.clone().requires_grad_(True) for t in leaves]
+    out = run(*leaves)
+    assert torch.equal(out.detach(), torch.zeros_like(q))
+    for leaf, g in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
+        assert g.shape == leaf.shape and torch.all(g == 0)
+    sparse_attn_cuda.device_status()
