@@ -282,7 +282,14 @@ SMA_API int sma_prefix_attn_fwd(const sma_attn_args* args, void* stream);
 SMA_API int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
                                float* scratch, void* stream);
 
-/* Floats of scratch sma_cross_attn_bwd needs; -1 for arguments that it refuses. */
+/*
+ * The same with dtable in FP32, for tables that are kept in FP32 (bias_table
+ * is of `dtype` here too): the sum over all queries is not rounded.
+ */
+SMA_API int sma_cross_attn_bwd_f32_table(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv,
+                                         float* dtable, float* scratch, void* stream);
+
+/* Floats of scratch either of them needs; -1 for arguments that it refuses. */
 SMA_API int64_t sma_cross_attn_bwd_scratch(const sma_attn_args* args);
 
 /*

@@ -1301,13 +1301,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 // blocks near the diagonal, [b][kb] by [d in the bucket's interval], and for
 // the last bucket of a side the sums of the blocks beyond.  Every thread adds
 // in a fixed order and the threads are added in a fixed tree, so the result
-// does not depend on timing; FP32 throughout, rounded once to the table's type.
+// does not depend on timing; FP32 throughout, rounded once to the table's type
+// T (FP32 tables: not at all; a sum over all queries of the batch passes the
+// range of fp16 where its terms do not).
 // Bound by the latency of its gathers (12 us at B4 H16 N1024, 3.7 MB of sums).
 constexpr int kReduceThreads = 256;
 
-template <bool BF16>
+template <typename T>
 __global__ void __launch_bounds__(kReduceThreads)
-    bias_reduce_kernel(const __grid_constant__ BwdGeo x, const __grid_constant__ BiasSpec s, void* dtable) {
+    bias_reduce_kernel(const __grid_constant__ BwdGeo x, const __grid_constant__ BiasSpec s, T* __restrict__ dtable) {
   __shared__ float part[kReduceThreads / 32];
   const int h = blockIdx.x, bucket = blockIdx.y;
   const bool high = bucket >= s.side;  // two-sided: keys after the query
@@ -1373,9 +1375,10 @@ __global__ void __launch_bounds__(kReduceThreads)
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kReduceThreads / 32; ++w) acc += part[w];
-    const int64_t at = static_cast<int64_t>(bucket) * s.H + h;
-    if constexpr (BF16) static_cast<__nv_bfloat16*>(dtable)[at] = __float2bfloat16_rn(acc);
-    else static_cast<__half*>(dtable)[at] = __float2half_rn(acc);
+    T& to = dtable[static_cast<int64_t>(bucket) * s.H + h];
+    if constexpr (std::is_same_v<T, float>) to = acc;
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) to = __float2bfloat16_rn(acc);
+    else to = __float2half_rn(acc);
   }
 }
 
@@ -1538,7 +1541,11 @@ int launch(const CrossParams& p, const CrossGrads& g, BwdGeo x, int device, cons
     // Not launched early like the others: its few blocks would gather on the
     // SMs that cross_dq_kernel leaves first (B4 H16 N1024 D64 causal, a whole
     // training pass: 158 us, launched early 169).
-    bias_reduce_kernel<BF16><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, g.dtable);
+    using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+    if (g.dtable_f32)
+      bias_reduce_kernel<float><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, static_cast<float*>(g.dtable));
+    else
+      bias_reduce_kernel<T><<<grid, kReduceThreads, 0, p.stream>>>(x, p.bias, static_cast<T*>(g.dtable));
   }
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {

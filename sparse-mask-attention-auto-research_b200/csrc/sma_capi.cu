@@ -428,6 +428,30 @@ int write_nothing(const sma::CrossParams& p) {
   return e == cudaSuccess ? sma::kOk : fail_cuda(e, "cudaMemsetAsync");
 }
 
+int cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
+                   bool dtable_f32, float* scratch, void* stream) {
+  NvtxRange range("sma_cross_attn_bwd");
+  sma::CrossParams p{};
+  bool empty = false;
+  int rc = cross_params(args, stream, &p, &empty);
+  if (rc != sma::kOk) return rc;
+  if (empty || p.Nk == 0) return fail(sma::kErrArg, "backward: no queries or no keys");
+  if (p.P > 0 || p.lengths) return fail(sma::kErrArg, "backward: no prefix and no lengths");
+  rc = tile_params(args, &p);
+  if (rc != sma::kOk) return rc;
+  if (!p.lse || !p.out_lo || !dout || !dq || !dk || !dv || !scratch || (p.bias.table && !dtable))
+    return fail(sma::kErrArg, "backward: null pointer");
+  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(scratch))
+    return fail(sma::kErrArg, "backward: dout/dq/dk/dv/scratch must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(dtable) & (dtable_f32 ? 3u : 1u)) return fail(sma::kErrArg, "backward: misaligned dtable");
+  rc = device_params(&p);
+  if (rc != sma::kOk) return rc;
+  const sma::CrossGrads g{dout, dq, dk, dv, dtable, dtable_f32, scratch};
+  const char* msg = nullptr;
+  rc = sma::launch_attn_cross_bwd(p, g, &msg);
+  return rc == sma::kOk ? rc : fail(rc, msg);
+}
+
 }  // namespace
 
 extern "C" {
@@ -453,26 +477,12 @@ int sma_cross_attn_fwd(const sma_attn_args* args, void* stream) {
 
 int sma_cross_attn_bwd(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv, void* dtable,
                        float* scratch, void* stream) {
-  NvtxRange range("sma_cross_attn_bwd");
-  sma::CrossParams p{};
-  bool empty = false;
-  int rc = cross_params(args, stream, &p, &empty);
-  if (rc != sma::kOk) return rc;
-  if (empty || p.Nk == 0) return fail(sma::kErrArg, "backward: no queries or no keys");
-  if (p.P > 0 || p.lengths) return fail(sma::kErrArg, "backward: no prefix and no lengths");
-  rc = tile_params(args, &p);
-  if (rc != sma::kOk) return rc;
-  if (!p.lse || !p.out_lo || !dout || !dq || !dk || !dv || !scratch || (p.bias.table && !dtable))
-    return fail(sma::kErrArg, "backward: null pointer");
-  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(scratch))
-    return fail(sma::kErrArg, "backward: dout/dq/dk/dv/scratch must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(dtable) & 1u) return fail(sma::kErrArg, "backward: misaligned dtable");
-  rc = device_params(&p);
-  if (rc != sma::kOk) return rc;
-  const sma::CrossGrads g{dout, dq, dk, dv, dtable, scratch};
-  const char* msg = nullptr;
-  rc = sma::launch_attn_cross_bwd(p, g, &msg);
-  return rc == sma::kOk ? rc : fail(rc, msg);
+  return cross_attn_bwd(args, dout, dq, dk, dv, dtable, false, scratch, stream);
+}
+
+int sma_cross_attn_bwd_f32_table(const sma_attn_args* args, const void* dout, void* dq, void* dk, void* dv,
+                                 float* dtable, float* scratch, void* stream) {
+  return cross_attn_bwd(args, dout, dq, dk, dv, dtable, true, scratch, stream);
 }
 
 int64_t sma_cross_attn_bwd_scratch(const sma_attn_args* args) {

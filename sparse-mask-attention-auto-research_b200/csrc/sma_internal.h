@@ -164,6 +164,7 @@ struct CrossGrads {
   void* dk;          // [B, Hkv, Nk, D]
   void* dv;
   void* dtable;      // [buckets, H], with a bias
+  bool dtable_f32;   // dtable is FP32, else of the inputs' type
   float* scratch;    // cross_bwd_scratch_floats elements
 };
 int64_t cross_bwd_scratch_floats(const CrossParams& p);

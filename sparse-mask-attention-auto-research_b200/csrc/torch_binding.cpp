@@ -38,6 +38,7 @@ struct Api {
   decltype(&sma_cross_attn_fwd) cross = nullptr;
   decltype(&sma_prefix_attn_fwd) prefix = nullptr;
   decltype(&sma_cross_attn_bwd) cross_bwd = nullptr;
+  decltype(&sma_cross_attn_bwd_f32_table) cross_bwd_f32_table = nullptr;
   decltype(&sma_cross_attn_bwd_scratch) cross_bwd_scratch = nullptr;
   decltype(&sma_last_error) last_error = nullptr;
 } api;
@@ -123,6 +124,11 @@ Mask mask_of(const std::optional<Tensor>& mask) {
   m.t = mask->size(3) > 1 && mask->stride(3) != 1 ? mask->contiguous() : *mask;
   for (int i = 0; i < 3; ++i) m.stride[i] = m.t.size(i) == 1 ? 0 : m.t.stride(i);
   return m;
+}
+
+// A bias table as the kernels read it, of q's type.
+Tensor table_of(const std::optional<Tensor>& table, const Tensor& q) {
+  return table.has_value() ? table->to(q.scalar_type()).contiguous() : Tensor();
 }
 
 // A relative position bias; its table and offsets are passed beside it.
@@ -243,6 +249,7 @@ struct Plan : torch::CustomClassHolder {
   Bias bias;
   Layout layout;
   std::array<int64_t, 3> mask_stride{};
+  bool table_f32 = false;  // the caller's table, and so its gradient
 };
 
 // Autograd node of cross_attention (no table) and relative_bias_attention.
@@ -251,13 +258,14 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
                         const std::optional<Tensor>& table_, const std::optional<Tensor>& mask_,
                         const std::optional<Tensor>& offsets_, double scale, const Bias& bias) {
     const Tensor q = strided(q_), k = strided(k_), v = strided(v_);
-    const Tensor table = table_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
+    const Tensor table = table_of(table_, q), offsets = offsets_.value_or(Tensor());
     const Mask mask = mask_of(mask_);
     auto plan = c10::make_intrusive<Plan>();
     plan->scale = scale;
     plan->bias = bias;
     plan->layout = layout_of(q, k, mask.on(), mask.stride, bias, true);
     plan->mask_stride = mask.stride;
+    plan->table_f32 = table_.has_value() && table_->scalar_type() == at::kFloat;
     const Tensor out = empty(q);
     const Tensor saved = tiles_forward(q, k, v, out, scale, mask, bias, table, offsets, plan->layout);
     ctx->save_for_backward({q, k, v, out, saved, table, offsets});
@@ -274,7 +282,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     Tensor dout = grads[0].contiguous();
     if (!aligned16(dout.const_data_ptr())) dout = dout.clone();
     Tensor dq = empty(q), dk = empty(k), dv = empty(k), dtable;
-    if (table.defined()) dtable = empty(table);
+    if (table.defined()) dtable = at::empty(table.sizes(), plan.table_f32 ? table.options().dtype(at::kFloat) : table.options());
     if (q.numel() == 0 || k.numel() == 0) {
       for (Tensor* t : {&dq, &dk, &dv, &dtable})
         if (t->defined()) t->zero_();
@@ -286,9 +294,14 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
       const int64_t floats = api.cross_bwd_scratch(&a);
       TORCH_CHECK(floats >= 0, "backward: unsupported arguments");
       const Tensor scratch = at::empty({floats}, q.options().dtype(at::kFloat));
-      check(api.cross_bwd(&a, dout.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                          dtable.defined() ? dtable.data_ptr() : nullptr, scratch.data_ptr<float>(),
-                          current_stream(q)));
+      if (plan.table_f32) {
+        check(api.cross_bwd_f32_table(&a, dout.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                      dtable.data_ptr<float>(), scratch.data_ptr<float>(), current_stream(q)));
+      } else {
+        check(api.cross_bwd(&a, dout.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                            dtable.defined() ? dtable.data_ptr() : nullptr, scratch.data_ptr<float>(),
+                            current_stream(q)));
+      }
     }
     variable_list out_grads = {dq, dk, dv, dtable};
     // Differentiable once: what is built on these gradients says so when it is
@@ -306,7 +319,8 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
   }
 };
 
-// out [B, H, Nq, D] of checked fp16 / bf16 inputs.
+// out [B, H, Nq, D] of checked fp16 / bf16 inputs.  `table` is the caller's: of
+// q's type or FP32.
 Tensor attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const std::optional<Tensor>& table,
                  const std::optional<Tensor>& mask_, const std::optional<Tensor>& offsets, double scale,
                  const Bias& bias) {
@@ -321,7 +335,7 @@ Tensor attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const std
   const Tensor q = strided(q_), k = strided(k_), v = strided(v_);
   const Mask mask = mask_of(mask_);
   const Tensor out = empty(q);
-  const Tensor tab = table.value_or(Tensor()), off = offsets.value_or(Tensor());
+  const Tensor tab = table_of(table, q), off = offsets.value_or(Tensor());
   if (few_rows(q, k, mask, bias)) {
     sma_attn_args a = args_of(q, k, v, out, scale);
     if (mask.on()) {
@@ -350,14 +364,14 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
 }
 
 // `starts`: host address of one side's `side` bucket starts (copied here).
-Tensor relative_bias_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table_,
+Tensor relative_bias_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
                                const std::optional<Tensor>& mask, uintptr_t starts, int64_t side, bool two_sided,
                                int64_t offset, const std::optional<Tensor>& offsets_, std::optional<double> scale_) {
   check_qkv(q, k, v);
   if (mask.has_value()) check_mask(*mask, q, k);
-  TORCH_CHECK(table_.device() == q.device(), "table must be on the same device as q");
-  TORCH_CHECK(table_.dim() == 2 && table_.size(1) == q.size(1), "table must be [num_buckets, H]");
-  TORCH_CHECK(table_.scalar_type() == q.scalar_type() || table_.scalar_type() == at::kFloat,
+  TORCH_CHECK(table.device() == q.device(), "table must be on the same device as q");
+  TORCH_CHECK(table.dim() == 2 && table.size(1) == q.size(1), "table must be [num_buckets, H]");
+  TORCH_CHECK(table.scalar_type() == q.scalar_type() || table.scalar_type() == at::kFloat,
               "table must have the dtype of q or be FP32");
   std::optional<Tensor> offsets = offsets_;
   if (offsets.has_value()) {
@@ -375,10 +389,9 @@ Tensor relative_bias_attention(const Tensor& q, const Tensor& k, const Tensor& v
   bias.offset = offset;
   std::copy_n(reinterpret_cast<const int32_t*>(starts), side, bias.starts.begin());
   const bool fp32 = q.scalar_type() == at::kFloat;
-  const auto type = fp32 ? at::kBFloat16 : q.scalar_type();
-  const Tensor table = table_.to(type).contiguous();
   if (!fp32) return attention(q, k, v, table, mask, offsets, scale, bias);
-  return attention(q.to(type), k.to(type), v.to(type), table, mask, offsets, scale, bias).to(at::kFloat);
+  return attention(q.to(at::kBFloat16), k.to(at::kBFloat16), v.to(at::kBFloat16), table, mask, offsets, scale, bias)
+      .to(at::kFloat);
 }
 
 Tensor shared_prefix_attention(const Tensor& q_, const Tensor& kp_, const Tensor& vp_, const Tensor& k_,
@@ -428,6 +441,7 @@ void bind(const py::dict& at, py::object sma_error) {
   api.cross = reinterpret_cast<decltype(api.cross)>(get("sma_cross_attn_fwd"));
   api.prefix = reinterpret_cast<decltype(api.prefix)>(get("sma_prefix_attn_fwd"));
   api.cross_bwd = reinterpret_cast<decltype(api.cross_bwd)>(get("sma_cross_attn_bwd"));
+  api.cross_bwd_f32_table = reinterpret_cast<decltype(api.cross_bwd_f32_table)>(get("sma_cross_attn_bwd_f32_table"));
   api.cross_bwd_scratch = reinterpret_cast<decltype(api.cross_bwd_scratch)>(get("sma_cross_attn_bwd_scratch"));
   api.last_error = reinterpret_cast<decltype(api.last_error)>(get("sma_last_error"));
   static py::object error;

@@ -70,6 +70,7 @@ SIGNATURES = {
     "sma_rows_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_cross_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_cross_attn_bwd": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sma_cross_attn_bwd_f32_table": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "sma_cross_attn_bwd_scratch": (_i64, [ctypes.c_char_p]),
     "sma_prefix_attn_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "sma_device_status": (ctypes.c_int, [_vp, ctypes.c_int]),

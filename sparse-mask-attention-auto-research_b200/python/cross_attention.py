@@ -71,7 +71,8 @@ def relative_bias_attention(q, k, v, table, mask=None, bidirectional=True, max_d
     query_offset), h] is added to the scaled score of query i and key j of
     head h.
 
-    ``table``: [num_buckets, H], of q's dtype or FP32 (rounded to q's dtype).
+    ``table``: [num_buckets, H], of q's dtype or FP32 (the kernels read it
+    rounded to q's dtype; its gradient, a sum over all queries, stays FP32).
     ``bidirectional``: half of the buckets are for keys after the query; else
     those keys all count as distance 0.  Half of a side's buckets hold one
     distance each, the others grow geometrically up to ``max_distance``, and

@@ -1,6 +1,6 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
-they take: bias tables with large or infinite entries, losses on gradients,
-no keys.  Bounds as in test_cross_backward_gpu.py."""
+they take: bias tables with large or infinite entries, FP32 tables, losses on
+gradients, no keys.  Bounds as in test_cross_backward_gpu.py."""
 
 import math
 
@@ -139,3 +139,52 @@ def test_no_keys_under_a_mask(bias, mask, Nq):
     for leaf, g in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
         assert g.shape == leaf.shape and torch.all(g == 0)
     sparse_attn_cuda.device_status()
+
+
+def coherent(dtype=F16):
+    """A call whose dtable is large: all of a bucket's dS have one sign."""
+    gen = torch.Generator(device=DEV).manual_seed(61)
+    q, k = heads(gen, 4, 2, 300, 64, dtype), heads(gen, 4, 2, 300, 64, dtype)
+    v = torch.where(torch.arange(300, device=DEV) < 150, 0.5, -0.5)[:, None].expand(4, 2, 300, 64).to(dtype).contiguous()
+    dout = (500 + torch.randn(4, 2, 300, 64, generator=gen, device=DEV)).to(dtype)
+    table = torch.randn(32, 2, generator=gen, device=DEV).to(dtype)
+    return q, k, v, table, dout
+
+
+def test_fp32_table_gets_an_fp32_gradient():
+    """Not by way of the queries' type: beyond its range, and not rounded to it."""
+    q, k, v, table, dout = coherent()
+    leaf = table.float().requires_grad_(True)
+    got, = torch.autograd.grad(relative_bias_attention(q, k, v, leaf), leaf, dout)
+    assert got.dtype == torch.float32
+    bucket = buckets_of(300, 300, 32, 128, True)
+    ref = RefGrads(q, k, v, dout, None, table.double().cpu().t()[:, bucket], dtype=F16).with_table(bucket, 32)
+    want = ref.grads["dtable"]
+    assert float(want.abs().max()) > 2 * torch.finfo(F16).max
+    ref.check(dtable=got)
+    small = (dout.float() / 512).to(F16)
+    got, = torch.autograd.grad(relative_bias_attention(q, k, v, leaf), leaf, small)
+    half = table.clone().requires_grad_(True)
+    rounded, = torch.autograd.grad(relative_bias_attention(q, k, v, half), half, small)
+    assert rounded.dtype == F16 and torch.isfinite(rounded).all()
+    assert torch.equal(got.half(), rounded) and not torch.equal(got, rounded.float())
+
+
+@pytest.mark.parametrize("inputs", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("turned", [False, True])
+def test_fp32_tables_of_every_input_type(inputs, turned):
+    """Contiguous or a transposed view; the parameter's own gradient."""
+    gen = torch.Generator(device=DEV).manual_seed(62)
+    kernel = BF16 if inputs == torch.float32 else inputs
+    q, k, v, dout = (heads(gen, 2, 4, n, 64, kernel) for n in (70, 133, 133, 70))
+    table = torch.randn(16, 4, generator=gen, device=DEV)
+    leaf = (table.t().contiguous() if turned else table.clone()).requires_grad_(True)
+    x = [t.to(inputs) for t in (q, k, v)]
+    out = relative_bias_attention(*x, leaf.t() if turned else leaf, query_offset=63)
+    assert out.dtype == inputs
+    out.backward(dout.to(inputs))
+    assert leaf.grad.dtype == torch.float32 and leaf.grad.shape == leaf.shape
+    bucket = buckets_of(70, 133, 16, 128, True, 63)
+    add = table.to(kernel).double().cpu().t()[:, bucket]
+    ref = RefGrads(q, k, v, dout, None, add, dtype=kernel).with_table(bucket, 16)
+    ref.check(dtable=leaf.grad.t() if turned else leaf.grad)
