@@ -220,7 +220,9 @@ bool few_rows(const Tensor& q, const Tensor& k, const Mask& mask, const Bias& bi
   if (Nk > SMA_MAX_SEQ_LEN) return true;
   const int64_t rows = H / std::max<int64_t>(Hkv, 1) * Nq;
   if (rows <= 16 || rows > 128) return rows <= 16;
-  if (bias.on || (mask.on() && (mask.t.size(1) != 1 || mask.t.size(2) != 1))) return false;
+  // A mask that all rows of a key head share may still be an expanded view.
+  const bool own_rows = mask.on() && ((Nq > 1 && mask.stride[2] != 0) || (H > Hkv && mask.stride[1] != 0));
+  if (bias.on || own_rows) return false;
   const double tiles = static_cast<double>((rows + 15) / 16);
   return static_cast<double>(B * Hkv * Nk * D) * ((D == 64 ? 0.6 : 0.75) * tiles - 1.0) <= 12e6;
 }

@@ -1,6 +1,6 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
 they take: bias tables with large or infinite entries, FP32 tables, losses on
-gradients, no keys.  Bounds as in test_cross_backward_gpu.py."""
+gradients, no keys, expanded masks.  Bounds as in test_cross_backward_gpu.py."""
 
 import math
 
@@ -188,3 +188,16 @@ def test_fp32_tables_of_every_input_type(inputs, turned):
     add = table.to(kernel).double().cpu().t()[:, bucket]
     ref = RefGrads(q, k, v, dout, None, add, dtype=kernel).with_table(bucket, 16)
     ref.check(dtable=leaf.grad.t() if turned else leaf.grad)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk", [(2, 4, 2, 1, 300), (2, 4, 4, 64, 500), (2, 8, 2, 10, 700), (1, 4, 2, 200, 300)])
+def test_expanded_masks_are_taken_as_broadcast(B, H, Hkv, Nq, Nk):
+    """A padding mask expanded over heads and queries: the same kernel, so the
+    same bits."""
+    gen = torch.Generator(device=DEV).manual_seed(67)
+    q = heads(gen, B, H, Nq, 64, F16)
+    k, v = (heads(gen, B, Hkv, Nk, 64, F16) for _ in range(2))
+    m = make_mask(gen, "padding", B, H, Nq, Nk)
+    want = cross_attention(q, k, v, m)
+    assert torch.equal(cross_attention(q, k, v, m.expand(B, H, Nq, Nk)), want)
+    Ref(q, k, v, m).check_out(want)
