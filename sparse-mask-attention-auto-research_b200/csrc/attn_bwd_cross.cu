@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // bytes into dS's two 64-query tiles and K.
             const int b = lp & 1;
             if (lp >= 2 && !wait_all(ctl.dq_free[b], ((lp >> 1) - 1) & 1)) return false;
-                const uint64_t dPair = smem_desc_sw128(base + C::kOffDS + b * 2 * C::kDSBytes, C::kDSBytes, 1024);
+            const uint64_t dPair = smem_desc_sw128(base + C::kOffDS + b * 2 * C::kDSBytes, C::kDSBytes, 1024);
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk)
               mma_ss_warp(tmem + C::col_dq(b), step(dPair, kk * 2048), step(dK, kk * 2048), idesc_q, kk > 0 ? 1u : 0u);
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = false;
               break;
             }
-                const uint32_t sQ = base + C::kOffQ + slot * C::kQBytes, sDO = base + C::kOffDO + slot * C::kQBytes;
+            const uint32_t sQ = base + C::kOffQ + slot * C::kQBytes, sDO = base + C::kOffDO + slot * C::kQBytes;
             const uint64_t dK = smem_desc_sw128(sK, 16, 1024), dV = smem_desc_sw128(sV, 16, 1024);
             const uint64_t dQ = smem_desc_sw128(sQ, 16, 1024), dDO = smem_desc_sw128(sDO, 16, 1024);
             // 16 head dims per instruction: swizzle chunk kk / 4 of the rows, 32 bytes into it.

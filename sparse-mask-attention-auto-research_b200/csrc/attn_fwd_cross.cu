@@ -59,7 +59,7 @@ __device__ __forceinline__ void expand_bias(const ExpandParams& e, int block, in
 // words a thread in flight instead of four 2 us more, eight 4 us more).
 constexpr int kPackThreads = 256;
 constexpr int kPackWords = 256;   // words of a row per CTA, at most
-constexpr int kPackPackRounds = 4;    // words per thread with their loads in flight
+constexpr int kPackRounds = 4;    // words per thread with their loads in flight
 
 struct PackParams {
   const uint8_t* mask;
@@ -80,7 +80,7 @@ template <bool kAligned>
 __global__ void __launch_bounds__(kPackThreads)
     pack_tiles_kernel(const __grid_constant__ PackParams p, const __grid_constant__ ExpandParams e) {
   pdl_launch_dependents();
-  constexpr int kPackRounds = kPackPackRounds, kVecs = kAligned ? 2 : 3;
+  constexpr int kVecs = kAligned ? 2 : 3;
   __shared__ uint32_t live[kPackWords / 2 / 32];  // a key tile is 2 or 4 words
   __shared__ uint32_t kept[kPackWords];
   if (static_cast<int>(blockIdx.x) < e.blocks) {
