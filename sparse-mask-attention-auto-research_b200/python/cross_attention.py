@@ -15,6 +15,15 @@ nothing gives 0) are those of ``sparse_attention``.  Masks broadcast:
 Inputs need not be contiguous: views with a contiguous last axis and 16-byte
 steps (such as a [B, N, H, D] projection transposed) are read in place, others
 are copied.  Work is enqueued on the current stream of the tensors' device.
+
+Keys that no query keeps may hold anything, NaN and infinities included;
+under gradients that holds behind a padding mask, and every other key, query
+and incoming gradient must be finite.  A gradient cannot be differentiated
+again (refused).  With gradients at most 65536 keys, and 2048 steps of 64
+queries over the heads that share a key head.  Without, past 65536 keys they
+are read again for every 16 query rows of a key head instead of every 128:
+B1 H8 D128 with 1024 queries takes 0.36 ms over 65536 keys and 1.64 over one
+more, with 16 queries 0.06 either way.
 """
 
 import ctypes

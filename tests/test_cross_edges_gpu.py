@@ -1,6 +1,6 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
 they take: bias tables with large or infinite entries, FP32 tables, losses on
-gradients, no keys, expanded masks.  Bounds as in test_cross_backward_gpu.py."""
+gradients, no keys, long ones, expanded masks.  Bounds as in test_cross_backward_gpu.py."""
 
 import math
 
@@ -201,3 +201,25 @@ def test_expanded_masks_are_taken_as_broadcast(B, H, Hkv, Nq, Nk):
     want = cross_attention(q, k, v, m)
     assert torch.equal(cross_attention(q, k, v, m.expand(B, H, Nq, Nk)), want)
     Ref(q, k, v, m).check_out(want)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("kind", ["none", "padding", "heads", "bias"])
+def test_more_keys_than_the_tiles_take(kind, D, dtype):
+    """Past 65536 keys every forward streams them."""
+    Nq, Nk = 33, 65536 + 77
+    gen = torch.Generator(device=DEV).manual_seed(68)
+    q = heads(gen, 1, 2, Nq, D, dtype)
+    k, v = (heads(gen, 1, 1, Nk, D, dtype) for _ in range(2))
+    m, add = make_mask(gen, "none" if kind == "bias" else kind, 1, 2, Nq, Nk), None
+    if kind == "bias":
+        table = torch.randn(32, 2, generator=gen, device=DEV).to(dtype)
+        add = table.double().cpu().t()[:, buckets_of(Nq, Nk, 32, 128, True, 65500)]
+        out = relative_bias_attention(q, k, v, table, query_offset=65500)
+    else:
+        out = cross_attention(q, k, v, m)
+    sparse_attn_cuda.device_status()
+    Ref(q, k, v, m, add).check_out(out)
+    leaf = q.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="65536"):
+        cross_attention(leaf, k, v, m)
