@@ -501,11 +501,10 @@ __global__ void __launch_bounds__(BwdCfg<D>::kThreads, 1)
     if (!ok && lane == 0) {
       fail();
       // Let the copies this warp started land before the CTA exits.
-      uint32_t zero = 0;
       for (int jj = li - kKVBufs; jj < li; ++jj)
-        if (jj >= 0) mbar_wait_bounded(smem_u32(&ctl.kv_full[jj % kKVBufs]), (jj / kKVBufs) & 1, &zero, timeout_ns);
+        if (jj >= 0) mbar_drain(smem_u32(&ctl.kv_full[jj % kKVBufs]), (jj / kKVBufs) & 1, timeout_ns);
       for (int g = last_copy - kQBufs + 1; g <= last_copy; ++g)
-        if (g >= 0) mbar_wait_bounded(smem_u32(&ctl.ld_full[g % kQBufs]), (g / kQBufs) & 1, &zero, timeout_ns);
+        if (g >= 0) mbar_drain(smem_u32(&ctl.ld_full[g % kQBufs]), (g / kQBufs) & 1, timeout_ns);
     }
   } else if (warp == C::kMmaWarp) {
     // ================================================================ MMA issuer
@@ -664,8 +663,7 @@ __global__ void __launch_bounds__(BwdCfg<D>::kThreads, 1)
       if (!ok) fail();
       // Every MMA this thread issued must complete before TMEM is released.
       mma_commit(smem_u32(&ctl.drain));
-      uint32_t zero = 0;
-      mbar_wait_bounded(smem_u32(&ctl.drain), 0, &zero, timeout_ns);
+      mbar_drain(smem_u32(&ctl.drain), 0, timeout_ns);
     }
   } else if (warp == C::kScanWarp) {
     // ================================================================ scanner

@@ -595,11 +595,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) {
       fail();
       // Let the copies this warp started land before the CTA exits.
-      uint32_t zero = 0;
       for (int jj = li - C::kKVBufs; jj < li; ++jj)
-        if (jj >= 0) mbar_wait_bounded(smem_u32(&ctl.kv_full[jj % C::kKVBufs]), (jj / C::kKVBufs) & 1, &zero, timeout_ns);
+        if (jj >= 0) mbar_drain(smem_u32(&ctl.kv_full[jj % C::kKVBufs]), (jj / C::kKVBufs) & 1, timeout_ns);
       for (int g = lt - kRing; g < lt; ++g)
-        if (g >= 0) mbar_wait_bounded(smem_u32(&ctl.ld_full[g % kRing]), (g / kRing) & 1, &zero, timeout_ns);
+        if (g >= 0) mbar_drain(smem_u32(&ctl.ld_full[g % kRing]), (g / kRing) & 1, timeout_ns);
     }
   } else if (warp == kMmaWarp) {
     // ================================================================ MMA issuer
@@ -764,8 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0) fail();
       // Every MMA this thread issued must complete before TMEM is released.
       mma_commit_warp(smem_u32(&ctl.drain));
-      uint32_t zero = 0;
-      mbar_wait_bounded(smem_u32(&ctl.drain), 0, &zero, timeout_ns);
+      mbar_drain(smem_u32(&ctl.drain), 0, timeout_ns);
     }
   } else if (warp == kScanWarp) {
     // ================================================================ scanner

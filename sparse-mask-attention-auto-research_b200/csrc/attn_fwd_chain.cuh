@@ -688,13 +688,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) {
         fail();
         // Let the copies this thread started land before the CTA exits.
-        uint32_t zero = 0;
         for (uint32_t x = (gk > static_cast<uint32_t>(kStages) ? gk - kStages : 0u); x < gk; ++x)
-          mbar_wait_bounded(smem_u32(&cc.k_full[x % kStages]), (x / kStages) & 1, &zero, timeout_ns);
+          mbar_drain(smem_u32(&cc.k_full[x % kStages]), (x / kStages) & 1, timeout_ns);
         for (uint32_t x = (gv > static_cast<uint32_t>(kStages) ? gv - kStages : 0u); x < gv; ++x)
-          mbar_wait_bounded(smem_u32(&cc.v_full[x % kStages]), (x / kStages) & 1, &zero, timeout_ns);
+          mbar_drain(smem_u32(&cc.v_full[x % kStages]), (x / kStages) & 1, timeout_ns);
         for (uint32_t q = (q_count > static_cast<uint32_t>(C::kQBufs) ? q_count - C::kQBufs : 0u); q < q_count; ++q)
-          mbar_wait_bounded(smem_u32(&cc.q_full[q % C::kQBufs]), (q / C::kQBufs) & 1, &zero, timeout_ns);
+          mbar_drain(smem_u32(&cc.q_full[q % C::kQBufs]), (q / C::kQBufs) & 1, timeout_ns);
       }
     }
   } else if (warp == 10 || warp == 11) {
@@ -798,8 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) fail();
       // Every MMA this thread issued must complete before TMEM is released.
       mma_commit(smem_u32(&cc.drain));
-      uint32_t zero = 0;
-      mbar_wait_bounded(smem_u32(&cc.drain), 0, &zero, timeout_ns);
+      mbar_drain(smem_u32(&cc.drain), 0, timeout_ns);
     }
   } else {
     // ================================================================ softmax

@@ -455,9 +455,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (!ok && lane == 0) {
     ctl.abort_flag = 1;
     atomicOr(p.err_word, kDevErrTimeout);
-    uint32_t zero = 0;  // the copies in flight land before the block leaves
+    // The copies in flight land before the block leaves.
     for (; n_used < n_issued; ++n_used)
-      mbar_wait_bounded(smem_u32(&ctl.full[warp][n_used % kStages]), (n_used / kStages) & 1, &zero, p.timeout_ns);
+      mbar_drain(smem_u32(&ctl.full[warp][n_used % kStages]), (n_used / kStages) & 1, p.timeout_ns);
   }
   __syncwarp();
 
@@ -480,7 +480,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       *reinterpret_cast<float2*>(po + r * D + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * u], o[n][2 * u + 1]);
   }
   __syncthreads();
-  if (ctl.abort_flag != 0u) return;
+  if (ctl.abort_flag != 0u) {
+    // Counted all the same: a replay of the launch uses the counter again.
+    if (threadIdx.x == 0 && p.pieces > 1 && claim_last_piece(p.cnt + item, p.epoch, p.pieces))
+      atomicExch(p.cnt + item, 0ull);
+    return;
+  }
   const int rows = min(kRows, p.R - rt * kRows);
   constexpr int kVec = D / 4;  // float4 per row
   // Writes row r's column group x: normalised, in the inputs' type, or as a

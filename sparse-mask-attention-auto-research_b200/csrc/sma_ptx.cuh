@@ -91,6 +91,15 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   }
 }
 
+// Before a CTA leaves: waits for copies or products that it has started itself.
+// They complete without anyone's help, so the limit is 2^31 ns or more and not
+// the caller's alone (sma_set_wait_timeout_ns), which may be shorter than a
+// load: a copy must not land in shared memory that another CTA has by then.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t budget_ns) {
+  uint32_t never = 0;
+  mbar_wait_bounded(bar, parity, &never, budget_ns | (1ull << 31));
+}
+
 // ---------------------------------------------------------------- register reallocation
 // Moves registers between the warps of a CTA: a warp lowers its limit to N
 // (freeing registers) or raises it to N (waiting until enough are free).
