@@ -1,6 +1,7 @@
 """Calls of cross_attention and relative_bias_attention at the edges of what
-they take: bias tables with large or infinite entries, FP32 tables, losses on
-gradients, no keys, long ones, expanded masks.  Bounds as in test_cross_backward_gpu.py."""
+they take: bias tables with large, infinite or FP32 entries, losses on
+gradients, no keys and more than the tiles take, expanded masks.  Bounds as in
+test_cross_backward_gpu.py."""
 
 import math
 
@@ -223,3 +224,32 @@ def test_more_keys_than_the_tiles_take(kind, D, dtype):
     leaf = q.clone().requires_grad_(True)
     with pytest.raises(RuntimeError, match="65536"):
         cross_attention(leaf, k, v, m)
+
+
+def test_fp32_table_in_a_captured_step():
+    """Forward and backward in one graph, replayed on new values of the table."""
+    q, k, v, table, dout = coherent(BF16)
+    leaf = table.float().requires_grad_(True)
+
+    def step():
+        out = relative_bias_attention(q, k, v, leaf)
+        return out.detach(), torch.autograd.grad(out, leaf, dout)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for shift in (0.5, -1.0):
+        with torch.no_grad():
+            leaf.add_(shift * torch.arange(32, device=DEV)[:, None] / 32)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+    assert got[1].dtype == torch.float32
+    sparse_attn_cuda.device_status()
