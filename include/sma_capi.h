@@ -303,7 +303,9 @@ SMA_API int sma_device_status(void* stream, int clear);
 
 /*
  * Upper bound, in nanoseconds, of every device-side wait in later launches
- * (default 2e9).  No reference counterpart.
+ * (default 2e9).  What a CTA that gave up has itself started (copies, matrix
+ * products) is waited for at least 2^31 ns, so that it lands before the CTA
+ * leaves.  No reference counterpart.
  */
 SMA_API int sma_set_wait_timeout_ns(uint64_t ns);
 
